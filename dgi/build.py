@@ -54,8 +54,10 @@ DEVICE_FLAGS = ["-munsafe-fp-atomics", "-Xclang", "-target-feature", "-Xclang", 
 # extension libraries: name -> (source folder, output).  "core" is every kernel of the Llama-family
 # runtime (dgi/_C.so); "mix" the mixer-block kernels of the per-layer-geometry models
 # (dgi/_C_mix.so: norms, q/k norm + rotary, masked attention, activations), which builds in
-# seconds so a model that needs only those does not wait for the big GEMM kernels.
-GROUPS = {"core": (CSRC, OUT), "mix": (os.path.join(CSRC, "mix"), os.path.join(HERE, "_C_mix.so"))}
+# seconds so a model that needs only those does not wait for the big GEMM kernels; "longctx" the
+# operators for long caches (dgi/_C_longctx.so: page bounds, page selection, selected and tree attention).
+GROUPS = {"core": (CSRC, OUT), "mix": (os.path.join(CSRC, "mix"), os.path.join(HERE, "_C_mix.so")),
+          "longctx": (os.path.join(CSRC, "longctx"), os.path.join(HERE, "_C_longctx.so"))}
 
 
 def build(verbose: bool = False, force: bool = False, group: str = "core") -> str:

@@ -1,0 +1,280 @@
+// dgi/csrc/longctx/bindings.cpp — torch.ops.dgi.* entries of the operators for long caches (dgi/_C_longctx.so): the append that keeps page
+// bounds, their rebuilding, page selection, attention over selected pages, attention of drafted trees.
+//
+// Operands are checked here, on the host, before any launch.  Launches go to the current stream of the operands' device, which is made
+// current for them; scratch memory comes from the caching allocator of that stream, a call's own.
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/core/GradMode.h>
+#include <c10/hip/HIPStream.h>
+#include <hip/hip_runtime.h>
+#include <torch/library.h>
+
+extern "C" {
+int dgi_rope_cache_bounds(const void* qkv, long long ld, int T, const int* positions, int max_pos, const float* cos_sin, int nh, int nkv,
+                          int hd, int rd, int mode, const int* slots, long long n_slots, void* q_out, void* k_cache, void* v_cache,
+                          void* bounds, int block_size, hipStream_t s);
+int dgi_page_bounds(const void* k_cache, void* bounds, const int* pages, const int* lens, int n, int num_blocks, int nkv, int hd,
+                    int block_size, hipStream_t s);
+int dgi_select_pages(const void* q, long long q_stride, const void* bounds, const int* tables, int table_stride, int table_cols, int n_seqs,
+                     int num_blocks, const int* ctx, const int* row_seq, int T, int nh, int nkv, int hd, int page, int count, int first,
+                     int recent, void* keys, int key_stride, int* out, hipStream_t s);
+int dgi_paged_selected(const void* q, long long q_stride, const void* k, const void* v, const int* tables, int table_stride, int table_cols,
+                       int n_seqs, int num_blocks, const int* ctx, const int* row_seq, const int* pages, int count, void* out,
+                       long long out_stride, float* part_o, float* part_l, int splits, int T, int nh, int nkv, int hd, int block_size,
+                       float scale, hipStream_t s);
+int dgi_tree_columns(int max_nodes, int G, int hd);
+int dgi_paged_tree(const void* q, long long q_stride, const void* k, const void* v, const int* tables, int table_stride, int table_cols,
+                   int n_seqs, int num_blocks, int rows, const int* cu, const int* ctx, const void* mask, int mask_stride, int max_nodes,
+                   void* out, long long out_stride, float* part_o, float* part_l, int splits, int min_part, int nh, int nkv, int hd,
+                   int block_size, float scale, hipStream_t s);
+}
+
+namespace {
+
+constexpr int64_t kInt = (1ll << 31) - 1;
+
+hipStream_t cur_stream() { return c10::hip::getCurrentHIPStream().stream(); }
+
+void check_rc(int rc, const char* what) {
+  TORCH_CHECK(rc == 0, "dgi kernel ", what, " failed with code ", rc,
+              rc > 0 ? (std::string(" (") + hipGetErrorString((hipError_t)rc) + ")") : std::string());
+}
+
+bool aligned(const at::Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
+
+// a bf16 operand on `dev` that starts on 16 bytes, and whose gradient nobody waits for
+void check_bf16(const at::Tensor& t, const at::Device& dev, const char* op, const char* name) {
+  TORCH_CHECK_VALUE(t.is_cuda() && t.device() == dev, op, ": ", name, " must be on the GPU of the other operands");
+  TORCH_CHECK_VALUE(t.scalar_type() == at::kBFloat16, op, ": ", name, " must be bfloat16");
+  TORCH_CHECK_VALUE(aligned(t), op, ": ", name, " must start on 16 bytes");
+  TORCH_CHECK_VALUE(!(t.requires_grad() && c10::GradMode::is_enabled()), op, ": no gradient goes through ", name);
+}
+
+void check_int(const at::Tensor& t, const at::Device& dev, at::ScalarType type, const char* op, const char* name) {
+  TORCH_CHECK_VALUE(t.is_cuda() && t.device() == dev, op, ": ", name, " must be on the GPU of the other operands");
+  TORCH_CHECK_VALUE(t.scalar_type() == type && t.is_contiguous(), op, ": ", name, " must be contiguous ", at::toString(type));
+}
+
+// rows of heads: [T, >= cols], any row stride that keeps 16 bytes
+void check_rows(const at::Tensor& t, int64_t cols, const at::Device& dev, const char* op, const char* name) {
+  check_bf16(t, dev, op, name);
+  TORCH_CHECK_VALUE(t.dim() == 2 && t.size(1) >= cols && (t.size(0) <= 1 || (t.stride(0) % 8 == 0 && t.stride(0) >= cols)) && t.stride(1) == 1,
+                    op, ": ", name, " must be rows of at least ", cols, " values, side by side, that start on 16 bytes");
+  TORCH_CHECK_VALUE(t.size(0) <= kInt, op, ": too many rows");
+}
+
+void check_heads(int64_t nh, int64_t nkv, int64_t hd, const char* op) {
+  TORCH_CHECK_VALUE(nkv > 0 && nh > 0 && nh % nkv == 0 && nh / nkv <= 16, op, ": heads must be 1 to 16 for each kv head");
+  TORCH_CHECK_VALUE(hd == 64 || hd == 128 || hd == 256, op, ": heads of 64, 128 or 256 dims");
+}
+
+void check_cache(const at::Tensor& c, int64_t nkv, const at::Device& dev, const char* op, const char* name) {
+  check_bf16(c, dev, op, name);
+  TORCH_CHECK_VALUE(c.dim() == 4 && c.is_contiguous() && c.size(0) > 0 && c.size(0) <= kInt && c.size(1) == nkv && c.size(2) > 0 &&
+                        c.size(2) <= (1 << 20),
+                    op, ": ", name, " must be contiguous [blocks, kv heads, block size, dims]");
+}
+
+void check_bounds(const at::Tensor& b, int64_t nkv, int64_t hd, const at::Device& dev, const char* op) {
+  check_bf16(b, dev, op, "bounds");
+  TORCH_CHECK_VALUE(b.dim() == 4 && b.is_contiguous() && b.size(0) > 0 && b.size(0) <= kInt && b.size(1) == nkv && b.size(2) == 2 &&
+                        b.size(3) == hd,
+                    op, ": bounds must be contiguous [blocks, kv heads, 2, dims]");
+}
+
+void check_tables(const at::Tensor& t, const at::Device& dev, const char* op) {
+  check_int(t, dev, at::kInt, op, "block_tables");
+  TORCH_CHECK_VALUE(t.dim() == 2 && t.size(0) <= kInt && t.size(1) <= kInt, op, ": block_tables must be [sequences, pages]");
+}
+
+const int* rows_of(const c10::optional<at::Tensor>& row_seq, const at::Tensor& tables, int64_t T, const at::Device& dev, const char* op) {
+  if (!row_seq.has_value()) {
+    TORCH_CHECK_VALUE(tables.size(0) >= T, op, ": block_tables must have a row for each row of q (or row_seq says which)");
+    return nullptr;
+  }
+  check_int(*row_seq, dev, at::kInt, op, "row_seq");
+  TORCH_CHECK_VALUE(row_seq->numel() == T, op, ": row_seq must have a number for each row of q");
+  return row_seq->data_ptr<int>();
+}
+
+void rope_cache_bounds(at::Tensor q_out, const at::Tensor& qkv, const at::Tensor& positions, const at::Tensor& cos_sin, int64_t nh,
+                       int64_t nkv, int64_t hd, const at::Tensor& slots, at::Tensor k_cache, at::Tensor v_cache, at::Tensor bounds,
+                       int64_t mode) {
+  const char* op = "rope_cache_bounds";
+  const at::Device dev = qkv.device();
+  check_heads(nh, nkv, hd, op);
+  check_rows(qkv, (nh + 2 * nkv) * hd, dev, op, "qkv");
+  check_cache(k_cache, nkv, dev, op, "k_cache");
+  check_cache(v_cache, nkv, dev, op, "v_cache");
+  check_bounds(bounds, nkv, hd, dev, op);
+  TORCH_CHECK_VALUE(k_cache.size(3) == hd && k_cache.sizes() == v_cache.sizes() && bounds.size(0) == k_cache.size(0), op,
+                    ": k_cache, v_cache and bounds must have the same blocks and dims");
+  const int64_t T = qkv.size(0);
+  check_int(positions, dev, at::kInt, op, "positions");
+  check_int(slots, dev, at::kInt, op, "slot_mapping");
+  TORCH_CHECK_VALUE(positions.numel() == T && slots.numel() == T, op, ": positions and slot_mapping must have a number for each row");
+  TORCH_CHECK_VALUE(cos_sin.is_cuda() && cos_sin.device() == dev && cos_sin.scalar_type() == at::kFloat && cos_sin.is_contiguous() &&
+                        cos_sin.dim() == 2 && cos_sin.size(0) > 0 && cos_sin.size(0) <= kInt && aligned(cos_sin),
+                    op, ": cos_sin must be contiguous fp32 [positions, rotated dims]");
+  const int64_t rd = cos_sin.size(1);
+  TORCH_CHECK_VALUE(mode == 0 || mode == 1, op, ": mode is 0 (halves) or 1 (interleaved pairs)");
+  TORCH_CHECK_VALUE(rd > 0 && rd <= hd && rd % (mode == 0 ? 16 : 8) == 0, op, ": rotated dims must be a multiple of ", mode == 0 ? 16 : 8,
+                    " and at most the head's");
+  check_rows(q_out, nh * hd, dev, op, "out");
+  TORCH_CHECK_VALUE(q_out.is_contiguous() && q_out.size(0) == T && q_out.size(1) == nh * hd, op, ": out must be contiguous [rows, heads * dims]");
+  const c10::DeviceGuard guard(dev);
+  check_rc(dgi_rope_cache_bounds(qkv.data_ptr(), qkv.stride(0), (int)T, positions.data_ptr<int>(), (int)cos_sin.size(0),
+                                 cos_sin.data_ptr<float>(), (int)nh, (int)nkv, (int)hd, (int)rd, (int)mode, slots.data_ptr<int>(),
+                                 k_cache.size(0) * k_cache.size(2), q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                                 bounds.data_ptr(), (int)k_cache.size(2), cur_stream()), op);
+}
+
+void page_bounds(const at::Tensor& k_cache, at::Tensor bounds, const at::Tensor& pages, const at::Tensor& lens) {
+  const char* op = "page_bounds";
+  const at::Device dev = k_cache.device();
+  TORCH_CHECK_VALUE(k_cache.dim() == 4, op, ": k_cache must be contiguous [blocks, kv heads, block size, dims]");
+  const int64_t nkv = k_cache.size(1), hd = k_cache.size(3);
+  check_cache(k_cache, nkv, dev, op, "k_cache");
+  check_heads(nkv, nkv, hd, op);
+  check_bounds(bounds, nkv, hd, dev, op);
+  TORCH_CHECK_VALUE(bounds.size(0) == k_cache.size(0), op, ": bounds must have the cache's blocks");
+  check_int(pages, dev, at::kInt, op, "pages");
+  check_int(lens, dev, at::kInt, op, "lens");
+  TORCH_CHECK_VALUE(pages.numel() == lens.numel() && pages.numel() <= kInt / nkv, op, ": pages and lens must be as many");
+  const c10::DeviceGuard guard(dev);
+  check_rc(dgi_page_bounds(k_cache.data_ptr(), bounds.data_ptr(), pages.data_ptr<int>(), lens.data_ptr<int>(), (int)pages.numel(),
+                           (int)k_cache.size(0), (int)nkv, (int)hd, (int)k_cache.size(2), cur_stream()), op);
+}
+
+void select_pages(at::Tensor out, const at::Tensor& q, const at::Tensor& bounds, const at::Tensor& tables, const at::Tensor& ctx, int64_t nh,
+                  int64_t nkv, int64_t page, int64_t first, int64_t recent, const c10::optional<at::Tensor>& row_seq) {
+  const char* op = "select_pages";
+  const at::Device dev = q.device();
+  TORCH_CHECK_VALUE(bounds.dim() == 4, op, ": bounds must be contiguous [blocks, kv heads, 2, dims]");
+  const int64_t hd = bounds.size(3), T = q.size(0);
+  check_heads(nh, nkv, hd, op);
+  check_rows(q, nh * hd, dev, op, "q");
+  check_bounds(bounds, nkv, hd, dev, op);
+  check_tables(tables, dev, op);
+  check_int(ctx, dev, at::kInt, op, "context_lens");
+  TORCH_CHECK_VALUE(ctx.numel() == T, op, ": context_lens must have a number for each row of q");
+  check_int(out, dev, at::kInt, op, "out");
+  TORCH_CHECK_VALUE(out.dim() == 3 && out.size(0) == T && out.size(1) == nkv, op, ": out must be [rows, kv heads, count]");
+  const int64_t count = out.size(2);
+  TORCH_CHECK_VALUE(page > 0 && page <= (1 << 20), op, ": a page has 1 to 2^20 tokens");
+  TORCH_CHECK_VALUE(first >= 0 && recent >= 1 && first + recent <= count, op, ": first >= 0, recent >= 1 and both within count");
+  const int* rows = rows_of(row_seq, tables, T, dev, op);
+  TORCH_CHECK_VALUE(T <= kInt / nkv && tables.size(1) <= (1 << 24), op, ": too many rows or pages");
+  const c10::DeviceGuard guard(dev);
+  const int64_t stride = tables.size(1);
+  const at::Tensor keys = at::empty({stride > count ? T * nkv * stride : 0}, q.options().dtype(at::kLong));
+  check_rc(dgi_select_pages(q.data_ptr(), q.stride(0), bounds.data_ptr(), tables.data_ptr<int>(), (int)tables.stride(0), (int)tables.size(1),
+                            (int)tables.size(0), (int)bounds.size(0), ctx.data_ptr<int>(), rows, (int)T, (int)nh, (int)nkv, (int)hd,
+                            (int)page, (int)count, (int)first, (int)recent, keys.data_ptr(), (int)stride, out.data_ptr<int>(), cur_stream()), op);
+}
+
+struct Attention {
+  int64_t hd, page;
+  at::Device dev;
+};
+
+Attention check_attention(const at::Tensor& out, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& tables,
+                          int64_t nh, int64_t nkv, const char* op) {
+  const at::Device dev = q.device();
+  TORCH_CHECK_VALUE(k.dim() == 4, op, ": k_cache must be contiguous [blocks, kv heads, block size, dims]");
+  const int64_t hd = k.size(3), page = k.size(2);
+  check_heads(nh, nkv, hd, op);
+  check_cache(k, nkv, dev, op, "k_cache");
+  check_cache(v, nkv, dev, op, "v_cache");
+  TORCH_CHECK_VALUE(k.sizes() == v.sizes(), op, ": k_cache and v_cache must be alike");
+  TORCH_CHECK_VALUE((page & (page - 1)) == 0, op, ": pages of a power of two");
+  check_rows(q, nh * hd, dev, op, "q");
+  check_rows(out, nh * hd, dev, op, "out");
+  TORCH_CHECK_VALUE(out.size(0) == q.size(0), op, ": out must have the rows of q");
+  check_tables(tables, dev, op);
+  TORCH_CHECK_VALUE(tables.size(1) <= (1 << 30) / page, op, ": a table has at most 2^30 tokens");
+  return {hd, page, dev};
+}
+
+void paged_selected(at::Tensor out, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& tables,
+                    const at::Tensor& ctx, const at::Tensor& pages, int64_t nh, int64_t nkv, double scale,
+                    const c10::optional<at::Tensor>& row_seq) {
+  const char* op = "paged_selected";
+  const Attention at_ = check_attention(out, q, k, v, tables, nh, nkv, op);
+  const int64_t T = q.size(0);
+  check_int(ctx, at_.dev, at::kInt, op, "context_lens");
+  TORCH_CHECK_VALUE(ctx.numel() == T, op, ": context_lens must have a number for each row of q");
+  check_int(pages, at_.dev, at::kInt, op, "pages");
+  TORCH_CHECK_VALUE(pages.dim() == 3 && pages.size(0) == T && pages.size(1) == nkv && pages.size(2) > 0 && pages.size(2) <= (1 << 24), op,
+                    ": pages must be [rows, kv heads, count]");
+  const int* rows = rows_of(row_seq, tables, T, at_.dev, op);
+  const int64_t count = pages.size(2);
+  TORCH_CHECK_VALUE(T <= kInt / nkv, op, ": too many rows");
+  const c10::DeviceGuard guard(at_.dev);
+  // runs of 256 keys at the least, as many as give the card two workgroups a compute unit
+  const int64_t least = std::max<int64_t>(1, 256 / at_.page);
+  const int64_t splits = std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(1, T * nkv), (count + least - 1) / least, 64}));
+  at::Tensor part_o, part_l;
+  if (splits > 1) {
+    part_o = at::empty({T * nkv * splits * 16 * at_.hd}, q.options().dtype(at::kFloat));
+    part_l = at::empty({T * nkv * splits * 16}, q.options().dtype(at::kFloat));
+  }
+  check_rc(dgi_paged_selected(q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(), tables.data_ptr<int>(), (int)tables.stride(0),
+                              (int)tables.size(1), (int)tables.size(0), (int)k.size(0), ctx.data_ptr<int>(), rows, pages.data_ptr<int>(),
+                              (int)count, out.data_ptr(), out.stride(0), splits > 1 ? part_o.data_ptr<float>() : nullptr,
+                              splits > 1 ? part_l.data_ptr<float>() : nullptr, (int)splits, (int)T, (int)nh, (int)nkv, (int)at_.hd,
+                              (int)at_.page, (float)scale, cur_stream()), op);
+}
+
+void paged_tree(at::Tensor out, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& tables,
+                const at::Tensor& cu, const at::Tensor& ctx, const at::Tensor& mask, int64_t nh, int64_t nkv, double scale,
+                int64_t max_nodes) {
+  const char* op = "paged_tree";
+  const Attention at_ = check_attention(out, q, k, v, tables, nh, nkv, op);
+  check_int(ctx, at_.dev, at::kInt, op, "context_lens");
+  const int64_t S = ctx.numel();
+  check_int(cu, at_.dev, at::kInt, op, "cu_seqlens_q");
+  TORCH_CHECK_VALUE(cu.numel() == S + 1 && tables.size(0) >= S, op, ": cu_seqlens_q must have one number more than context_lens, block_tables as many rows");
+  check_int(mask, at_.dev, at::kLong, op, "tree_mask");
+  TORCH_CHECK_VALUE(max_nodes >= 1 && max_nodes <= 64, op, ": trees of 1 to 64 nodes");
+  TORCH_CHECK_VALUE(mask.dim() == 2 && mask.size(0) >= S && mask.size(1) >= max_nodes && mask.size(1) <= kInt, op,
+                    ": tree_mask must be [sequences, nodes]");
+  const c10::DeviceGuard guard(at_.dev);
+  const int64_t G = nh / nkv, cols = dgi_tree_columns((int)max_nodes, (int)G, (int)at_.hd), tiles = (max_nodes * G + cols - 1) / cols;
+  TORCH_CHECK_VALUE(S <= kInt / (nkv * tiles), op, ": too many sequences");
+  const int64_t items = S * tiles * nkv, min_part = 128;
+  const int64_t splits = std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(1, items), (tables.size(1) * at_.page + min_part - 1) / min_part, 64}));
+  at::Tensor part_o, part_l;
+  if (splits > 1) {
+    part_o = at::empty({items * splits * cols * at_.hd}, q.options().dtype(at::kFloat));
+    part_l = at::empty({items * splits * cols}, q.options().dtype(at::kFloat));
+  }
+  check_rc(dgi_paged_tree(q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(), tables.data_ptr<int>(), (int)tables.stride(0),
+                          (int)tables.size(1), (int)S, (int)k.size(0), (int)q.size(0), cu.data_ptr<int>(), ctx.data_ptr<int>(),
+                          mask.data_ptr(), (int)mask.stride(0), (int)max_nodes, out.data_ptr(), out.stride(0),
+                          splits > 1 ? part_o.data_ptr<float>() : nullptr, splits > 1 ? part_l.data_ptr<float>() : nullptr, (int)splits,
+                          (int)min_part, (int)nh, (int)nkv, (int)at_.hd, (int)at_.page, (float)scale, cur_stream()), op);
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(dgi, m) {
+  m.def("rope_cache_bounds(Tensor(a!) out, Tensor qkv, Tensor positions, Tensor cos_sin, int nh, int nkv, int hd, Tensor slot_mapping, "
+        "Tensor(b!) k_cache, Tensor(c!) v_cache, Tensor(d!) bounds, int mode) -> ()");
+  m.def("page_bounds(Tensor k_cache, Tensor(a!) bounds, Tensor pages, Tensor lens) -> ()");
+  m.def("select_pages(Tensor(a!) out, Tensor q, Tensor bounds, Tensor block_tables, Tensor context_lens, int nh, int nkv, int page, int first, "
+        "int recent, Tensor? row_seq) -> ()");
+  m.def("paged_selected(Tensor(a!) out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, Tensor context_lens, Tensor pages, "
+        "int nh, int nkv, float scale, Tensor? row_seq) -> ()");
+  m.def("paged_tree(Tensor(a!) out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, Tensor cu_seqlens_q, Tensor context_lens, "
+        "Tensor tree_mask, int nh, int nkv, float scale, int max_nodes) -> ()");
+}
+
+TORCH_LIBRARY_IMPL(dgi, CUDA, m) {
+  m.impl("rope_cache_bounds", &rope_cache_bounds);
+  m.impl("page_bounds", &page_bounds);
+  m.impl("select_pages", &select_pages);
+  m.impl("paged_selected", &paged_selected);
+  m.impl("paged_tree", &paged_tree);
+}

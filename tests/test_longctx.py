@@ -1,0 +1,798 @@
+"""Operators for long caches (``dgi.ops.longctx``) against a plain implementation in 64 bits, on the CPU's reference path and (``gpu``) on
+the HIP kernels: layouts, lengths from none to long ones, pages that end inside a tile, rows that see nothing, values that are no numbers
+in places that nobody sees, refusals, graphs, streams.
+
+Tolerances count roundings.  A bf16 result is off by at most 2^-8 of itself; attention weights rounded to bf16 put at most
+2^-8 of A = sum p |v| / sum p on top; a score is a sum of hd products in fp32, off by at most d = (hd + 4) 2^-24 scale max |q| . |k|, which puts
+2 d on each weight and its sum; exp2 and the sums over n keys take (n + 16) 2^-24 of A.
+"""
+import math
+
+import pytest
+import torch
+
+from dgi import ops
+from dgi.ops import longctx
+
+gpu = pytest.mark.gpu
+BF16, F64, I32 = torch.bfloat16, torch.float64, torch.int32
+U8, U24 = 2.0 ** -8, 2.0 ** -24
+
+
+@pytest.fixture(params=["cpu", pytest.param("cuda", marks=gpu)])
+def dev(request):
+    if request.param == "cuda":
+        longctx.load_native(required=True)
+    return request.param
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _randn(g, *shape, scale=1.0, dev="cpu", dtype=BF16):
+    return (torch.randn(*shape, generator=g) * scale).to(dtype).to(dev)
+
+
+def _tables(g, need, cols, pool, dev):
+    """Shuffled page ids for sequences of ``need`` pages each."""
+    ids = torch.randperm(pool, generator=g)[: sum(need)].to(I32)
+    t = torch.full((len(need), cols), -1, dtype=I32)
+    at = 0
+    for i, n in enumerate(need):
+        t[i, :n] = ids[at:at + n]
+        at += n
+    return t.to(dev)
+
+
+def _close(got, want, tol, what=""):
+    got, want, tol = got.double().cpu(), want.double().cpu(), tol.double().cpu()
+    bad = ~((got - want).abs() <= tol) & ~((got == want) | (got.isnan() & want.isnan()))
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {float(((got - want).abs() / tol)[bad].max())} of its tolerance"
+
+
+def _attention(q, k, v, scale):
+    """q [G, hd] over k, v [n, hd] in 64 bits, and the tolerance."""
+    if k.shape[0] == 0:
+        return torch.zeros_like(q, dtype=F64), torch.zeros_like(q, dtype=F64)
+    q, k, v = q.double(), k.double(), v.double()
+    p = torch.softmax(q @ k.t() * scale, -1)
+    o, a = p @ v, p @ v.abs()
+    d = (q.shape[1] + 4) * U24 * abs(scale) * float((q.abs() @ k.abs().t()).max())
+    return o, U8 * o.abs() + (U8 + 4 * d + (k.shape[0] + 16) * U24) * a + 1e-30
+
+
+# ---- the append -------------------------------------------------------------------------------------------------------------------------
+
+def _rotate64(x, cs, mode):
+    """x [T, heads, hd] rotated in 64 bits, and the size of what is added up."""
+    x, cs = x.double(), cs.double()
+    y, size = x.clone(), x.abs()
+    half = cs.shape[1] // 2
+    for i in range(half):
+        a, b = (i, i + half) if mode == 0 else (2 * i, 2 * i + 1)
+        c, s = cs[:, i, None], cs[:, half + i, None]
+        y[..., a], y[..., b] = x[..., a] * c - x[..., b] * s, x[..., b] * c + x[..., a] * s
+        size[..., a] = size[..., b] = x[..., a].abs() + x[..., b].abs()
+    return y, size
+
+
+def _append_case(dev, nh, nkv, hd, rd, mode, page, spans, extra=0, seed=0, pool=None):
+    """Portions ``spans`` = (first position, rows) of sequences whose pages hold what came before."""
+    g = _gen(seed)
+    need = [(p + n + page - 1) // page for p, n in spans]
+    pool = pool or sum(need) + 5
+    tables = _tables(g, need, max(need), pool, "cpu")
+    pos = torch.cat([torch.arange(p, p + n) for p, n in spans]).to(I32)
+    slots = torch.cat([tables[i, torch.arange(p, p + n) // page] * page + torch.arange(p, p + n) % page for i, (p, n) in enumerate(spans)]).to(I32)
+    k, v = _randn(g, pool, nkv, page, hd), _randn(g, pool, nkv, page, hd)
+    bounds = torch.stack([k.amin(2), k.amax(2)], 2) * 0.25      # narrow, so that keys of this step widen them
+    qkv = _randn(g, len(pos), (nh + 2 * nkv) * hd + extra)
+    cs = ops.rope_cos_sin(rd, int(pos.max()) + 3, 10000.0)
+    return [x.to(dev) for x in (qkv, pos, cs, slots, k, v, bounds)]
+
+
+def _append_check(dev, nh, nkv, hd, mode, page, case):
+    qkv, pos, cs, slots, k, v, bounds = case
+    k0, v0, b0, qkv0 = k.clone(), v.clone(), bounds.clone(), qkv.clone()
+    q = longctx.rope_cache_bounds(qkv, pos, cs, nh, nkv, hd, slots, k, v, bounds, mode)
+    T = qkv.shape[0]
+    assert torch.equal(qkv, qkv0)
+    rows = qkv[:, : (nh + 2 * nkv) * hd].reshape(T, nh + 2 * nkv, hd).cpu()
+    want, size = _rotate64(rows[:, : nh + nkv], cs.cpu()[pos.cpu().long()], mode)
+    tol = (U8 + 4 * U24) * want.abs() + 4 * U24 * size      # two products, a sum, each rounded, then bf16
+    _close(q.view(T, nh, hd), want[:, :nh], tol[:, :nh], "q")
+    k, v, bounds, k0, v0, b0 = (x.cpu() for x in (k, v, bounds, k0, v0, b0))
+    for t, s in enumerate(slots.tolist()):
+        if s < 0:
+            continue
+        at, off = s // page, s % page
+        _close(k[at, :, off], want[t, nh:], tol[t, nh:], "k")
+        assert torch.equal(v[at, :, off], rows[t, nh + nkv:])
+        k0[at, :, off], v0[at, :, off] = k[at, :, off], v[at, :, off]
+        if off == 0:
+            b0[at, :, 0], b0[at, :, 1] = k[at, :, 0], k[at, :, 0]
+        else:
+            b0[at, :, 0], b0[at, :, 1] = torch.minimum(b0[at, :, 0], k[at, :, off]), torch.maximum(b0[at, :, 1], k[at, :, off])
+    assert torch.equal(k, k0) and torch.equal(v, v0)      # nothing else is written
+    assert torch.equal(bounds, b0)                        # a minimum rounds nothing
+
+
+@pytest.mark.parametrize("nh,nkv,hd,rd,mode", [(8, 2, 64, 64, 0), (4, 4, 128, 128, 0), (16, 1, 128, 64, 1), (14, 2, 64, 16, 0), (7, 1, 256, 128, 0),
+                                               (6, 3, 64, 8, 1)])
+@pytest.mark.parametrize("page", [16, 8, 12])
+def test_append(dev, nh, nkv, hd, rd, mode, page):
+    """Decode rows at a page's first, middle and last slot, portions within a page, across pages, and of whole ones."""
+    spans = [(0, 1), (page - 1, 1), (page, 1), (5, 1), (0, page), (3, 2), (2, 3 * page + 1), (page, 2 * page)]
+    _append_check(dev, nh, nkv, hd, mode, page, _append_case(dev, nh, nkv, hd, rd, mode, page, spans))
+
+
+def test_append_strided_rows_and_rows_without_a_slot(dev):
+    case = _append_case(dev, 8, 2, 64, 64, 0, 16, [(3, 20), (16, 1), (30, 4)], extra=72)
+    case[3][[1, 20, 24]] = -1      # inside a portion, a decode row, the last row
+    _append_check(dev, 8, 2, 64, 0, 16, case)
+    case = _append_case(dev, 8, 2, 64, 64, 0, 16, [(3, 20)])
+    case[0] = case[0].repeat_interleave(2, 0)[::2]      # every other row of a buffer
+    _append_check(dev, 8, 2, 64, 0, 16, case)
+
+
+def test_append_no_rows_one_row_many_rows(dev):
+    for spans in ([(0, 1)], [(100, 1)] * 37, [(7, 700)]):
+        _append_check(dev, 8, 2, 64, 0, 16, _append_case(dev, 8, 2, 64, 64, 0, 16, spans))
+    case = _append_case(dev, 8, 2, 64, 64, 0, 16, [(0, 1)])
+    case[0], case[1], case[3] = case[0][:0], case[1][:0], case[3][:0]
+    _append_check(dev, 8, 2, 64, 0, 16, case)
+
+
+def test_append_keeps_what_is_no_number(dev):
+    """A key that is no number makes its channel's bounds no number until the page starts anew; infinities bound."""
+    case = _append_case(dev, 2, 1, 64, 64, 0, 16, [(3, 4)])
+    qkv, pos, cs, slots, k, v, bounds = case
+    qkv[1, 2 * 64 + 5] = math.nan
+    qkv[2, 2 * 64 + 60] = math.inf
+    longctx.rope_cache_bounds(qkv, pos, cs, 2, 1, 64, slots, k, v, bounds)
+    b = bounds[int(slots[0]) // 16, 0].float()
+    assert b[:, [5, 37]].isnan().all() and not b[:, [4, 36]].isnan().any()
+    assert torch.isinf(b[:, [60, 28]]).any(0).all()
+
+
+@pytest.mark.parametrize("nkv,hd,page", [(1, 64, 16), (8, 128, 16), (3, 256, 32), (2, 128, 5), (2, 64, 128)])
+def test_page_bounds(dev, nkv, hd, page):
+    g = _gen(1)
+    nb = 41
+    k = _randn(g, nb, nkv, page, hd)
+    k[7, 0, 2, 3] = math.nan
+    k[9, nkv - 1, 0, 1] = -math.inf
+    pages = torch.randperm(nb, generator=g)[:30].to(I32)
+    pages[:2] = torch.tensor([7, 9], dtype=I32)
+    pages = torch.tensor(list(dict.fromkeys(pages.tolist())) + [-1, nb, nb + 100], dtype=I32)
+    lens = torch.randint(0, page + 1, (len(pages),), generator=g).to(I32)
+    lens[:6] = torch.tensor([page, page, 0, 1, page + 3, -1], dtype=I32)      # clamped to the page
+    bounds = longctx.empty_bounds(k.to(dev))
+    old = bounds.cpu().clone()
+    longctx.page_bounds(k.to(dev), bounds, pages.to(dev), lens.to(dev))
+    for p, n in zip(pages.tolist(), lens.tolist()):
+        if 0 <= p < nb and n > 0:
+            old[p, :, 0], old[p, :, 1] = k[p, :, : min(n, page)].amin(1), k[p, :, : min(n, page)].amax(1)
+    assert torch.equal(bounds.cpu().isnan(), old.isnan())
+    assert torch.equal(bounds.cpu().nan_to_num(7.0), old.nan_to_num(7.0))
+    longctx.page_bounds(k.to(dev), bounds, pages[:0].to(dev), lens[:0].to(dev))
+
+
+# ---- the selection ----------------------------------------------------------------------------------------------------------------------
+
+def _selection64(q, bounds, tables, ctx, nh, nkv, page, count, first, recent, seq):
+    """By sorting, page by page, from the definition: what a key within the bounds can give each head at most."""
+    out = torch.full((q.shape[0], nkv, count), -1, dtype=I32)
+    hd = bounds.shape[-1]
+    for t in range(q.shape[0]):
+        n = min(-(-int(ctx[t]) // page), tables.shape[1])
+        for h in range(nkv):
+            x = q[t, : nh * hd].double().view(nkv, -1, hd)[h]
+            if n <= count:
+                keep = list(range(max(n, 0)))
+            else:
+                b = bounds[tables[int(seq[t]), :n].long(), h].double()
+                most = sum(torch.where(x[i] > 0, x[i] * b[:, 1], x[i] * b[:, 0]).sum(-1) for i in range(x.shape[0]))
+                most = torch.where(most.isnan(), -math.inf, most).tolist()
+                forced = list(range(first)) + list(range(n - recent, n))
+                rest = sorted(range(first, n - recent), key=lambda p: (-most[p], p))[: count - first - recent]
+                keep = sorted(forced + rest)
+            out[t, h, : len(keep)] = torch.tensor(keep, dtype=I32)
+    return out
+
+
+def _select_case(nh, nkv, hd, page, lens, rows, seed=0, whole=False, extra=0):
+    """``rows`` rows at the end of each sequence of ``lens`` tokens; ``whole``: small whole numbers, so that many scores are alike."""
+    g = _gen(seed)
+    need = [-(-n // page) for n in lens]
+    pool = sum(need) + 3
+    tables = _tables(g, need, max(need) + 2, pool, "cpu")
+    if whole:
+        b = torch.randint(-1, 2, (pool, nkv, 2, hd), generator=g).to(BF16).sort(2).values
+        q = torch.randint(-1, 2, (len(lens) * rows, nh * hd + extra), generator=g).to(BF16)
+    else:
+        b = _randn(g, pool, nkv, 2, hd).sort(2).values
+        q = _randn(g, len(lens) * rows, nh * hd + extra)
+    ctx = torch.cat([torch.arange(n - rows + 1, n + 1) for n in lens]).to(I32)
+    seq = torch.arange(len(lens), dtype=I32).repeat_interleave(rows)
+    return q, b, tables, ctx, seq
+
+
+def _select_check(dev, nh, nkv, page, count, first, recent, q, b, tables, ctx, seq):
+    got = longctx.select_pages(q.to(dev), b.to(dev), tables.to(dev), ctx.to(dev), nh, nkv, page, count, first, recent, row_seq=seq.to(dev))
+    assert got.dtype == I32
+    assert torch.equal(got.cpu(), _selection64(q, b, tables, ctx, nh, nkv, page, count, first, recent, seq))
+
+
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 64), (7, 1, 128), (16, 1, 64), (4, 4, 256)])
+@pytest.mark.parametrize("count,first,recent", [(8, 1, 2), (5, 0, 1), (3, 1, 2), (1, 0, 1), (64, 1, 1)])
+def test_select(dev, nh, nkv, hd, count, first, recent):
+    """Contexts of one token, of exactly ``count`` pages, of one page more, of many."""
+    lens = [1, 16 * count, 16 * count + 1, 16 * count + 17, 700, 1601]
+    _select_check(dev, nh, nkv, 16, count, first, recent, *_select_case(nh, nkv, hd, 16, lens, 1))
+
+
+@pytest.mark.parametrize("rows,page,extra", [(37, 16, 0), (5, 64, 64), (64, 16, 8), (130, 32, 0)])
+def test_select_rows_of_prompts(dev, rows, page, extra):
+    """Rows that follow each other see one key more each; their sequence's table is given by ``row_seq``."""
+    _select_check(dev, 8, 2, page, 6, 1, 2, *_select_case(8, 2, 64, page, [max(rows, 300), max(rows, 900), 1777], rows, extra=extra))
+
+
+@pytest.mark.parametrize("lens", [[400, 1000, 2222], [40000]])
+def test_select_alike_pages_go_to_the_lowest(dev, lens):
+    _select_check(dev, 4, 2, 16, 12, 1, 1, *_select_case(4, 2, 64, 16, lens, 1, whole=True))
+    q, b, tables, ctx, seq = _select_case(4, 2, 64, 16, lens, 1, whole=True)
+    _select_check(dev, 4, 2, 16, 12, 1, 1, q * 0, b, tables, ctx, seq)      # all alike, zeros of both signs
+
+
+def test_select_close_scores(dev):
+    """Pages whose scores differ in the last bits of 64: one channel of the bounds is a little larger."""
+    q, b, tables, ctx, seq = _select_case(4, 1, 128, 16, [3000], 1)
+    b[:] = b[:1]
+    b[:, 0, 1, 17] += (torch.randperm(b.shape[0], generator=_gen(3)) % 5).to(BF16) * 2.0 ** -6
+    q[:, 17::128] = 2.0 ** -30
+    _select_check(dev, 4, 1, 16, 40, 1, 1, q, b, tables, ctx, seq)
+
+
+def test_select_values_that_are_no_numbers(dev):
+    q, b, tables, ctx, seq = _select_case(4, 2, 64, 16, [900, 900, 900, 900], 1)
+    b[tables[0, 7], 0, 1, 3] = math.nan
+    b[tables[0, 9], 1] = torch.tensor([math.inf, -math.inf], dtype=BF16)[:, None]      # bounds of a page without keys
+    b[tables[1, 11], :, 1, 5] = math.inf
+    b[tables[1, 12], :, 0, 5] = -math.inf
+    q[2, 70] = math.nan
+    q[3, 70] = math.inf
+    _select_check(dev, 4, 2, 16, 8, 1, 1, q, b, tables, ctx, seq)
+
+
+def test_select_empty_rows_and_unknown_pages(dev):
+    q, b, tables, ctx, seq = _select_case(4, 2, 64, 16, [900, 900, 500], 1)
+    ctx[1] = 0
+    got = longctx.select_pages(q.to(dev), b.to(dev), tables.to(dev), ctx.to(dev), 4, 2, 16, 8).cpu()
+    assert (got[1] == -1).all()
+    tables[0, [5, 6]] = torch.tensor([-1, 1 << 30], dtype=I32)      # never read, never preferred
+    got = longctx.select_pages(q.to(dev), b.to(dev), tables.to(dev), ctx.to(dev), 4, 2, 16, 54, row_seq=seq.to(dev)).cpu()
+    assert not torch.isin(got[0], torch.tensor([5, 6], dtype=I32)).any() and (got[0] >= 0).all()
+    ctx[0] = 1 << 30      # more than the table has: its pages are all there are
+    got = longctx.select_pages(q.to(dev), b.to(dev), tables.to(dev), ctx.to(dev), 4, 2, 16, 8).cpu()
+    assert (got[0] < tables.shape[1]).all() and (got[0].diff() > 0).all()
+    assert longctx.select_pages(q[:0].to(dev), b.to(dev), tables.to(dev), ctx[:0].to(dev), 4, 2, 16, 8).shape == (0, 2, 8)
+
+
+# ---- attention over selected pages ------------------------------------------------------------------------------------------------------
+
+def _selected_case(nh, nkv, hd, page, lens, count, rows=1, seed=0, extra=0):
+    g = _gen(seed)
+    need = [-(-max(n, 1) // page) for n in lens]
+    pool = sum(need) + 3
+    tables = _tables(g, need, max(need), pool, "cpu")
+    k, v = _randn(g, pool, nkv, page, hd), _randn(g, pool, nkv, page, hd)
+    q = _randn(g, len(lens) * rows, nh * hd + extra)
+    ctx = torch.cat([torch.arange(n - rows + 1, n + 1) for n in lens]).to(I32)
+    seq = torch.arange(len(lens), dtype=I32).repeat_interleave(rows)
+    pages = torch.full((q.shape[0], nkv, count), -1, dtype=I32)
+    for t in range(q.shape[0]):
+        n = -(-int(ctx[t]) // page)
+        for h in range(nkv):
+            some = torch.randperm(n, generator=g)[:count].sort().values if n > 0 else torch.empty(0, dtype=torch.long)
+            pages[t, h, : len(some)] = some.to(I32)
+            if n > 0:
+                pages[t, h, max(len(some) - 1, 0)] = n - 1      # the page that is not full
+    return q, k, v, tables, ctx, pages, seq
+
+
+def _selected_want(nh, nkv, scale, q, k, v, tables, ctx, pages, seq):
+    T, page, hd, G = q.shape[0], k.shape[2], k.shape[3], nh // nkv
+    o, tol = torch.zeros(T, nkv, G, hd, dtype=F64), torch.zeros(T, nkv, G, hd, dtype=F64)
+    for t in range(T):
+        for h in range(nkv):
+            kk = [k[tables[seq[t], p], h, : int(ctx[t]) - p * page] for p in pages[t, h].tolist() if 0 <= p * page < int(ctx[t])]
+            vv = [v[tables[seq[t], p], h, : int(ctx[t]) - p * page] for p in pages[t, h].tolist() if 0 <= p * page < int(ctx[t])]
+            x = q[t, : nh * hd].view(nkv, G, hd)[h]
+            o[t, h], tol[t, h] = _attention(x, torch.cat(kk) if kk else k[0, 0, :0], torch.cat(vv) if vv else v[0, 0, :0], scale)
+    return o.view(T, -1), tol.view(T, -1)
+
+
+def _selected_check(dev, nh, nkv, case, scale=None, **kw):
+    scale = scale if scale is not None else case[1].shape[-1] ** -0.5
+    q, k, v, tables, ctx, pages, seq = (x.to(dev) for x in case)
+    got = longctx.paged_selected(q, k, v, tables, ctx, pages, nh, nkv, scale, row_seq=seq, **kw)
+    want, tol = _selected_want(nh, nkv, scale, *case)
+    _close(got[:, : want.shape[1]], want, tol)
+    return got
+
+
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 64), (7, 1, 128), (16, 1, 128), (4, 4, 256), (3, 3, 64)])
+@pytest.mark.parametrize("page", [16, 8, 64])
+def test_selected(dev, nh, nkv, hd, page):
+    """Contexts of one token up to many pages, lists shorter than ``count``, last pages of every fill."""
+    _selected_check(dev, nh, nkv, _selected_case(nh, nkv, hd, page, [1, 2, 15, 16, 17, 31, 33, 100, 777], 9))
+
+
+@pytest.mark.parametrize("rows,lens", [(21, [21, 300]), (70, [1000])])
+def test_selected_rows_of_prompts(dev, rows, lens):
+    _selected_check(dev, 8, 2, _selected_case(8, 2, 64, 16, lens, 6, rows=rows, extra=24))
+
+
+@pytest.mark.parametrize("count,lens", [(1, [5]), (2, [4000]), (200, [9000]), (700, [13000, 3]), (64, [2000] * 9)])
+def test_selected_few_rows_long_lists(dev, count, lens):
+    """Lists that are cut between workgroups, longer than a workgroup's list, or nearly empty."""
+    _selected_check(dev, 4, 1, _selected_case(4, 1, 64, 16, lens, count))
+
+
+def test_selected_lists_in_any_order(dev):
+    """Empty entries anywhere, pages behind the context, pages twice, nothing at all."""
+    case = _selected_case(4, 2, 64, 16, [500, 500, 500, 0, 40], 12)
+    pages = case[5]
+    pages[0, 0] = torch.tensor([-1, 31, -1, 4, 4, 0, -1, 30, 99, 31, -1, 1 << 30], dtype=I32)
+    pages[0, 1] = -1
+    pages[1, 0] = torch.tensor([31] * 12, dtype=I32)
+    pages[2] = pages[2].flip(-1)
+    pages[3] = torch.arange(12, dtype=I32)      # a row without a context
+    got = _selected_check(dev, 4, 2, case)
+    assert (got[0, 128:] == 0).all() and (got[3] == 0).all()
+    case[3][0, 4] = -7                          # a page that is not in the cache counts as not there
+    case[3][1, 31] = 1 << 30
+    q, k, v, tables, ctx, pages, seq = (x.to(dev) for x in case)
+    got = longctx.paged_selected(q, k, v, tables, ctx, pages, 4, 2, 0.125)
+    pages = case[5].clone()
+    pages[0][pages[0] == 4] = -1
+    pages[1][pages[1] == 31] = -1
+    case[3][0, 4], case[3][1, 31] = 0, 0
+    want, tol = _selected_want(4, 2, 0.125, *case[:5], pages, case[6])
+    _close(got, want, tol)
+
+
+def test_selected_places_that_nobody_sees(dev):
+    """NaN and infinities behind the context, in other pages, and in no page of the list reach nothing; large scores do not overflow."""
+    case = _selected_case(4, 2, 64, 16, [37, 500, 16, 161], 5)
+    q, k, v, tables, ctx, pages, seq = case
+    used = torch.zeros(k.shape[0], 2, 16, dtype=torch.bool)
+    for t in range(4):
+        for h in range(2):
+            for p in pages[t, h].tolist():
+                if 0 <= p * 16 < int(ctx[t]):
+                    used[tables[t, p], h, : int(ctx[t]) - 16 * p] = True
+    k[~used] = math.nan
+    v[~used] = math.inf
+    v[~used & (torch.arange(16) % 2 == 0)] = math.nan
+    _selected_check(dev, 4, 2, case)
+    q.mul_(1e3)
+    _selected_check(dev, 4, 2, case)
+    _selected_check(dev, 4, 2, case, scale=-0.125)
+    _selected_check(dev, 4, 2, case, scale=0.0)
+
+
+def test_selected_out_and_strides(dev):
+    case = _selected_case(8, 2, 64, 16, [300, 50, 1], 8, extra=40)
+    out = torch.full((3, 8 * 64 + 16), 5.0, dtype=BF16, device=dev)
+    got = _selected_check(dev, 8, 2, case, out=out)
+    assert got.data_ptr() == out.data_ptr() and (out[:, 512:] == 5.0).all()
+    empty = [x[:0] if i in (0, 4, 5, 6) else x for i, x in enumerate(case)]
+    q, k, v, tables, ctx, pages, seq = (x.to(dev) for x in empty)
+    assert longctx.paged_selected(q, k, v, tables, ctx, pages, 8, 2, 0.125).shape == (0, 512)
+
+
+# ---- trees ------------------------------------------------------------------------------------------------------------------------------
+
+def _tree_case(nh, nkv, hd, page, ctx, nodes, seed=0, extra=0, behind=0):
+    g = _gen(seed)
+    need = [-(-c // page) for c in ctx]
+    pool = sum(need) + 3
+    tables = _tables(g, need, max(max(need), 1) + 1, pool, "cpu")
+    k, v = _randn(g, pool, nkv, page, hd), _randn(g, pool, nkv, page, hd)
+    cu = torch.tensor([sum(nodes[:i]) for i in range(len(nodes) + 1)], dtype=I32)
+    q = _randn(g, int(cu[-1]) + behind, nh * hd + extra)
+    par = torch.full((len(nodes), 64), -1, dtype=I32)
+    for a in range(1, 64):
+        par[:, a] = torch.randint(0, a, (len(nodes),), generator=g)
+    mask, _ = ops.tree_mask_ref(par)
+    return q, k, v, tables, cu, torch.tensor(ctx, dtype=I32), mask
+
+
+def _tree_want(nh, nkv, scale, q, k, v, tables, cu, ctx, mask):
+    page, hd, G = k.shape[2], k.shape[3], nh // nkv
+    o, tol = torch.zeros(q.shape[0], nh, hd, dtype=F64), torch.zeros(q.shape[0], nh, hd, dtype=F64)
+    for s in range(len(cu) - 1):
+        n, c = int(cu[s + 1] - cu[s]), int(ctx[s])
+        ids = tables[s, : -(-c // page)].long()
+        for a in range(n):
+            row = int(cu[s]) + a
+            see = torch.tensor([j < c - n or bool(int(mask[s, a]) >> (j - c + n) & 1) for j in range(c)], dtype=torch.bool)
+            for h in range(nkv):
+                kk, vv = k[ids, h].reshape(-1, hd)[:c][see], v[ids, h].reshape(-1, hd)[:c][see]
+                x = q[row, : nh * hd].view(nkv, G, hd)[h]
+                o[row, h * G:(h + 1) * G], tol[row, h * G:(h + 1) * G] = _attention(x, kk, vv, scale)
+    return o.view(q.shape[0], -1), tol.view(q.shape[0], -1)
+
+
+def _tree_check(dev, nh, nkv, case, max_nodes=64, scale=None, **kw):
+    scale = scale or case[1].shape[-1] ** -0.5
+    got = longctx.paged_tree(*(x.to(dev) for x in case), nh, nkv, scale, max_nodes=max_nodes, **kw)
+    want, tol = _tree_want(nh, nkv, scale, *case)
+    n = int(case[4][-1])
+    _close(got[:n, : want.shape[1]], want[:n], tol[:n])
+    return got
+
+
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 64), (7, 1, 128), (16, 1, 64), (4, 4, 256), (8, 1, 128), (2, 2, 128)])
+@pytest.mark.parametrize("nodes", [[1], [5, 9, 2], [64, 33]])
+def test_tree(dev, nh, nkv, hd, nodes):
+    """Trees of one to 64 nodes over contexts from nothing but the tree to several tiles."""
+    ctx = [n + c for n, c in zip(nodes, [0, 1, 130] if len(nodes) == 3 else [47, 0])]
+    _tree_check(dev, nh, nkv, _tree_case(nh, nkv, hd, 16, ctx, nodes), max_nodes=max(nodes))
+
+
+@pytest.mark.parametrize("page", [8, 16, 32, 128])
+def test_tree_pages(dev, page):
+    _tree_check(dev, 8, 2, _tree_case(8, 2, 64, page, [200, 77, 12, 260], [12, 7, 12, 1], extra=16), max_nodes=12)
+
+
+def test_tree_long_contexts(dev):
+    """Contexts cut between workgroups, beside a short one; a limit of nodes that no tree reaches."""
+    _tree_check(dev, 4, 1, _tree_case(4, 1, 64, 16, [5000, 20], [6, 8]), max_nodes=8)
+    _tree_check(dev, 4, 1, _tree_case(4, 1, 64, 16, [9001], [3]))
+
+
+def test_tree_empty_sequences_and_rows_behind(dev):
+    """Padded sequences: no nodes, no context; rows of no sequence stay as they are."""
+    case = _tree_case(8, 2, 64, 16, [30, 0, 40, 25], [4, 0, 3, 0], behind=5)
+    out = torch.full((12, 512), 3.0, dtype=BF16, device=dev)
+    _tree_check(dev, 8, 2, case, max_nodes=4, out=out)
+    assert (out[7:] == 3.0).all()
+    case = _tree_case(8, 2, 64, 16, [30, 40], [4, 3])
+    case[5][1] = 0                                     # rows without keys
+    got = longctx.paged_tree(*(x.to(dev) for x in case), 8, 2, 0.125, max_nodes=4)
+    assert (got[4:] == 0).all() and (got[:4] != 0).any()
+    case = _tree_case(8, 2, 64, 16, [30], [4])
+    case[6][:] = 0                                     # nodes that see none of the tree, and no prefix
+    case[5][0] = 4
+    assert (longctx.paged_tree(*(x.to(dev) for x in case), 8, 2, 0.125, max_nodes=4) == 0).all()
+    none = [case[0][:0], *case[1:3], case[3][:0], torch.zeros(1, dtype=I32), case[5][:0], case[6][:0]]
+    assert longctx.paged_tree(*(x.to(dev) for x in none), 8, 2, 0.125).shape == (0, 512)
+
+
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 64), (8, 1, 128), (2, 2, 64)])
+def test_tree_keys_that_a_row_does_not_see(dev, nh, nkv, hd):
+    """NaN and infinities in a drafted key or value reach the rows that see it, and no other; nor do those behind the context."""
+    case = _tree_case(nh, nkv, hd, 16, [100, 45], [9, 13])
+    q, k, v, tables, cu, ctx, mask = case
+    for s, (c, n, bad) in enumerate([(100, 9, 4), (45, 13, 6)]):
+        key = c - n + bad
+        v[tables[s, key // 16], :, key % 16, ::3] = math.inf
+        k[tables[s, (key + 1) // 16], :, (key + 1) % 16] = math.nan
+        v[tables[s, (key + 1) // 16], :, (key + 1) % 16] = math.nan
+        for j in range(c, -(-c // 16) * 16):
+            k[tables[s, j // 16], :, j % 16], v[tables[s, j // 16], :, j % 16] = math.nan, math.nan
+    got = longctx.paged_tree(*(x.to(dev) for x in case), nh, nkv, hd ** -0.5, max_nodes=13)
+    want, tol = _tree_want(nh, nkv, hd ** -0.5, *case)
+    assert torch.equal(got.isnan().cpu(), want.isnan())
+    assert torch.equal(got.isinf().cpu(), want.isinf())
+    fin = want.isfinite()
+    assert fin.any() and not fin.all()
+    _close(got.cpu()[fin], want[fin], tol[fin])
+
+
+def test_tree_unknown_pages(dev):
+    case = _tree_case(8, 2, 64, 16, [100], [5])
+    case[3][0, 2] = -1
+    got = longctx.paged_tree(*(x.to(dev) for x in case), 8, 2, 0.125, max_nodes=5)
+    case[3][0, 2] = 1 << 30
+    assert torch.equal(got, longctx.paged_tree(*(x.to(dev) for x in case), 8, 2, 0.125, max_nodes=5))
+    q, k, v, tables, cu, ctx, mask = case
+    keep = [j for j in range(100) if not 32 <= j < 48]      # the same as a context without those keys
+    ids = [(int(tables[0, j // 16]), j % 16) for j in keep]
+    k2, v2 = torch.zeros_like(k), torch.zeros_like(v)
+    t2 = torch.arange(k.shape[0], dtype=I32)[None, : tables.shape[1]].contiguous()
+    for i, (p, o) in enumerate(ids):
+        k2[i // 16, :, i % 16], v2[i // 16, :, i % 16] = k[p, :, o], v[p, :, o]
+    want, tol = _tree_want(8, 2, 0.125, q, k2, v2, t2, cu, torch.tensor([84], dtype=I32), mask)
+    _close(got, want, tol)
+
+
+# ---- together ---------------------------------------------------------------------------------------------------------------------------
+
+def _server(dev, nh, nkv, hd, prompts, steps, page=16, seed=0):
+    """State of a small server: caches, bounds, tables, and the rows of a prompt step and some decode steps."""
+    g = _gen(seed)
+    need = [-(-(n + steps) // page) for n in prompts]
+    pool = sum(need) + 2
+    tables = _tables(g, need, max(need), pool, dev)
+    k, v = torch.full((pool, nkv, page, hd), math.nan, dtype=BF16, device=dev), torch.full((pool, nkv, page, hd), math.nan, dtype=BF16, device=dev)
+    return dict(tables=tables, k=k, v=v, bounds=longctx.empty_bounds(k), cs=ops.rope_cos_sin(hd, max(prompts) + steps + 1, 10000.0, device=dev), g=g)
+
+
+def _step(s, nh, nkv, hd, spans, count, page=16, qkv=None):
+    """One step: positions ``spans`` = [(first, rows)] of each sequence; append, select, attend."""
+    dev = s["k"].device
+    pos = torch.cat([torch.arange(p, p + n) for p, n in spans]).to(I32).to(dev)
+    seq = torch.tensor([i for i, (_, n) in enumerate(spans) for _ in range(n)], dtype=I32, device=dev)
+    slots = s["tables"][seq.long(), pos.long() // page] * page + pos % page
+    qkv = _randn(s["g"], len(pos), (nh + 2 * nkv) * hd, dev=dev) if qkv is None else qkv
+    q = longctx.rope_cache_bounds(qkv, pos, s["cs"], nh, nkv, hd, slots, s["k"], s["v"], s["bounds"])
+    pages = longctx.select_pages(q, s["bounds"], s["tables"], pos + 1, nh, nkv, page, count, 1, 2, row_seq=seq)
+    return q, pos + 1, seq, pages, longctx.paged_selected(q, s["k"], s["v"], s["tables"], pos + 1, pages, nh, nkv, hd ** -0.5, row_seq=seq)
+
+
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 64), (4, 1, 128)])
+def test_steps_of_a_server(dev, nh, nkv, hd):
+    """A prompt step, the rest of a prompt beside decode rows, decode steps: bounds as rebuilt, selections and outputs as in 64 bits, and where a
+    context has no more pages than are kept, full attention."""
+    prompts = [50, 7, 130]
+    s = _server(dev, nh, nkv, hd, prompts, 20)
+    count = 5
+    plan = [[(0, 50), (0, 7), (0, 90)], [(50, 1), (7, 1), (90, 40)]] + [[(51 + i, 1), (8 + i, 1), (130 + i, 1)] for i in range(12)]
+    for spans in plan:
+        q, ctx, seq, pages, got = _step(s, nh, nkv, hd, spans, count)
+        ends = [p + n for p, n in spans]
+        rebuilt = longctx.empty_bounds(s["k"])
+        held = [(int(s["tables"][i, j]), min(16, e - 16 * j)) for i, e in enumerate(ends) for j in range(-(-e // 16))]
+        longctx.page_bounds(s["k"], rebuilt, torch.tensor([p for p, _ in held], dtype=I32, device=dev),
+                            torch.tensor([n for _, n in held], dtype=I32, device=dev))
+        assert torch.equal(rebuilt, s["bounds"])
+        cpu = [x.cpu() for x in (q, s["k"], s["v"], s["tables"], ctx, pages, seq)]
+        assert torch.equal(cpu[5], _selection64(cpu[0], s["bounds"].cpu(), cpu[3], cpu[4], nh, nkv, 16, count, 1, 2, cpu[6]))
+        want, tol = _selected_want(nh, nkv, hd ** -0.5, *cpu)
+        _close(got, want, tol)
+        short = (ctx <= count * 16).cpu()
+        full = ops.paged_decode_ref(q.cpu(), s["k"].cpu(), s["v"].cpu(), s["tables"].cpu()[seq.cpu().long()], ctx.cpu(), nh, nkv, hd ** -0.5)
+        _close(got.cpu()[short], full[short], 2 * tol[short])
+    # a draft of four nodes behind the last step, then its rejection: bounds stay wide, and the next step starts its page anew if it begins one
+    pos = [p + 1 for (p, _) in plan[-1]]
+    spans = [(p, 4) for p in pos]
+    q, ctx, seq, _, _ = _step(s, nh, nkv, hd, spans, count)
+    par = torch.tensor([[-1, 0, 0, 1]] * 3, dtype=I32)
+    mask, _ = ops.tree_mask_ref(par)
+    cu = torch.tensor([0, 4, 8, 12], dtype=I32)
+    ends = torch.tensor([p + 4 for p in pos], dtype=I32)
+    got = longctx.paged_tree(q, s["k"], s["v"], s["tables"], cu.to(dev), ends.to(dev), mask.to(dev), nh, nkv, hd ** -0.5, max_nodes=4)
+    want, tol = _tree_want(nh, nkv, hd ** -0.5, q.cpu(), s["k"].cpu(), s["v"].cpu(), s["tables"].cpu(), cu, ends, mask)
+    _close(got, want, tol)
+
+
+# ---- refusals ---------------------------------------------------------------------------------------------------------------------------
+
+def test_refusals(dev):
+    def refused(f, *a, **kw):
+        with pytest.raises(ValueError):
+            f(*a, **kw)
+
+    def change(args, i, x):
+        return [*args[:i], x, *args[i + 1:]]
+
+    qkv, pos, cs, slots, k, v, b = _append_case(dev, 8, 2, 64, 64, 0, 16, [(3, 5)])
+    good = [qkv, pos, cs, 8, 2, 64, slots, k, v, b]
+    longctx.rope_cache_bounds(*good)
+    f = longctx.rope_cache_bounds
+    refused(f, *change(good, 0, qkv[:, :500]))
+    refused(f, *change(good, 1, pos[:4]))
+    refused(f, *change(good, 1, pos.long()))
+    refused(f, *change(good, 2, cs[:, :24].contiguous()))
+    refused(f, *change(good, 3, 9))
+    refused(f, *change(good, 3, 64))
+    refused(f, *change(good, 6, slots[:-1]))
+    refused(f, *change(good, 7, k[:, :1]))
+    refused(f, *change(good, 8, v[1:]))
+    refused(f, *change(good, 9, b[:, :, :1]))
+    refused(f, *good, mode=2)
+    refused(f, *good, out=torch.empty(5, 500, dtype=BF16, device=dev))
+
+    f = longctx.page_bounds
+    pages, lens = torch.zeros(2, dtype=I32, device=dev), torch.ones(2, dtype=I32, device=dev)
+    refused(f, k[0], b, pages, lens)
+    refused(f, k, b[1:], pages, lens)
+    refused(f, k, b, pages.long(), lens)
+    refused(f, k, b, pages, lens[:1])
+
+    q, bb, tables, ctx, seq = (x.to(dev) for x in _select_case(8, 2, 64, 16, [300, 900], 3))
+    f = longctx.select_pages
+    good = [q, bb, tables, ctx, 8, 2, 16, 6]
+    f(*good, row_seq=seq)
+    refused(f, *good)      # a table for each row, or row_seq
+    refused(f, *good, row_seq=seq[1:])
+    refused(f, *good, row_seq=seq.long())
+    refused(f, *good, first=5, recent=2, row_seq=seq)
+    refused(f, *good, recent=0, row_seq=seq)
+    refused(f, *good, first=-1, row_seq=seq)
+    refused(f, *change(good, 0, q[:, :500]), row_seq=seq)
+    refused(f, *change(good, 1, bb[:, :, 0]), row_seq=seq)
+    refused(f, *change(good, 2, tables.long()), row_seq=seq)
+    refused(f, *change(good, 3, ctx[1:]), row_seq=seq)
+    refused(f, *change(good, 4, 64), row_seq=seq)
+    refused(f, *change(good, 6, 0), row_seq=seq)
+    refused(f, *good, row_seq=seq, out=torch.empty(6, 2, 5, dtype=I32, device=dev))
+    refused(f, *change(good, 0, q.clone().requires_grad_()), row_seq=seq)
+
+    q, k, v, tables, ctx, pages, seq = (x.to(dev) for x in _selected_case(8, 2, 64, 16, [300, 90], 6))
+    f = longctx.paged_selected
+    good = [q, k, v, tables, ctx, pages, 8, 2, 0.125]
+    f(*good)
+    refused(f, *change(good, 1, k[:, :, :12]))
+    refused(f, *change(good, 2, v[1:]))
+    refused(f, *change(good, 3, tables[:1]))
+    refused(f, *change(good, 4, ctx[:1]))
+    refused(f, *change(good, 5, pages[:, :1].contiguous()))
+    refused(f, *change(good, 5, pages.long()))
+    refused(f, *change(good, 5, pages[:, :, :0]))
+    refused(f, *change(good, 6, 7))
+    refused(f, *good, out=torch.empty(1, 512, dtype=BF16, device=dev))
+    refused(f, *change(good, 0, q.clone().requires_grad_()))
+    k12 = torch.zeros(4, 2, 12, 64, dtype=BF16, device=dev)
+    refused(f, *change(change(good, 1, k12), 2, k12))      # pages of a power of two
+
+    case = [x.to(dev) for x in _tree_case(8, 2, 64, 16, [300, 90], [6, 4])]
+    f = longctx.paged_tree
+    f(*case, 8, 2, 0.125, max_nodes=6)
+    refused(f, *case, 8, 2, 0.125, max_nodes=65)
+    refused(f, *case, 8, 2, 0.125, max_nodes=0)
+    refused(f, *change(case, 4, case[4][:2]), 8, 2, 0.125)
+    refused(f, *change(case, 6, case[6][:, :3].contiguous()), 8, 2, 0.125)
+    refused(f, *change(case, 6, case[6].int()), 8, 2, 0.125)
+    refused(f, *change(case, 3, case[3][:1]), 8, 2, 0.125)
+    refused(f, *case, 8, 3, 0.125)
+
+
+@gpu
+def test_refusals_of_the_kernels():
+    """What only the kernels cannot take: other types and head sizes, starts off 16 bytes, tensors of other devices."""
+    dev = "cuda"
+    longctx.load_native(required=True)
+    q, k, v, tables, ctx, pages, seq = (x.to(dev) for x in _selected_case(8, 2, 64, 16, [300, 90], 6))
+    f = longctx.paged_selected
+    good = [q, k, v, tables, ctx, pages, 8, 2, 0.125]
+    with pytest.raises(ValueError):
+        f(q.float(), *good[1:])
+    with pytest.raises(ValueError):
+        f(q, k.half(), v.half(), *good[3:])
+    with pytest.raises(ValueError):
+        f(torch.zeros(2, 8 * 64 + 1, dtype=BF16, device=dev)[:, 1:], *good[1:])
+    with pytest.raises(ValueError):
+        f(q, k.cpu(), v.cpu(), *good[3:])
+    k32 = torch.zeros(4, 2, 16, 32, dtype=BF16, device=dev)
+    with pytest.raises(ValueError):
+        f(q, k32, k32, *good[3:])
+    with pytest.raises(ValueError):
+        f(*good, out=torch.empty(2, 512, dtype=torch.float32, device=dev))
+
+
+# ---- on the device ----------------------------------------------------------------------------------------------------------------------
+
+@gpu
+def test_captured_steps():
+    """Append, selection, attention and a tree in one graph, replayed with other inputs between the program's own work: as eagerly."""
+    dev, nh, nkv, hd = "cuda", 8, 2, 64
+    longctx.load_native(required=True)
+    g = _gen(4)
+    R, cols, nodes = 3, 60, 8
+    tables = torch.randperm(R * cols, generator=g).to(I32).view(R, cols).to(dev)
+    cs = ops.rope_cos_sin(hd, cols * 16 + 1, 10000.0, device=dev)
+    k0, v0 = _randn(g, R * cols, nkv, 16, hd, dev=dev), _randn(g, R * cols, nkv, 16, hd, dev=dev)
+    b0 = torch.stack([k0.amin(2), k0.amax(2)], 2)
+    mask, _ = ops.tree_mask_ref(torch.tensor([[-1, 0, 0, 1, 1, 2, 3, 3]] * R, dtype=I32))
+    st = dict(k=k0.clone(), v=v0.clone(), b=b0.clone(), qkv=torch.zeros(R * nodes, (nh + 2 * nkv) * hd, dtype=BF16, device=dev),
+              pos=torch.zeros(R * nodes, dtype=I32, device=dev), slots=torch.zeros(R * nodes, dtype=I32, device=dev),
+              ends=torch.zeros(R, dtype=I32, device=dev), seq=torch.arange(R, dtype=I32, device=dev).repeat_interleave(nodes),
+              cu=torch.arange(0, R * nodes + 1, nodes, dtype=I32, device=dev), mask=mask.to(dev))
+
+    def step(s):
+        q = longctx.rope_cache_bounds(s["qkv"], s["pos"], cs, nh, nkv, hd, s["slots"], s["k"], s["v"], s["b"])
+        ctx = s["pos"] + 1
+        pages = longctx.select_pages(q, s["b"], tables, ctx, nh, nkv, 16, 7, 1, 2, row_seq=s["seq"])
+        o = longctx.paged_selected(q, s["k"], s["v"], tables, ctx, pages, nh, nkv, hd ** -0.5, row_seq=s["seq"])
+        t = longctx.paged_tree(q, s["k"], s["v"], tables, s["cu"], s["ends"], s["mask"], nh, nkv, hd ** -0.5, max_nodes=nodes)
+        return q, pages, o, t
+
+    def load(s, seed):
+        g = _gen(seed)
+        starts = torch.randint(1, cols * 16 - nodes, (R,), generator=g)
+        pos = (starts[:, None] + torch.arange(nodes)).view(-1)
+        s["pos"].copy_(pos.to(I32))
+        s["slots"].copy_((tables.cpu()[torch.arange(R).repeat_interleave(nodes), pos // 16] * 16 + pos % 16).to(I32))
+        s["ends"].copy_((starts + nodes).to(I32))
+        s["qkv"].copy_(_randn(g, *s["qkv"].shape))
+        for name, x in (("k", k0), ("v", v0), ("b", b0)):
+            s[name].copy_(x)
+
+    with torch.inference_mode():
+        load(st, 0)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(st)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step(st)
+        for seed in range(1, 6):
+            load(st, seed)
+            want = [x.clone() for x in (*step(st), st["k"], st["v"], st["b"])]
+            load(st, seed)
+            graph.replay()
+            torch.cuda.synchronize()
+            for a, b in zip((*outs, st["k"], st["v"], st["b"]), want):
+                assert torch.equal(a, b)
+
+
+@gpu
+def test_two_streams_at_once():
+    """Calls on two streams, unlike in size, do not share scratch memory."""
+    longctx.load_native(required=True)
+    cases = [[x.cuda() for x in _selected_case(4, 1, 64, 16, [9000], 300, seed=1)], [x.cuda() for x in _selected_case(4, 1, 64, 16, [5000, 100], 200, seed=2)]]
+    trees = [[x.cuda() for x in _tree_case(4, 1, 64, 16, [5000], [6], seed=3)], [x.cuda() for x in _tree_case(4, 1, 64, 16, [900, 4000], [9, 2], seed=4)]]
+
+    def both(i):
+        q, k, v, tables, ctx, pages, seq = cases[i]
+        return longctx.paged_selected(q, k, v, tables, ctx, pages, 4, 1, 0.125, row_seq=seq), longctx.paged_tree(*trees[i], 4, 1, 0.125, max_nodes=9)
+
+    want = [both(0), both(1)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(both(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for a, b in got[i]:
+            assert torch.equal(a, want[i][0]) and torch.equal(b, want[i][1])
+
+
+@gpu
+def test_offsets_past_32_bits():
+    """A cache of more than 2^31 values: pages at its end are read and written where they lie."""
+    longctx.load_native(required=True)
+    dev, nh, nkv, hd, page = "cuda", 16, 8, 128, 16
+    nb = (1 << 31) // (nkv * page * hd) + 70
+    k = torch.zeros(nb, nkv, page, hd, dtype=BF16, device=dev)
+    v = torch.zeros_like(k)
+    g = _gen(9)
+    last = torch.arange(nb - 64, nb, dtype=I32)
+    small_k, small_v = _randn(g, 64, nkv, page, hd, dev=dev), _randn(g, 64, nkv, page, hd, dev=dev)
+    k[last.long()], v[last.long()] = small_k, small_v
+    perm = torch.randperm(64, generator=g).to(I32)
+    tables, small_tables = last[perm.long()][None].contiguous().to(dev), perm[None].contiguous().to(dev)
+    bounds, small_bounds = longctx.empty_bounds(k), longctx.empty_bounds(small_k)
+    lens = torch.full((64,), 16, dtype=I32, device=dev)
+    longctx.page_bounds(k, bounds, last.to(dev), lens)
+    longctx.page_bounds(small_k, small_bounds, torch.arange(64, dtype=I32, device=dev), lens)
+    assert torch.equal(bounds[last.long()], small_bounds)
+    qkv = _randn(g, 3, (nh + 2 * nkv) * hd, dev=dev)
+    pos = torch.tensor([1000, 1001, 1002], dtype=I32, device=dev)
+    cs = ops.rope_cos_sin(hd, 1024, 10000.0, device=dev)
+    outs = []
+    for kk, vv, tt, bb in ((k, v, tables, bounds), (small_k, small_v, small_tables, small_bounds)):
+        # 2^31 values are 2^27 slots of 16: slots stay within 32 bits where offsets do not
+        slots = tt[0, pos.long() // 16] * 16 + pos % 16
+        q = longctx.rope_cache_bounds(qkv, pos, cs, nh, nkv, hd, slots, kk, vv, bb)
+        seq = torch.zeros(3, dtype=I32, device=dev)
+        pages = longctx.select_pages(q, bb, tt, pos + 1, nh, nkv, 16, 20, 1, 1, row_seq=seq)
+        o = longctx.paged_selected(q, kk, vv, tt, pos + 1, pages, nh, nkv, hd ** -0.5, row_seq=seq)
+        mask, _ = ops.tree_mask_ref(torch.tensor([[-1, 0, 0]], dtype=I32))
+        t = longctx.paged_tree(q, kk, vv, tt, torch.tensor([0, 3], dtype=I32, device=dev), torch.tensor([1003], dtype=I32, device=dev),
+                               mask.to(dev), nh, nkv, hd ** -0.5, max_nodes=3)
+        outs.append((q, pages, o, t, kk[tt[0].long()], vv[tt[0].long()], bb[tt[0].long()]))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
