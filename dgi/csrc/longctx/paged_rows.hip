@@ -56,36 +56,6 @@ __device__ __forceinline__ int v_lds_off(int row, int col) {
 template <int HD>
 constexpr int wave_lds() { return 32 * HD * 2 > 16 * HD * 4 ? 32 * HD * 2 : 16 * HD * 4; }
 
-template <int N>
-__device__ __forceinline__ bool not_finite(const u32x4 (&v)[N]) {
-  bool odd = false;
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) odd = odd || (v[i][j] & 0x7f80u) == 0x7f80u || (v[i][j] & 0x7f800000u) == 0x7f800000u;
-  return odd;
-}
-
-// O^T += V^T P^T of a tile of 32 keys in vt, without the products of zero weights.
-template <int NQ, int NC>
-__device__ __forceinline__ void add_key_by_key(f32x4 (&o)[NQ][NC], const u32x4 (&pf)[NQ], const uint16_t* vt, int lane) {
-  const int qi = lane & 15, g = lane >> 4;
-  for (int from = 0; from < 4; ++from)      // the lanes that hold the weights of keys 16 u + 4 from + i
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-      for (int n = 0; n < NQ; ++n) {
-        const uint32_t two = __shfl(pf[n][j >> 1], 16 * from + qi, 64);
-        const float p = __uint_as_float(j & 1 ? two & 0xffff0000u : two << 16);
-        const int row = 16 * (j >> 2) + 4 * from + (j & 3);
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (p != 0.f) o[n][c][i] += p * bf16_to_f32(vt[v_lds_off<16 * NC>(row, 16 * c + 4 * g + i)]);
-      }
-}
-
 // Runs of a tree's keys: as many as there are places for, of min_part keys at least, each a multiple of 32 keys and of a page.
 __device__ __forceinline__ int tree_part(const Args& a, int ctx) {
   const int n = max(1, min(a.splits, (ctx + a.min_part - 1) / a.min_part));
@@ -221,6 +191,26 @@ __global__ __launch_bounds__(64 * NW) void paged_rows_kernel(Args a) {
         const uint16_t* p = a.v + ((((size_t)pg.x * a.nkv + h) << a.bs_log2) + off) * HD + (lane % VCH) * 8;
         vr[i] = tok < keys && off < pg.y ? *reinterpret_cast<const u32x4*>(p) : u32x4{0, 0, 0, 0};
       }
+      // Values of the tree's keys that are infinite or no numbers reach the rows that see them alone, but zero times such a value is no
+      // number: they are taken out here and added below where the weight is not zero.
+      unsigned odd = 0;
+      if constexpr (TREE) {
+        if (at + 32 * t + 32 > tree_key) {
+#pragma unroll
+          for (int i = 0; i < VCH / 2; ++i) {
+            bool is = false;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const bool lo_odd = (vr[i][j] & 0x7f80u) == 0x7f80u, hi_odd = (vr[i][j] & 0x7f800000u) == 0x7f800000u;
+              is = is || lo_odd || hi_odd;
+              vr[i][j] &= (lo_odd ? 0xffff0000u : ~0u) & (hi_odd ? 0xffffu : ~0u);
+            }
+            const unsigned long long b = __ballot(is);
+#pragma unroll
+            for (int j = 0; j < 64 / VCH; ++j) odd |= (b >> (j * VCH) & ((1ull << VCH) - 1)) ? 1u << (i * (64 / VCH) + j) : 0u;
+          }
+        }
+      }
       // ---- which of the lane's keys (16 u + 4 g + i) are there
       bool there[2][4];
 #pragma unroll
@@ -277,14 +267,6 @@ __global__ __launch_bounds__(64 * NW) void paged_rows_kernel(Args a) {
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_wave_barrier();
-      if constexpr (TREE) {
-        // Values of drafted keys that are no numbers or infinite reach the rows that see them alone (zero times such a value is no
-        // number): key by key where the weight is not zero.
-        if (at + 32 * t + 32 > tree_key && __any(not_finite(vr))) {
-          add_key_by_key(o, pf, vt, lane);
-          continue;
-        }
-      }
       const int tq = qi >> 2, tp = qi & 3;
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
@@ -297,6 +279,24 @@ __global__ __launch_bounds__(64 * NW) void paged_rows_kernel(Args a) {
         vf[3] = (uint32_t)(uint16_t)a1[2] | ((uint32_t)(uint16_t)a1[3] << 16);
 #pragma unroll
         for (int n = 0; n < NQ; ++n) o[n][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(vf), as_bf16x8(pf[n]), o[n][c], 0, 0, 0);
+      }
+      if constexpr (TREE) {
+        for (; odd; odd &= odd - 1) {      // what was taken out: key kk of the tile
+          const int kk = __ffs(odd) - 1, tok = 32 * t + kk, j = (kk >> 4) * 4 + (kk & 3);
+          const uint16_t* vp = a.v + ((((size_t)list[tok >> a.bs_log2].x * a.nkv + h) << a.bs_log2) + (tok & (bs - 1))) * HD + 4 * g;
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) {
+            const uint32_t two = __shfl(j & 4 ? (j & 2 ? pf[n][3] : pf[n][2]) : (j & 2 ? pf[n][1] : pf[n][0]), 16 * (kk >> 2 & 3) + qi, 64);
+            const float p = __uint_as_float(j & 1 ? two & 0xffff0000u : two << 16);
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint16_t x = vp[16 * c + i];
+                if ((x & 0x7f80) == 0x7f80 && p != 0.f) o[n][c][i] += p * bf16_to_f32(x);
+              }
+          }
+        }
       }
     }
   }
@@ -402,11 +402,8 @@ int launch_dims(const Args& a, int items, int hd, hipStream_t s) {
 
 }  // namespace
 
-// Query columns of a workgroup of a tree: 16, 32 or (up to 128 dims, whose sums fit the registers) 64 of its (node, head) pairs.
-extern "C" int dgi_tree_columns(int max_nodes, int G, int hd) {
-  const int pairs = max_nodes * G;
-  return pairs <= 16 ? 16 : pairs <= 32 || hd > 128 ? 32 : 64;
-}
+// Query columns of a workgroup of a tree: 16 or 32 of its (node, head) pairs.
+extern "C" int dgi_tree_columns(int max_nodes, int G) { return max_nodes * G <= 16 ? 16 : 32; }
 
 extern "C" int dgi_paged_selected(const void* q, long long q_stride, const void* k, const void* v, const int* tables, int table_stride,
                                   int table_cols, int n_seqs, int num_blocks, const int* ctx, const int* row_seq, const int* pages, int count,
@@ -471,9 +468,7 @@ extern "C" int dgi_paged_tree(const void* q, long long q_stride, const void* k, 
   a.mask_stride = mask_stride;
   a.max_nodes = max_nodes;
   a.min_part = min_part;
-  const int cols = dgi_tree_columns(max_nodes, nh / nkv, hd), items = n_seqs * ((max_nodes * (nh / nkv) + cols - 1) / cols);
+  const int cols = dgi_tree_columns(max_nodes, nh / nkv), items = n_seqs * ((max_nodes * (nh / nkv) + cols - 1) / cols);
   if (cols == 16) return launch_dims<1, 4, true>(a, items, hd, s);
-  if (cols == 32) return launch_dims<2, 4, true>(a, items, hd, s);
-  if (hd == 64) return launch<64, 4, 4, true>(a, items, s);
-  return launch<128, 4, 4, true>(a, items, s);
+  return launch_dims<2, 4, true>(a, items, hd, s);
 }

@@ -1,0 +1,457 @@
+// dgi/csrc/longctx/tree_tiles.hip — attention of drafted trees of many (node, head) pairs over a paged cache.
+//
+// All heads of a kv head's group and all nodes of a sequence see the same keys but for the tree's own: their (node, head) pairs are the
+// rows of one product, r = node G + head.  A workgroup owns 128 of them (32 a wave) and a run of keys.  Tiles of 64 keys and values go
+// straight to LDS, two stages, one barrier a tile; scores are formed transposed, S^T = K Q^T, so that a lane owns a row and the weights are
+// the operand of O^T += V^T P^T where they lie.  Only the tiles that hold the tree's keys are masked.
+//
+// Bound by the matrix cores where there are many pairs (4 nodes n heads hd products a key), by the cache's bytes where there are few; with
+// few sequences also by how many workgroups share the keys.  Runs are cut on the device, to one length for all sequences: about `places`
+// of them in all, so that a long context beside short ones does not hold up the launch.  Runs of one sequence are added up by a second
+// launch.
+#include "../prefill_attention_kernel.h"
+
+using namespace dgi;
+using namespace dgi::prefill;
+
+namespace {
+
+constexpr int kRows = 128, kWaves = 4;      // rows of a workgroup
+
+struct Args {
+  const uint16_t* q;
+  long long q_stride;
+  const uint16_t* k;
+  const uint16_t* v;
+  const int* tables;
+  int table_stride, table_cols, n_seqs, num_blocks, rows;
+  const int* cu;
+  const int* ctx;
+  const unsigned long long* mask;
+  int mask_stride, max_nodes;
+  uint16_t* out;
+  long long out_stride;
+  float* part_o;      // [run][tile][kv head][128][HD] of normalised sums, [run][tile][kv head][128] of their log2 sums
+  float* part_l;
+  int places, min_part, nh, nkv, bs_log2;
+  float scale_log2;
+};
+
+__device__ __forceinline__ int context_of(const Args& a, int s) { return min(max(a.ctx[s], 0), a.table_cols << a.bs_log2); }
+
+__device__ __forceinline__ int runs_of(int ctx, int part) { return max(1, (ctx + part - 1) / part); }
+
+// The length of a run: all contexts cut into `places` in all, of min_part keys at least, a multiple of a tile and of a page.  One wave.
+__device__ int run_length(const Args& a, int lane) {
+  long long sum = 0;
+  for (int s = lane; s < a.n_seqs; s += 64) sum += context_of(a, s);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  const int unit = max(KT, 1 << a.bs_log2);
+  const int part = (int)max((long long)a.min_part, (sum + a.places - 1) / a.places);
+  return (part + unit - 1) / unit * unit;
+}
+
+// Runs of the sequences before lane's, for the 64 from s0 on; `runs`: the lane's own, `all`: of all 64.  One wave.
+__device__ __forceinline__ int runs_before(const Args& a, int s0, int part, int lane, int& runs, int& all) {
+  runs = s0 + lane < a.n_seqs ? runs_of(context_of(a, s0 + lane), part) : 0;
+  int sum = runs;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int x = __shfl_up(sum, o, 64);
+    if (lane >= o) sum += x;
+  }
+  all = __shfl(sum, 63, 64);
+  return sum - runs;
+}
+
+template <int HD>
+__global__ __launch_bounds__(kWaves * 64, 2) void tree_tiles_kernel(Args a) {
+  __shared__ __attribute__((aligned(16))) uint16_t lds[2 * KT * 2 * HD];
+  __shared__ int s_seq, s_run, s_part;
+  const int G = a.nh / a.nkv, tiles = (a.max_nodes * G + kRows - 1) / kRows;
+  // kv heads side by side: with eight of them each has an XCD's L2 to itself
+  const int unit = blockIdx.x / a.nkv, kvh = blockIdx.x - unit * a.nkv, work = unit / tiles, mt = unit - work * tiles;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  if (w == 0) {
+    const int part = run_length(a, lane);
+    int seq = -1, run = 0;
+    for (int s0 = 0, done = 0; s0 < a.n_seqs && seq < 0; s0 += 64) {
+      int runs, all;
+      const int before = done + runs_before(a, s0, part, lane, runs, all);
+      const unsigned long long mine = __ballot(work >= before && work < before + runs);
+      if (mine) {
+        const int l = __ffsll(mine) - 1;
+        seq = s0 + l;
+        run = work - __shfl(before, l, 64);
+      }
+      done += all;
+    }
+    if (lane == 0) {
+      s_seq = seq;
+      s_run = run;
+      s_part = part;
+    }
+  }
+  __syncthreads();
+  const int seq = __builtin_amdgcn_readfirstlane(s_seq), part = __builtin_amdgcn_readfirstlane(s_part);
+  if (seq < 0) return;
+  const int q0 = a.cu[seq], nodes = q0 < 0 ? 0 : min(min(a.cu[seq + 1], a.rows) - q0, a.max_nodes);
+  if (mt * kRows >= nodes * G) return;
+  const int ctx = context_of(a, seq), kv_begin = __builtin_amdgcn_readfirstlane(s_run) * part, kv_end = min(kv_begin + part, ctx);
+  const int bs = 1 << a.bs_log2;
+  const int* bt = a.tables + (size_t)seq * a.table_stride;
+  const int nkv = a.nkv;
+
+  // a page that is not in the cache: its keys are not there, page 0 is read in its place
+  bool bad = false;
+  for (int e = (kv_begin >> a.bs_log2) + tid; e < (kv_end + bs - 1) >> a.bs_log2; e += kWaves * 64) bad = bad || (unsigned)bt[e] >= (unsigned)a.num_blocks;
+  bad = __syncthreads_or(bad);
+
+  const int lr = lane & 31, hh = lane >> 5;
+  const int r = mt * kRows + 32 * w + lr, node = r / G, head = kvh * G + r - node * G;
+  const bool row_valid = node < nodes, wave_rows = mt * kRows + 32 * w < nodes * G;
+  const int tree_key = ctx - nodes;      // the key of node 0
+  const unsigned long long tmask = row_valid ? a.mask[(size_t)seq * a.mask_stride + node] : 0;
+
+  constexpr int NS = HD / 16, ND = HD / 32, CH = HD / 8;
+  u32x4 qf[NS];
+  {
+    const uint16_t* qp = a.q + (size_t)(q0 + (row_valid ? node : 0)) * a.q_stride + (row_valid ? head : 0) * HD;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) qf[s] = row_valid ? *reinterpret_cast<const u32x4*>(qp + 16 * s + 8 * hh) : u32x4{0, 0, 0, 0};
+    __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): or every tile's first product waits for the next tile's loads
+    // the softmax takes maxima of raw scores: a negative scale is the query's sign, zero stays above it (unseen keys are -inf)
+    if (a.scale_log2 < 0.f) {
+#pragma unroll
+      for (int s = 0; s < NS; ++s) qf[s] ^= 0x80008000u;
+    }
+  }
+  const float scale = fmaxf(fabsf(a.scale_log2), 1e-30f);
+  float m_run = -1e30f, l_run = 0.f;
+  f32x16 o[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+
+  // A wave stages RW rows of a tile, 1 KB a load; in pages of at least RW tokens they lie side by side, so that its loads share an
+  // id and an address.  The swizzle is in which chunk of its row a lane loads.
+  const size_t head_stride = (size_t)bs * HD;
+  constexpr int RW = KT / kWaves, NP = RW * CH / 64;
+  const int row0 = w * RW;
+  const bool whole_rows = bs >= RW;
+  int k_at[NP], v_at;
+#pragma unroll
+  for (int p = 0; p < NP; ++p) {
+    const int row = p * (64 / CH) + lane / CH;
+    k_at[p] = 2 * (row * HD + 8 * k_slot<HD>(row0 + row, lane % CH)) - 1024 * p;
+  }
+  v_at = 2 * (lane / CH * HD + 8 * v_slot<HD>(row0 + lane / CH, lane % CH));
+  int none = 0;
+  asm("" : "+v"(none));                   // a vector load: a scalar one's wait would be one for all reads of LDS
+  auto known = [&](int id) __attribute__((always_inline)) { return (unsigned)id < (unsigned)a.num_blocks ? id : 0; };
+  auto read_id = [&](int kb0) __attribute__((always_inline)) {
+    return whole_rows ? bt[(min(kb0 + row0, kv_end - 1) >> a.bs_log2) + none] : bt[min(kb0 + row0 + lane % RW, kv_end - 1) >> a.bs_log2];
+  };
+  auto full = [&](int kb0) __attribute__((always_inline)) { return whole_rows && kb0 + KT <= kv_end; };
+  __amdgpu_buffer_rsrc_t k_rows, v_rows;
+  auto at_page = [&](int id, int key) __attribute__((always_inline)) {
+    const size_t from = ((size_t)known(__builtin_amdgcn_readfirstlane(id)) * nkv + kvh) * head_stride + (size_t)(key & (bs - 1)) * HD;
+    k_rows = __builtin_amdgcn_make_buffer_rsrc((void*)(a.k + from), 0, RW * HD * 2, 0x00027000);
+    v_rows = __builtin_amdgcn_make_buffer_rsrc((void*)(a.v + from), 0, RW * HD * 2, 0x00027000);
+  };
+  auto load = [&](auto l_, int stage) __attribute__((always_inline)) {
+    constexpr int l = decltype(l_)::value, p = l < NP ? l : l - NP;
+    const lds_ptr at = (lds_ptr)(lds + stage * KT * 2 * HD + (l < NP ? 0 : KT * HD) + row0 * HD);
+    load_chunk<1024 * p>(l < NP ? k_rows : v_rows, l < NP ? k_at[p] : v_at, at);
+  };
+  // a tile that ends early, or whose rows have several pages: each lane finds its own, no row is after the last key
+  auto load_part = [&](int kb0, int stage, int id) __attribute__((always_inline)) {
+    const lds_ptr kl = (lds_ptr)(lds + stage * KT * 2 * HD + row0 * HD), vl = (lds_ptr)(lds + stage * KT * 2 * HD + KT * HD + row0 * HD);
+    int part_lane = lane;
+    asm volatile("" : "+v"(part_lane));      // computed here: kept from before the loop its addresses would cost registers
+    const int first = min(kb0 + row0, kv_end - 1), last = kv_end - 1 - first;
+    if (whole_rows) {
+      at_page(id, first);
+#pragma unroll 1
+      for (int p = 0; p < NP; ++p) {
+        const int row = p * (64 / CH) + part_lane / CH;
+        load_chunk<0>(k_rows, 2 * (min(row, last) * HD + 8 * k_slot<HD>(row0 + row, part_lane % CH)), kl + p * 1024);
+        load_chunk<0>(v_rows, 2 * (min(row, last) * HD + 8 * v_slot<HD>(row0 + row, part_lane % CH)), vl + p * 1024);
+      }
+      return;
+    }
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      const int row = p * (64 / CH) + part_lane / CH;
+      const size_t from = ((size_t)known(__shfl(id, row, 64)) * nkv + kvh) * head_stride + (size_t)(min(kb0 + row0 + row, kv_end - 1) & (bs - 1)) * HD;
+      load_chunk((const char*)(a.k + from + 8 * k_slot<HD>(row0 + row, part_lane % CH)), kl + p * 1024);
+      load_chunk((const char*)(a.v + from + 8 * v_slot<HD>(row0 + row, part_lane % CH)), vl + p * 1024);
+    }
+  };
+  int id = 0;
+  if (kv_end > kv_begin) {
+    id = read_id(kv_begin);
+    if (full(kv_begin)) {
+      at_page(id, kv_begin + row0);
+      each<0, 2 * NP>([&](auto l) __attribute__((always_inline)) { load(l, 0); });
+    } else load_part(kv_begin, 0, id);
+    id = read_id(kv_begin + KT);
+  }
+  // LDS addresses of this lane's operands in stage 0: keys lr, dims 16 s + 8 hh ..; values of dims 32 d .., keys 4 hh + tq
+  typedef __attribute__((address_space(3))) const char* lds_at;
+  lds_at ka[NS], va[ND];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    ka[s] = (lds_at)(lds + k_off<HD>(lr, 2 * s + hh));
+    asm("" : "+v"(ka[s]));
+  }
+#pragma unroll
+  for (int d = 0; d < ND; ++d) {
+    const int col = 32 * d + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    va[d] = (lds_at)(lds + KT * HD + v_off<HD>(4 * hh + ((lane & 15) >> 2), col >> 3) + (col & 7));
+    asm("" : "+v"(va[d]));
+  }
+
+  auto step = [&](int kb0, auto stage_) __attribute__((always_inline)) {
+    constexpr int stage = decltype(stage_)::value, at = stage * KT * 2 * HD * 2;
+    __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): this wave's loads of the tile
+    __syncthreads();                      // everybody's; and the other stage has been read
+    const bool next = full(kb0 + KT);
+    if (next) {
+      at_page(id, kb0 + KT + row0);
+      each<0, 2 * NP>([&](auto l) __attribute__((always_inline)) { load(l, 1 - stage); });
+    } else if (kb0 + KT < kv_end) load_part(kb0 + KT, 1 - stage, id);
+    id = read_id(kb0 + 2 * KT);
+    // Values of the tree's keys that are infinite or no numbers reach the rows that see them alone, but zero times such a value is no
+    // number: they are taken out of the tile here and added below where the weight is not zero.
+    unsigned long long odd = 0;
+    if (kb0 + KT > tree_key) {
+      uint16_t* vt = lds + stage * KT * 2 * HD + KT * HD;
+#pragma unroll 1
+      for (int p = 0; p < KT * CH / 64; ++p) {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(vt + p * 512 + lane * 8);
+        bool is = false;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) is = is || (x[j] & 0x7f80u) == 0x7f80u || (x[j] & 0x7f800000u) == 0x7f800000u;
+        const unsigned long long b = __ballot(is);
+        for (int i = 0; i < 64 / CH; ++i)
+          if (b >> (i * CH) & (CH == 16 ? 0xffffull : 0xffull)) odd |= 1ull << (p * (64 / CH) + i);
+      }
+      __syncthreads();      // all have looked
+      if (odd) {
+#pragma unroll 1
+        for (int p = w; p < KT * CH / 64; p += kWaves) {
+          u32x4* at_v = reinterpret_cast<u32x4*>(vt + p * 512 + lane * 8);
+          u32x4 x = *at_v;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if ((x[j] & 0x7f80u) == 0x7f80u) x[j] &= 0xffff0000u;
+            if ((x[j] & 0x7f800000u) == 0x7f800000u) x[j] &= 0xffffu;
+          }
+          *at_v = x;
+        }
+        __syncthreads();
+      }
+    }
+    if (!wave_rows) return;
+    // ---- S^T = K Q^T for two 32-key blocks: the first block's operands all under way before its products, the second's between them,
+    // the first values between the second's
+    f32x16 sc[2];
+    auto read_v = [&](int j, int d) __attribute__((always_inline)) {
+      const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(va[d] + (at + 32 * HD * j)));
+      const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(va[d] + (at + 32 * HD * j + 16 * HD)));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    auto read_k = [&](int kb, int s) __attribute__((always_inline)) {
+      return *(const __attribute__((address_space(3))) bf16x8*)(ka[s] + (at + 64 * HD * kb));
+    };
+    typedef short short8v __attribute__((ext_vector_type(8)));
+    short8v vf[2][ND];
+    {
+      bf16x8 kf[NS];
+#pragma unroll
+      for (int s = 0; s < NS; ++s) kf[s] = read_k(0, s);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[kb][i] = 0.f;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+          sc[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[s], as_bf16x8(qf[s]), sc[kb], 0, 0, 0);
+          if (kb == 0) kf[s] = read_k(1, s);
+          else {
+#pragma unroll
+            for (int f = s * 2 * ND / NS; f < (s + 1) * 2 * ND / NS; ++f) vf[f / ND][f % ND] = read_v(f / ND, f % ND);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    }
+    // ---- online softmax; lane owns row lr, keys kb0 + 32 kb + (i & 3) + 8 (i >> 2) + 4 hh
+    if (kb0 + KT > tree_key || kb0 + KT > kv_end || bad) {
+      const int key0 = kb0 + 4 * hh;
+      const int lim = kv_end - 1 - key0, t = tree_key - key0;      // last key; keys before t are seen, after it as the mask says
+      unsigned long long see = lim < 0 ? 0 : lim >= 63 ? ~0ull : (2ull << lim) - 1;
+      see &= t >= 64 ? ~0ull : t >= 0 ? (tmask << t) | ((1ull << t) - 1) : t > -64 ? tmask >> -t : 0ull;
+      if (bad) see &= __ballot((unsigned)bt[min(kb0 + lane, kv_end - 1) >> a.bs_log2] < (unsigned)a.num_blocks) >> (4 * hh);
+      const unsigned see_lo = (unsigned)see, see_hi = (unsigned)(see >> 32);
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[kb][i] = (kb ? see_hi : see_lo) >> ((i & 3) + 8 * (i >> 2)) & 1 ? sc[kb][i] : -__builtin_inff();
+    }
+    float mx = -__builtin_inff();
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[kb][i]);
+    mx *= scale;
+    // the sums are scaled anew only where the maximum grows by more than 8 (weights stay below 2^8)
+    if (__any(mx > m_run + 8.f)) {
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float m_new = fmaxf(m_run, mx);
+      const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+      l_run *= alpha;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) o[d] *= alpha;
+      m_run = m_new;
+    }
+    float ps[4];
+    u32x4 pf;
+    auto weight = [&](int kb, int i) __attribute__((always_inline)) {
+      sc[kb][i] = __builtin_amdgcn_exp2f(sc[kb][i] * scale - m_run);
+      ps[i & 3] = kb == 0 && i < 4 ? sc[kb][i] : ps[i & 3] + sc[kb][i];
+    };
+#pragma unroll
+    for (int i = 0; i < 16; ++i) weight(0, i);
+    __builtin_amdgcn_sched_barrier(0);
+    each<0, 4 * ND>([&](auto i_) __attribute__((always_inline)) {
+      constexpr int i = decltype(i_)::value, j = i / ND, d = i % ND;
+      if constexpr (d == 0) {
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj) pf[jj] = pack_bf16x2(sc[j >> 1][8 * (j & 1) + 2 * jj], sc[j >> 1][8 * (j & 1) + 2 * jj + 1]);
+      }
+      o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, vf[j & 1][d]), as_bf16x8(pf), o[d], 0, 0, 0);
+      if constexpr (j < 2) {
+        vf[j][d] = read_v(j + 2, d);
+#pragma unroll
+        for (int k = i * 8 / ND; k < (i + 1) * 8 / ND; ++k) weight(1, k);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+    // ---- what was taken out of the tile
+    while (odd) {
+      const int kk = __ffsll(odd) - 1, key = kb0 + kk;
+      odd &= odd - 1;
+      if (key >= kv_end) break;
+      float p = 0.f;
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (i == ((kk >> 5) << 4 | (kk >> 3 & 3) << 2 | (kk & 3))) p = sc[i >> 4][i & 15];
+      p = __shfl(p, lr + 32 * (kk >> 2 & 1), 64);
+      const uint16_t* vp = a.v + ((size_t)known(bt[key >> a.bs_log2]) * nkv + kvh) * head_stride + (size_t)(key & (bs - 1)) * HD;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const uint16_t x = vp[32 * d + 8 * (i >> 2) + 4 * hh + (i & 3)];
+          if ((x & 0x7f80) == 0x7f80 && p != 0.f) o[d][i] += p * bf16_to_f32(x);
+        }
+    }
+  };
+  for (int kb0 = kv_begin; kb0 < kv_end; kb0 += 2 * KT) {
+    step(kb0, ic<0>{});
+    if (kb0 + KT < kv_end) step(kb0 + KT, ic<1>{});
+  }
+  l_run += __shfl_xor(l_run, 32, 64);
+  if (!row_valid) return;
+  const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+  if (runs_of(ctx, part) == 1) {
+    uint16_t* op = a.out + (size_t)(q0 + node) * a.out_stride + head * HD;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint2 x;
+        x.x = pack_bf16x2(o[d][4 * i] * inv, o[d][4 * i + 1] * inv);
+        x.y = pack_bf16x2(o[d][4 * i + 2] * inv, o[d][4 * i + 3] * inv);
+        *reinterpret_cast<uint2*>(op + 32 * d + 8 * i + 4 * hh) = x;
+      }
+    return;
+  }
+  const size_t at = (size_t)blockIdx.x * kRows + 32 * w + lr;
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<f32x4*>(a.part_o + at * HD + 32 * d + 8 * i + 4 * hh) =
+          f32x4{o[d][4 * i] * inv, o[d][4 * i + 1] * inv, o[d][4 * i + 2] * inv, o[d][4 * i + 3] * inv};
+  if (hh == 0) a.part_l[at] = l_run == 0.f ? -__builtin_inff() : m_run + __builtin_amdgcn_logf(l_run);
+}
+
+// A wave per row: its runs' results, weighed by their sums.
+template <int HD>
+__global__ __launch_bounds__(256) void tree_runs_kernel(Args a) {
+  const int G = a.nh / a.nkv, tiles = (a.max_nodes * G + kRows - 1) / kRows;
+  const int unit = blockIdx.x / a.nkv, kvh = blockIdx.x - unit * a.nkv, seq = unit / tiles, mt = unit - seq * tiles;
+  const int lane = threadIdx.x & 63, in_tile = blockIdx.y * 4 + (threadIdx.x >> 6), r = mt * kRows + in_tile, node = r / G;
+  const int q0 = a.cu[seq];
+  if (q0 < 0 || node >= min(min(a.cu[seq + 1], a.rows) - q0, a.max_nodes)) return;
+  const int part = run_length(a, lane), mine = runs_of(context_of(a, seq), part);
+  if (mine == 1) return;
+  int first = 0;
+  for (int s0 = 0; s0 <= seq; s0 += 64) {
+    int runs, all;
+    const int before = runs_before(a, s0, part, lane, runs, all);
+    if (seq < s0 + 64) first += __shfl(before, seq - s0, 64);
+    else first += all;
+  }
+  const size_t at = (((size_t)first * tiles + mt) * a.nkv + kvh) * kRows + in_tile, step = (size_t)tiles * a.nkv * kRows;
+  constexpr int D = HD / 64;
+  float M = -__builtin_inff(), W = 0.f, acc[D] = {};
+  for (int i = 0; i < mine; ++i) M = fmaxf(M, a.part_l[at + i * step]);
+  for (int i = 0; i < mine; ++i) {
+    const float l = a.part_l[at + i * step];
+    if (l == -__builtin_inff()) continue;
+    const float wgt = exp2f(l - M);
+    W += wgt;
+#pragma unroll
+    for (int j = 0; j < D; ++j) acc[j] += wgt * a.part_o[(at + i * step) * HD + D * lane + j];
+  }
+  uint16_t* op = a.out + (size_t)(q0 + node) * a.out_stride + (kvh * G + r - node * G) * HD + D * lane;
+#pragma unroll
+  for (int j = 0; j < D; ++j) op[j] = f32_to_bf16(W == 0.f ? 0.f : acc[j] / W);
+}
+
+template <int HD>
+int launch(const Args& a, hipStream_t s) {
+  const int tiles = (a.max_nodes * (a.nh / a.nkv) + kRows - 1) / kRows;
+  tree_tiles_kernel<HD><<<(a.places + a.n_seqs) * tiles * a.nkv, kWaves * 64, 0, s>>>(a);
+  DGI_CHECK_LAUNCH();
+  if (a.places > 1) {
+    tree_runs_kernel<HD><<<dim3(a.n_seqs * tiles * a.nkv, kRows / 4), 256, 0, s>>>(a);
+    DGI_CHECK_LAUNCH();
+  }
+  return 0;
+}
+
+}  // namespace
+
+extern "C" int dgi_tree_tiles(const void* q, long long q_stride, const void* k, const void* v, const int* tables, int table_stride,
+                              int table_cols, int n_seqs, int num_blocks, int rows, const int* cu, const int* ctx, const void* mask,
+                              int mask_stride, int max_nodes, void* out, long long out_stride, float* part_o, float* part_l, int places,
+                              int min_part, int nh, int nkv, int hd, int block_size, float scale, hipStream_t s) {
+  if (n_seqs == 0 || rows == 0) return 0;
+  Args a{(const uint16_t*)q, q_stride, (const uint16_t*)k, (const uint16_t*)v, tables, table_stride, table_cols, n_seqs, num_blocks, rows, cu, ctx,
+         (const unsigned long long*)mask, mask_stride, max_nodes, (uint16_t*)out, out_stride, part_o, part_l, places, min_part, nh, nkv, 0,
+         scale * 1.4426950408889634f};
+  while ((1 << a.bs_log2) < block_size) ++a.bs_log2;
+  if (hd == 64) return launch<64>(a, s);
+  if (hd == 128) return launch<128>(a, s);
+  return -5;
+}
