@@ -30,7 +30,7 @@ int dgi_paged_tree(const void* q, long long q_stride, const void* k, const void*
                    int block_size, float scale, hipStream_t s);
 int dgi_tree_tiles(const void* q, long long q_stride, const void* k, const void* v, const int* tables, int table_stride, int table_cols,
                    int n_seqs, int num_blocks, int rows, const int* cu, const int* ctx, const void* mask, int mask_stride, int max_nodes,
-                   void* out, long long out_stride, float* part_o, float* part_l, int places, int min_part, int nh, int nkv, int hd,
+                   void* out, long long out_stride, float* part_o, float* part_l, int shares, int least, int nh, int nkv, int hd,
                    int block_size, float scale, hipStream_t s);
 }
 
@@ -247,19 +247,19 @@ void paged_tree(at::Tensor out, const at::Tensor& q, const at::Tensor& k, const 
   const c10::DeviceGuard guard(at_.dev);
   const int64_t G = nh / nkv, width = tables.size(1) * at_.page;
   if (max_nodes * G > 32 && at_.hd <= 128) {
-    const int64_t tiles = (max_nodes * G + 127) / 128, min_part = 256;
-    const int64_t places = std::max<int64_t>(1, std::min<int64_t>({1024 / (tiles * nkv), S * (width + min_part - 1) / min_part}));
-    TORCH_CHECK_VALUE((places + S) * tiles * nkv <= kInt, op, ": too many sequences");
+    const int64_t tiles = (max_nodes * G + 127) / 128, least = 4;
+    const int64_t shares = std::max<int64_t>(1, std::min<int64_t>(512 / nkv, (S * tiles * ((width + 63) / 64) + least - 1) / least));
+    TORCH_CHECK_VALUE(S * tiles * nkv <= kInt, op, ": too many sequences");
     at::Tensor part_o, part_l;
-    if (places > 1) {
-      part_l = at::empty({(places + S) * tiles * nkv * 128}, q.options().dtype(at::kFloat));
-      part_o = at::empty({(places + S) * tiles * nkv * 128 * at_.hd}, q.options().dtype(at::kFloat));
+    if (shares > 1) {
+      part_l = at::empty({shares * nkv * 2 * 128}, q.options().dtype(at::kFloat));
+      part_o = at::empty({shares * nkv * 2 * 128 * at_.hd}, q.options().dtype(at::kFloat));
     }
     check_rc(dgi_tree_tiles(q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(), tables.data_ptr<int>(), (int)tables.stride(0),
                             (int)tables.size(1), (int)S, (int)k.size(0), (int)q.size(0), cu.data_ptr<int>(), ctx.data_ptr<int>(),
                             mask.data_ptr(), (int)mask.stride(0), (int)max_nodes, out.data_ptr(), out.stride(0),
-                            places > 1 ? part_o.data_ptr<float>() : nullptr, places > 1 ? part_l.data_ptr<float>() : nullptr, (int)places,
-                            (int)min_part, (int)nh, (int)nkv, (int)at_.hd, (int)at_.page, (float)scale, cur_stream()), op);
+                            shares > 1 ? part_o.data_ptr<float>() : nullptr, shares > 1 ? part_l.data_ptr<float>() : nullptr, (int)shares,
+                            (int)least, (int)nh, (int)nkv, (int)at_.hd, (int)at_.page, (float)scale, cur_stream()), op);
     return;
   }
   const int64_t cols = dgi_tree_columns((int)max_nodes, (int)G), tiles = (max_nodes * G + cols - 1) / cols;

@@ -6,9 +6,9 @@
 // the operand of O^T += V^T P^T where they lie.  Only the tiles that hold the tree's keys are masked.
 //
 // Bound by the matrix cores where there are many pairs (4 nodes n heads hd products a key), by the cache's bytes where there are few; with
-// few sequences also by how many workgroups share the keys.  Runs are cut on the device, to one length for all sequences: about `places`
-// of them in all, so that a long context beside short ones does not hold up the launch.  Runs of one sequence are added up by a second
-// launch.
+// few sequences also by how many workgroups share the keys.  The tiles of 64 keys of all (128 rows, sequence) of a kv head, one after
+// another, are dealt out in equal shares, so that a long context beside short ones does not hold up the launch; what a share's ends
+// cut is added up by a second launch.
 #include "../prefill_attention_kernel.h"
 
 using namespace dgi;
@@ -31,83 +31,119 @@ struct Args {
   int mask_stride, max_nodes;
   uint16_t* out;
   long long out_stride;
-  float* part_o;      // [run][tile][kv head][128][HD] of normalised sums, [run][tile][kv head][128] of their log2 sums
+  float* part_o;      // [share][kv head][2][128][HD] of normalised sums, [share][kv head][2][128] of their log2 sums
   float* part_l;
-  int places, min_part, nh, nkv, bs_log2;
+  int shares, least, nh, nkv, bs_log2;      // shares of a kv head at most, steps of a share at least
   float scale_log2;
 };
 
-__device__ __forceinline__ int context_of(const Args& a, int s) { return min(max(a.ctx[s], 0), a.table_cols << a.bs_log2); }
-
-__device__ __forceinline__ int runs_of(int ctx, int part) { return max(1, (ctx + part - 1) / part); }
-
-// The length of a run: all contexts cut into `places` in all, of min_part keys at least, a multiple of a tile and of a page.  One wave.
-__device__ int run_length(const Args& a, int lane) {
-  long long sum = 0;
-  for (int s = lane; s < a.n_seqs; s += 64) sum += context_of(a, s);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-  const int unit = max(KT, 1 << a.bs_log2);
-  const int part = (int)max((long long)a.min_part, (sum + a.places - 1) / a.places);
-  return (part + unit - 1) / unit * unit;
+// A sequence: its first row, its nodes, its row tiles, its context, and the steps (tiles of 64 keys, one for an empty context) that each row
+// tile takes.
+struct Seq {
+  int q0, nodes, tiles, ctx, steps;
+};
+// kLead more steps go into the deal for each: what it costs to begin and end one (10 us where a step takes 2)
+constexpr int kLead = 4;
+__device__ __forceinline__ Seq sequence(const Args& a, int s) {
+  if (s >= a.n_seqs) return {0, 0, 0, 0, 0};
+  const int q0 = a.cu[s], q1 = a.cu[s + 1], ctx = min(max(a.ctx[s], 0), a.table_cols << a.bs_log2);
+  const int nodes = q0 < 0 ? 0 : max(0, min(min(q1, a.rows) - q0, a.max_nodes));
+  return {q0, nodes, (nodes * (a.nh / a.nkv) + kRows - 1) / kRows, ctx, kLead + max(1, (ctx + KT - 1) / KT)};
 }
 
-// Runs of the sequences before lane's, for the 64 from s0 on; `runs`: the lane's own, `all`: of all 64.  One wave.
-__device__ __forceinline__ int runs_before(const Args& a, int s0, int part, int lane, int& runs, int& all) {
-  runs = s0 + lane < a.n_seqs ? runs_of(context_of(a, s0 + lane), part) : 0;
-  int sum = runs;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int x = __shfl_up(sum, o, 64);
-    if (lane >= o) sum += x;
+// The order of a kv head's steps: row tile 0 of every sequence, row tile 1, ..  One wave counts; `first` is its lane's sequence, of the first
+// 64; results are in all lanes.
+__device__ int steps_before(const Args& a, const Seq& first, int lane, int mt, int seq) {      // sequences before `seq` in row tile mt, all tiles before it
+  long long sum = 0;
+  Seq q = first;
+  for (int s0 = 0;;) {
+    sum += (long long)q.steps * (min(q.tiles, mt) + (s0 + lane < seq && q.tiles > mt ? 1 : 0));
+    if ((s0 += 64) >= a.n_seqs) break;
+    q = sequence(a, s0 + lane);
   }
-  all = __shfl(sum, 63, 64);
-  return sum - runs;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  return (int)min(sum, 0x7fffffffll);
+}
+// steps of a share
+__device__ __forceinline__ int share_of(const Args& a, const Seq& first, int lane) {
+  return max(a.least, (steps_before(a, first, lane, 1 << 20, 0) + a.shares - 1) / a.shares);
+}
+// whose step `at` is; row tile -1: behind the last one
+struct Place {
+  int mt, seq, step;
+};
+__device__ Place place_of(const Args& a, const Seq& first, int lane, int at) {
+  for (int mt = 0, before = 0;; ++mt) {
+    int any = 0;
+    Seq q = first;
+    for (int s0 = 0;;) {
+      const int mine = q.tiles > mt ? q.steps : 0;
+      int sum = mine;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int x = __shfl_up(sum, o, 64);
+        if (lane >= o) sum += x;
+      }
+      const int from = before + sum - mine;
+      const unsigned long long here = __ballot(at >= from && at < from + mine);
+      if (here) {
+        const int l = __ffsll(here) - 1;
+        return {mt, s0 + l, at - __shfl(from, l, 64)};
+      }
+      const int all = __shfl(sum, 63, 64);
+      before += all;
+      any += all;
+      if ((s0 += 64) >= a.n_seqs) break;
+      q = sequence(a, s0 + lane);
+    }
+    if (!any) return {-1, 0, 0};
+  }
 }
 
 template <int HD>
 __global__ __launch_bounds__(kWaves * 64, 2) void tree_tiles_kernel(Args a) {
   __shared__ __attribute__((aligned(16))) uint16_t lds[2 * KT * 2 * HD];
-  __shared__ int s_seq, s_run, s_part;
-  const int G = a.nh / a.nkv, tiles = (a.max_nodes * G + kRows - 1) / kRows;
+  __shared__ int s_place[4];
+  __shared__ unsigned s_odd[kWaves];
+  const int G = a.nh / a.nkv, nkv = a.nkv, bs = 1 << a.bs_log2;
   // kv heads side by side: with eight of them each has an XCD's L2 to itself
-  const int unit = blockIdx.x / a.nkv, kvh = blockIdx.x - unit * a.nkv, work = unit / tiles, mt = unit - work * tiles;
+  const int share = blockIdx.x / nkv, kvh = blockIdx.x - share * nkv;
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   if (w == 0) {
-    const int part = run_length(a, lane);
-    int seq = -1, run = 0;
-    for (int s0 = 0, done = 0; s0 < a.n_seqs && seq < 0; s0 += 64) {
-      int runs, all;
-      const int before = done + runs_before(a, s0, part, lane, runs, all);
-      const unsigned long long mine = __ballot(work >= before && work < before + runs);
-      if (mine) {
-        const int l = __ffsll(mine) - 1;
-        seq = s0 + l;
-        run = work - __shfl(before, l, 64);
-      }
-      done += all;
-    }
+    const Seq first = sequence(a, lane);
+    const int len = share_of(a, first, lane);
+    const Place p = (long long)share * len > 0x7fffffff ? Place{-1, 0, 0} : place_of(a, first, lane, share * len);
     if (lane == 0) {
-      s_seq = seq;
-      s_run = run;
-      s_part = part;
+      s_place[0] = p.mt;
+      s_place[1] = p.seq;
+      s_place[2] = p.step;
+      s_place[3] = len;
     }
   }
   __syncthreads();
-  const int seq = __builtin_amdgcn_readfirstlane(s_seq), part = __builtin_amdgcn_readfirstlane(s_part);
-  if (seq < 0) return;
-  const int q0 = a.cu[seq], nodes = q0 < 0 ? 0 : min(min(a.cu[seq + 1], a.rows) - q0, a.max_nodes);
-  if (mt * kRows >= nodes * G) return;
-  const int ctx = context_of(a, seq), kv_begin = __builtin_amdgcn_readfirstlane(s_run) * part, kv_end = min(kv_begin + part, ctx);
-  const int bs = 1 << a.bs_log2;
+  int mt = __builtin_amdgcn_readfirstlane(s_place[0]), seq = __builtin_amdgcn_readfirstlane(s_place[1]);
+  int step0 = __builtin_amdgcn_readfirstlane(s_place[2]), left = __builtin_amdgcn_readfirstlane(s_place[3]);
+  if (mt < 0) return;
+  const int most = (a.max_nodes * G + kRows - 1) / kRows;
+  for (; left > 0; step0 = 0) {      // a sequence's row tile, or the part of it that is the share's
+  Seq sq = sequence(a, seq);
+  while (sq.tiles <= mt) {
+    if (++seq >= a.n_seqs) {
+      seq = 0;
+      if (++mt >= most) return;
+    }
+    sq = sequence(a, seq);
+  }
+  const int q0 = sq.q0, nodes = sq.nodes, ctx = sq.ctx, dealt = min(sq.steps - step0, left);
+  left -= dealt;
+  // without the lead: steps [begin, end) of the sequence
+  const int begin = max(step0 - kLead, 0), end = step0 + dealt - kLead;
+  if (end <= begin) return;      // a lead alone: whoever has the next share begins
+  const int kv_begin = min(begin * KT, ctx), kv_end = min(end * KT, ctx);
+  const bool begins = begin == 0, whole = begins && end == sq.steps - kLead;
   const int* bt = a.tables + (size_t)seq * a.table_stride;
-  const int nkv = a.nkv;
-
-  // a page that is not in the cache: its keys are not there, page 0 is read in its place
-  bool bad = false;
-  for (int e = (kv_begin >> a.bs_log2) + tid; e < (kv_end + bs - 1) >> a.bs_log2; e += kWaves * 64) bad = bad || (unsigned)bt[e] >= (unsigned)a.num_blocks;
-  bad = __syncthreads_or(bad);
 
   const int lr = lane & 31, hh = lane >> 5;
   const int r = mt * kRows + 32 * w + lr, node = r / G, head = kvh * G + r - node * G;
@@ -116,18 +152,6 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_tiles_kernel(Args a) {
   const unsigned long long tmask = row_valid ? a.mask[(size_t)seq * a.mask_stride + node] : 0;
 
   constexpr int NS = HD / 16, ND = HD / 32, CH = HD / 8;
-  u32x4 qf[NS];
-  {
-    const uint16_t* qp = a.q + (size_t)(q0 + (row_valid ? node : 0)) * a.q_stride + (row_valid ? head : 0) * HD;
-#pragma unroll
-    for (int s = 0; s < NS; ++s) qf[s] = row_valid ? *reinterpret_cast<const u32x4*>(qp + 16 * s + 8 * hh) : u32x4{0, 0, 0, 0};
-    __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): or every tile's first product waits for the next tile's loads
-    // the softmax takes maxima of raw scores: a negative scale is the query's sign, zero stays above it (unseen keys are -inf)
-    if (a.scale_log2 < 0.f) {
-#pragma unroll
-      for (int s = 0; s < NS; ++s) qf[s] ^= 0x80008000u;
-    }
-  }
   const float scale = fmaxf(fabsf(a.scale_log2), 1e-30f);
   float m_run = -1e30f, l_run = 0.f;
   f32x16 o[ND];
@@ -191,14 +215,27 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_tiles_kernel(Args a) {
       load_chunk((const char*)(a.v + from + 8 * v_slot<HD>(row0 + row, part_lane % CH)), vl + p * 1024);
     }
   };
-  int id = 0;
+  // The first tile's page id, the queries, a look at the run's pages, then the first tile: three round trips, not one behind the other.
+  int id = kv_end > kv_begin ? read_id(kv_begin) : 0;
+  u32x4 qf[NS];
+  const uint16_t* qp = a.q + (size_t)(q0 + (row_valid ? node : 0)) * a.q_stride + (row_valid ? head : 0) * HD;
+#pragma unroll
+  for (int s = 0; s < NS; ++s) qf[s] = row_valid ? *reinterpret_cast<const u32x4*>(qp + 16 * s + 8 * hh) : u32x4{0, 0, 0, 0};
+  // a page that is not in the cache: its keys are not there, page 0 is read in its place
+  bool bad = false;
+  for (int e = (kv_begin >> a.bs_log2) + tid; e < (kv_end + bs - 1) >> a.bs_log2; e += kWaves * 64) bad = bad || (unsigned)bt[e] >= (unsigned)a.num_blocks;
+  bad = __syncthreads_or(bad);      // and all have read the LDS of the part before
   if (kv_end > kv_begin) {
-    id = read_id(kv_begin);
     if (full(kv_begin)) {
       at_page(id, kv_begin + row0);
       each<0, 2 * NP>([&](auto l) __attribute__((always_inline)) { load(l, 0); });
     } else load_part(kv_begin, 0, id);
     id = read_id(kv_begin + KT);
+  }
+  // the softmax takes maxima of raw scores: a negative scale is the query's sign, zero stays above it (unseen keys are -inf)
+  if (a.scale_log2 < 0.f) {
+#pragma unroll
+    for (int s = 0; s < NS; ++s) qf[s] ^= 0x80008000u;
   }
   // LDS addresses of this lane's operands in stage 0: keys lr, dims 16 s + 8 hh ..; values of dims 32 d .., keys 4 hh + tq
   typedef __attribute__((address_space(3))) const char* lds_at;
@@ -229,32 +266,32 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_tiles_kernel(Args a) {
     // number: they are taken out of the tile here and added below where the weight is not zero.
     unsigned long long odd = 0;
     if (kb0 + KT > tree_key) {
-      uint16_t* vt = lds + stage * KT * 2 * HD + KT * HD;
-#pragma unroll 1
-      for (int p = 0; p < KT * CH / 64; ++p) {
-        const u32x4 x = *reinterpret_cast<const u32x4*>(vt + p * 512 + lane * 8);
+      // a wave looks at the rows that it staged; row r of the tile is bit r
+      uint16_t* vt = lds + stage * KT * 2 * HD + KT * HD + row0 * HD;
+      unsigned mine = 0;
+      u32x4 x[NP];
+#pragma unroll
+      for (int p = 0; p < NP; ++p) x[p] = *reinterpret_cast<const u32x4*>(vt + p * 512 + lane * 8);
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
         bool is = false;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) is = is || (x[j] & 0x7f80u) == 0x7f80u || (x[j] & 0x7f800000u) == 0x7f800000u;
-        const unsigned long long b = __ballot(is);
-        for (int i = 0; i < 64 / CH; ++i)
-          if (b >> (i * CH) & (CH == 16 ? 0xffffull : 0xffull)) odd |= 1ull << (p * (64 / CH) + i);
-      }
-      __syncthreads();      // all have looked
-      if (odd) {
-#pragma unroll 1
-        for (int p = w; p < KT * CH / 64; p += kWaves) {
-          u32x4* at_v = reinterpret_cast<u32x4*>(vt + p * 512 + lane * 8);
-          u32x4 x = *at_v;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if ((x[j] & 0x7f80u) == 0x7f80u) x[j] &= 0xffff0000u;
-            if ((x[j] & 0x7f800000u) == 0x7f800000u) x[j] &= 0xffffu;
-          }
-          *at_v = x;
+        for (int j = 0; j < 4; ++j) {
+          const bool lo_odd = (x[p][j] & 0x7f80u) == 0x7f80u, hi_odd = (x[p][j] & 0x7f800000u) == 0x7f800000u;
+          is = is || lo_odd || hi_odd;
+          x[p][j] &= (lo_odd ? 0xffff0000u : ~0u) & (hi_odd ? 0xffffu : ~0u);
         }
-        __syncthreads();
+        const unsigned long long b = __ballot(is);
+        if (b) {
+          *reinterpret_cast<u32x4*>(vt + p * 512 + lane * 8) = x[p];
+#pragma unroll
+          for (int i = 0; i < 64 / CH; ++i) mine |= (b >> (i * CH) & ((1ull << CH) - 1)) ? 1u << (p * (64 / CH) + i) : 0u;
+        }
       }
+      if (lane == 0) s_odd[w] = mine;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) odd |= (unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane(s_odd[i]) << (RW * i);
     }
     if (!wave_rows) return;
     // ---- S^T = K Q^T for two 32-key blocks: the first block's operands all under way before its products, the second's between them,
@@ -369,9 +406,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_tiles_kernel(Args a) {
     if (kb0 + KT < kv_end) step(kb0 + KT, ic<1>{});
   }
   l_run += __shfl_xor(l_run, 32, 64);
-  if (!row_valid) return;
   const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
-  if (runs_of(ctx, part) == 1) {
+  if (row_valid && whole) {
     uint16_t* op = a.out + (size_t)(q0 + node) * a.out_stride + head * HD;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
@@ -382,59 +418,85 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_tiles_kernel(Args a) {
         x.y = pack_bf16x2(o[d][4 * i + 2] * inv, o[d][4 * i + 3] * inv);
         *reinterpret_cast<uint2*>(op + 32 * d + 8 * i + 4 * hh) = x;
       }
-    return;
+  } else if (row_valid) {
+    // a share has one part at most that a share before has begun, and one that it begins and does not end
+    const size_t at = ((size_t)blockIdx.x * 2 + begins) * kRows + 32 * w + lr;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<f32x4*>(a.part_o + at * HD + 32 * d + 8 * i + 4 * hh) =
+            f32x4{o[d][4 * i] * inv, o[d][4 * i + 1] * inv, o[d][4 * i + 2] * inv, o[d][4 * i + 3] * inv};
+    if (hh == 0) a.part_l[at] = l_run == 0.f ? -__builtin_inff() : m_run + __builtin_amdgcn_logf(l_run);
   }
-  const size_t at = (size_t)blockIdx.x * kRows + 32 * w + lr;
-#pragma unroll
-  for (int d = 0; d < ND; ++d)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      *reinterpret_cast<f32x4*>(a.part_o + at * HD + 32 * d + 8 * i + 4 * hh) =
-          f32x4{o[d][4 * i] * inv, o[d][4 * i + 1] * inv, o[d][4 * i + 2] * inv, o[d][4 * i + 3] * inv};
-  if (hh == 0) a.part_l[at] = l_run == 0.f ? -__builtin_inff() : m_run + __builtin_amdgcn_logf(l_run);
+  ++seq;
+  }
 }
 
-// A wave per row: its runs' results, weighed by their sums.
+// The parts of a sequence's row tile that several shares have, weighed by their sums: HD / 8 lanes a row.
 template <int HD>
-__global__ __launch_bounds__(256) void tree_runs_kernel(Args a) {
-  const int G = a.nh / a.nkv, tiles = (a.max_nodes * G + kRows - 1) / kRows;
-  const int unit = blockIdx.x / a.nkv, kvh = blockIdx.x - unit * a.nkv, seq = unit / tiles, mt = unit - seq * tiles;
-  const int lane = threadIdx.x & 63, in_tile = blockIdx.y * 4 + (threadIdx.x >> 6), r = mt * kRows + in_tile, node = r / G;
-  const int q0 = a.cu[seq];
-  if (q0 < 0 || node >= min(min(a.cu[seq + 1], a.rows) - q0, a.max_nodes)) return;
-  const int part = run_length(a, lane), mine = runs_of(context_of(a, seq), part);
-  if (mine == 1) return;
-  int first = 0;
-  for (int s0 = 0; s0 <= seq; s0 += 64) {
-    int runs, all;
-    const int before = runs_before(a, s0, part, lane, runs, all);
-    if (seq < s0 + 64) first += __shfl(before, seq - s0, 64);
-    else first += all;
-  }
-  const size_t at = (((size_t)first * tiles + mt) * a.nkv + kvh) * kRows + in_tile, step = (size_t)tiles * a.nkv * kRows;
-  constexpr int D = HD / 64;
-  float M = -__builtin_inff(), W = 0.f, acc[D] = {};
-  for (int i = 0; i < mine; ++i) M = fmaxf(M, a.part_l[at + i * step]);
-  for (int i = 0; i < mine; ++i) {
-    const float l = a.part_l[at + i * step];
-    if (l == -__builtin_inff()) continue;
-    const float wgt = exp2f(l - M);
-    W += wgt;
+__global__ __launch_bounds__(256) void tree_parts_kernel(Args a) {
+  constexpr int L = HD / 8, R = 256 / L;
+  const int G = a.nh / a.nkv, most = (a.max_nodes * G + kRows - 1) / kRows;
+  const int unit = blockIdx.x / a.nkv, kvh = blockIdx.x - unit * a.nkv, seq = unit / most, mt = unit - seq * most;
+  const int lane = threadIdx.x & 63;
+  const Seq first = sequence(a, lane), sq = sequence(a, seq);
+  if (sq.tiles <= mt) return;
+  const int len = share_of(a, first, lane);
+  const int from = steps_before(a, first, lane, mt, seq), to = from + sq.steps - 1, s0 = (from + kLead) / len, s1 = to / len;
+  if (s0 == s1) return;
+  const int in_tile = blockIdx.y * R + threadIdx.x / L, r = mt * kRows + in_tile, node = r / G, d = threadIdx.x % L * 8;
+  if (node >= sq.nodes) return;
+  // the first part is one that its share begins, the others are not
+  auto at = [&](int s) { return ((size_t)(s * a.nkv + kvh) * 2 + (s == s0)) * kRows + in_tile; };
+  // several parts under way at a time
+  constexpr int U = 8;
+  float M = -__builtin_inff(), W = 0.f, acc[8] = {};
+  for (int s = s0; s <= s1; s += U) {
+    float l[U], m = M;
+    f32x4 x[U], y[U];
 #pragma unroll
-    for (int j = 0; j < D; ++j) acc[j] += wgt * a.part_o[(at + i * step) * HD + D * lane + j];
-  }
-  uint16_t* op = a.out + (size_t)(q0 + node) * a.out_stride + (kvh * G + r - node * G) * HD + D * lane;
+    for (int u = 0; u < U; ++u) {
+      const size_t p = at(min(s + u, s1));
+      l[u] = a.part_l[p];
+      x[u] = *reinterpret_cast<const f32x4*>(a.part_o + p * HD + d);
+      y[u] = *reinterpret_cast<const f32x4*>(a.part_o + p * HD + d + 4);
+    }
 #pragma unroll
-  for (int j = 0; j < D; ++j) op[j] = f32_to_bf16(W == 0.f ? 0.f : acc[j] / W);
+    for (int u = 0; u < U; ++u) {
+      if (s + u > s1) l[u] = -__builtin_inff();
+      m = fmaxf(m, l[u]);
+    }
+    if (m == -__builtin_inff()) continue;
+    const float old = exp2f(M - m);
+    M = m;
+    W *= old;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] *= old;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float wgt = exp2f(l[u] - M);
+      W += wgt;
+      if (wgt == 0.f) continue;      // of a part without keys
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        acc[j] += wgt * x[u][j];
+        acc[4 + j] += wgt * y[u][j];
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) acc[j] = W == 0.f ? 0.f : acc[j] / W;
+  *reinterpret_cast<u32x4*>(a.out + (size_t)(sq.q0 + node) * a.out_stride + (kvh * G + r - node * G) * HD + d) = pack8(acc);
 }
 
 template <int HD>
 int launch(const Args& a, hipStream_t s) {
-  const int tiles = (a.max_nodes * (a.nh / a.nkv) + kRows - 1) / kRows;
-  tree_tiles_kernel<HD><<<(a.places + a.n_seqs) * tiles * a.nkv, kWaves * 64, 0, s>>>(a);
+  tree_tiles_kernel<HD><<<a.shares * a.nkv, kWaves * 64, 0, s>>>(a);
   DGI_CHECK_LAUNCH();
-  if (a.places > 1) {
-    tree_runs_kernel<HD><<<dim3(a.n_seqs * tiles * a.nkv, kRows / 4), 256, 0, s>>>(a);
+  if (a.shares > 1) {
+    const int most = (a.max_nodes * (a.nh / a.nkv) + kRows - 1) / kRows;
+    tree_parts_kernel<HD><<<dim3(a.n_seqs * most * a.nkv, kRows * HD / 8 / 256), 256, 0, s>>>(a);
     DGI_CHECK_LAUNCH();
   }
   return 0;
@@ -444,11 +506,11 @@ int launch(const Args& a, hipStream_t s) {
 
 extern "C" int dgi_tree_tiles(const void* q, long long q_stride, const void* k, const void* v, const int* tables, int table_stride,
                               int table_cols, int n_seqs, int num_blocks, int rows, const int* cu, const int* ctx, const void* mask,
-                              int mask_stride, int max_nodes, void* out, long long out_stride, float* part_o, float* part_l, int places,
-                              int min_part, int nh, int nkv, int hd, int block_size, float scale, hipStream_t s) {
+                              int mask_stride, int max_nodes, void* out, long long out_stride, float* part_o, float* part_l, int shares,
+                              int least, int nh, int nkv, int hd, int block_size, float scale, hipStream_t s) {
   if (n_seqs == 0 || rows == 0) return 0;
   Args a{(const uint16_t*)q, q_stride, (const uint16_t*)k, (const uint16_t*)v, tables, table_stride, table_cols, n_seqs, num_blocks, rows, cu, ctx,
-         (const unsigned long long*)mask, mask_stride, max_nodes, (uint16_t*)out, out_stride, part_o, part_l, places, min_part, nh, nkv, 0,
+         (const unsigned long long*)mask, mask_stride, max_nodes, (uint16_t*)out, out_stride, part_o, part_l, shares, least, nh, nkv, 0,
          scale * 1.4426950408889634f};
   while ((1 << a.bs_log2) < block_size) ++a.bs_log2;
   if (hd == 64) return launch<64>(a, s);
