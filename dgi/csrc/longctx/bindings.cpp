@@ -24,7 +24,7 @@ int dgi_paged_selected(const void* q, long long q_stride, const void* k, const v
                        long long out_stride, float* part_o, float* part_l, int splits, int T, int nh, int nkv, int hd, int block_size,
                        float scale, hipStream_t s);
 int dgi_tree_columns(int max_nodes, int G);
-int dgi_paged_tree(const void* q, long long q_stride, const void* k, const void* v, const int* tables, int table_stride, int table_cols,
+int dgi_tree_rows(const void* q, long long q_stride, const void* k, const void* v, const int* tables, int table_stride, int table_cols,
                    int n_seqs, int num_blocks, int rows, const int* cu, const int* ctx, const void* mask, int mask_stride, int max_nodes,
                    void* out, long long out_stride, float* part_o, float* part_l, int splits, int min_part, int nh, int nkv, int hd,
                    int block_size, float scale, hipStream_t s);
@@ -221,8 +221,8 @@ void paged_selected(at::Tensor out, const at::Tensor& q, const at::Tensor& k, co
   const int64_t splits = std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(1, T * nkv), (count + least - 1) / least, 64}));
   at::Tensor part_o, part_l;
   if (splits > 1) {
-    part_o = at::empty({T * nkv * splits * 16 * at_.hd}, q.options().dtype(at::kFloat));
-    part_l = at::empty({T * nkv * splits * 16}, q.options().dtype(at::kFloat));
+    part_o = at::empty({T * nh * splits * at_.hd}, q.options().dtype(at::kFloat));
+    part_l = at::empty({T * nh * splits}, q.options().dtype(at::kFloat));
   }
   check_rc(dgi_paged_selected(q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(), tables.data_ptr<int>(), (int)tables.stride(0),
                               (int)tables.size(1), (int)tables.size(0), (int)k.size(0), ctx.data_ptr<int>(), rows, pages.data_ptr<int>(),
@@ -271,7 +271,7 @@ void paged_tree(at::Tensor out, const at::Tensor& q, const at::Tensor& k, const 
     part_o = at::empty({items * splits * cols * at_.hd}, q.options().dtype(at::kFloat));
     part_l = at::empty({items * splits * cols}, q.options().dtype(at::kFloat));
   }
-  check_rc(dgi_paged_tree(q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(), tables.data_ptr<int>(), (int)tables.stride(0),
+  check_rc(dgi_tree_rows(q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(), tables.data_ptr<int>(), (int)tables.stride(0),
                           (int)tables.size(1), (int)S, (int)k.size(0), (int)q.size(0), cu.data_ptr<int>(), ctx.data_ptr<int>(),
                           mask.data_ptr(), (int)mask.stride(0), (int)max_nodes, out.data_ptr(), out.stride(0),
                           splits > 1 ? part_o.data_ptr<float>() : nullptr, splits > 1 ? part_l.data_ptr<float>() : nullptr, (int)splits,

@@ -1,17 +1,11 @@
-// dgi/csrc/longctx/paged_rows.hip — attention of few rows over a paged cache: rows that each read pages of their own (paged_selected) and
-// drafted trees (paged_tree).
+// dgi/csrc/longctx/tree_rows.hip — attention of drafted trees of few (node, head) pairs over a paged cache.
 //
-//   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^(x_j - max x),  x_j = scale log2(e) q . k_j     over the keys j that a row sees,
-// in one pass over the keys with the running maximum and sum in fp32; a row that sees nothing is zero.
-//
-// A workgroup owns the query columns of one kv head (selected: the G heads of a row; tree: 16 NQ of the (node, head) pairs of a
-// sequence) and a run of keys; its waves take tiles of 32 keys in turn and are merged through LDS, runs of one row by a second launch.
-// Scores are formed transposed, S^T = K Q^T, so that a lane owns a query column and the weights stay in the registers that the product
-// O^T += V^T P^T takes them from; V is transposed on its way out of LDS.  Weights are rounded to bf16 for that product (as the cached
-// values are; their sum is taken before), everything else is fp32.
-//
-// Pages reach a workgroup as a list in LDS of what there is to read: the page, and how many of its keys are seen.  Entries without any
-// are left out, so that short rows and ragged lists cost what they hold.
+// Up to 32 pairs of a sequence's nodes and a kv head's group are the columns of one product (tree_tiles.hip has more of them).  A
+// workgroup owns them and a run of keys; its waves take tiles of 32 keys in turn and are merged through LDS, runs of one sequence by a
+// second launch.  Scores are formed transposed, S^T = K Q^T, so that a lane owns a query column and the weights stay in the registers
+// that the product O^T += V^T P^T takes them from; V is transposed on its way out of LDS.  Weights are rounded to bf16 for that product
+// (as the cached values are; their sum is taken before), everything else is fp32.  Bound by the cache's bytes where contexts are
+// long, else by the chain of loads that a run is.
 #include "../common.h"
 
 using namespace dgi;
@@ -34,11 +28,6 @@ struct Args {
   float* part_l;
   int splits, nh, nkv, bs_log2;
   float scale_log2;
-  // selected
-  const int* pages;
-  const int* row_seq;
-  int count;
-  // tree
   const int* cu;
   const unsigned long long* mask;
   int mask_stride, max_nodes, min_part;
@@ -63,8 +52,8 @@ __device__ __forceinline__ int tree_part(const Args& a, int ctx) {
   return (((ctx + n - 1) / n) + unit - 1) / unit * unit;
 }
 
-template <int HD, int NQ, int NW, bool TREE>
-__global__ __launch_bounds__(64 * NW) void paged_rows_kernel(Args a) {
+template <int HD, int NQ, int NW>
+__global__ __launch_bounds__(64 * NW) void tree_rows_kernel(Args a) {
   constexpr int KS = HD / 32, NC = HD / 16, VCH = HD / 8, NT = 64 * NW;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   int2* list = reinterpret_cast<int2*>(smem + NW * wave_lds<HD>());      // [kList] (page, keys seen)
@@ -77,45 +66,27 @@ __global__ __launch_bounds__(64 * NW) void paged_rows_kernel(Args a) {
   uint16_t* vt = reinterpret_cast<uint16_t*>(smem + w * wave_lds<HD>());
 
   // ---- whose rows, which keys
-  int seq, ctx, row0 = 0, nodes = 0, first_node = 0;
-  int lo, hi;      // tree: keys [lo, hi) of the sequence; selected: entries [lo, hi) of the row's list
-  if constexpr (TREE) {
-    const int tiles = (a.max_nodes * G + 16 * NQ - 1) / (16 * NQ);
-    seq = item / tiles;
-    row0 = a.cu[seq];
-    nodes = row0 < 0 ? 0 : min(min(a.cu[seq + 1], a.rows) - row0, a.max_nodes);
-    first_node = (item - seq * tiles) * 16 * NQ;                 // (node, head) pairs from here on
-    if (first_node >= nodes * G) return;
-    ctx = min(max(a.ctx[seq], 0), a.table_cols << a.bs_log2);
-    const int part = tree_part(a, ctx);
-    lo = split * part;
-    hi = min(lo + part, ctx);
-    if (lo >= hi && split > 0) return;
-  } else {
-    row0 = item;
-    seq = a.row_seq ? a.row_seq[item] : item;
-    ctx = a.ctx[item];
-    if (seq < 0 || seq >= a.n_seqs) ctx = 0, seq = 0;
-    const int part = (a.count + a.splits - 1) / a.splits;
-    lo = split * part;
-    hi = min(lo + part, a.count);
-    if (ctx <= 0) hi = lo;
-  }
+  const int tiles = (a.max_nodes * G + 16 * NQ - 1) / (16 * NQ), seq = item / tiles;
+  const int row0 = a.cu[seq], nodes = row0 < 0 ? 0 : min(min(a.cu[seq + 1], a.rows) - row0, a.max_nodes);
+  const int first_node = (item - seq * tiles) * 16 * NQ;                 // (node, head) pairs from here on
+  if (first_node >= nodes * G) return;
+  const int ctx = min(max(a.ctx[seq], 0), a.table_cols << a.bs_log2);
+  const int part = tree_part(a, ctx), lo = split * part, hi = min(lo + part, ctx);
+  if (lo >= hi && split > 0) return;
   const int* table = a.tables + (size_t)seq * a.table_stride;
-  const int* sel = TREE ? nullptr : a.pages + ((size_t)item * a.nkv + h) * a.count;
 
   // ---- queries: column qi of group n; fragments of the second operand, dims 32 s + 8 g ..
   u32x4 qf[NQ][KS];
-  unsigned long long bits[TREE ? NQ : 1];
+  unsigned long long bits[NQ];
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     const int r = first_node + 16 * n + qi;
-    const int node = TREE ? r / G : 0, head = h * G + (TREE ? r - node * G : r);
-    const bool live = TREE ? node < nodes : r < G;
+    const int node = r / G, head = h * G + r - node * G;
+    const bool live = node < nodes;
     const uint16_t* qp = a.q + (size_t)(row0 + (live ? node : 0)) * a.q_stride + (live ? head : 0) * HD + 8 * g;
 #pragma unroll
     for (int s = 0; s < KS; ++s) qf[n][s] = live ? *reinterpret_cast<const u32x4*>(qp + 32 * s) : u32x4{0, 0, 0, 0};
-    if constexpr (TREE) bits[n] = live ? a.mask[(size_t)seq * a.mask_stride + node] : 0;
+    bits[n] = live ? a.mask[(size_t)seq * a.mask_stride + node] : 0;
   }
   const int tree_key = ctx - nodes;      // the key of node 0
 
@@ -129,43 +100,15 @@ __global__ __launch_bounds__(64 * NW) void paged_rows_kernel(Args a) {
     for (int c = 0; c < NC; ++c) o[n][c] = f32x4{0, 0, 0, 0};
   }
 
-  const int per = TREE ? kList << a.bs_log2 : kList;
+  const int per = kList << a.bs_log2;
   for (int at = lo; at < hi; at += per) {
-    // ---- the list: tree: the pages of keys at .. (one after another, also those without a page, so that a place says which key it is)
+    // ---- the list: the pages of keys at .., also those that are not in the cache, so that a place says which key it is
     __syncthreads();
-    int entries;
-    if constexpr (TREE) {
-      const int n = min(per, hi - at);
-      entries = (n + bs - 1) >> a.bs_log2;
-      for (int e = tid; e < entries; e += NT) {
-        const int id = table[(at >> a.bs_log2) + e];
-        const bool there = id >= 0 && id < a.num_blocks;
-        list[e] = int2{there ? id : 0, there ? min(bs, hi - at - (e << a.bs_log2)) : 0};
-      }
-    } else {
-      entries = 0;
-      for (int e0 = at; e0 < min(at + per, hi); e0 += NT) {
-        const int e = e0 + tid;
-        int id = -1, seen = 0;
-        if (e < hi && e < at + per) {
-          const int ord = sel[e];
-          if (ord >= 0 && ord < a.table_cols && ((long long)ord << a.bs_log2) < ctx) {
-            id = table[ord];
-            seen = min(bs, ctx - (ord << a.bs_log2));
-          }
-        }
-        const bool there = id >= 0 && id < a.num_blocks;
-        const unsigned long long b = __ballot(there);
-        if (lane == 0) s_n[w] = __popcll(b);
-        __syncthreads();
-        int before = entries;
-        for (int v = 0; v < NW; ++v) {
-          if (v < w) before += s_n[v];
-          entries += s_n[v];
-        }
-        if (there) list[before + __popcll(b & ((1ull << lane) - 1))] = int2{id, seen};
-        __syncthreads();
-      }
+    const int n = min(per, hi - at), entries = (n + bs - 1) >> a.bs_log2;
+    for (int e = tid; e < entries; e += NT) {
+      const int id = table[(at >> a.bs_log2) + e];
+      const bool there = id >= 0 && id < a.num_blocks;
+      list[e] = int2{there ? id : 0, there ? min(bs, hi - at - (e << a.bs_log2)) : 0};
     }
     __syncthreads();
     const int keys = entries << a.bs_log2, ntiles = (keys + 31) >> 5;
@@ -194,21 +137,19 @@ __global__ __launch_bounds__(64 * NW) void paged_rows_kernel(Args a) {
       // Values of the tree's keys that are infinite or no numbers reach the rows that see them alone, but zero times such a value is no
       // number: they are taken out here and added below where the weight is not zero.
       unsigned odd = 0;
-      if constexpr (TREE) {
-        if (at + 32 * t + 32 > tree_key) {
+      if (at + 32 * t + 32 > tree_key) {
 #pragma unroll
-          for (int i = 0; i < VCH / 2; ++i) {
-            bool is = false;
+        for (int i = 0; i < VCH / 2; ++i) {
+          bool is = false;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const bool lo_odd = (vr[i][j] & 0x7f80u) == 0x7f80u, hi_odd = (vr[i][j] & 0x7f800000u) == 0x7f800000u;
-              is = is || lo_odd || hi_odd;
-              vr[i][j] &= (lo_odd ? 0xffff0000u : ~0u) & (hi_odd ? 0xffffu : ~0u);
-            }
-            const unsigned long long b = __ballot(is);
-#pragma unroll
-            for (int j = 0; j < 64 / VCH; ++j) odd |= (b >> (j * VCH) & ((1ull << VCH) - 1)) ? 1u << (i * (64 / VCH) + j) : 0u;
+          for (int j = 0; j < 4; ++j) {
+            const bool lo_odd = (vr[i][j] & 0x7f80u) == 0x7f80u, hi_odd = (vr[i][j] & 0x7f800000u) == 0x7f800000u;
+            is = is || lo_odd || hi_odd;
+            vr[i][j] &= (lo_odd ? 0xffff0000u : ~0u) & (hi_odd ? 0xffffu : ~0u);
           }
+          const unsigned long long b = __ballot(is);
+#pragma unroll
+          for (int j = 0; j < 64 / VCH; ++j) odd |= (b >> (j * VCH) & ((1ull << VCH) - 1)) ? 1u << (i * (64 / VCH) + j) : 0u;
         }
       }
       // ---- which of the lane's keys (16 u + 4 g + i) are there
@@ -236,10 +177,8 @@ __global__ __launch_bounds__(64 * NW) void paged_rows_kernel(Args a) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             bool see = there[u][i];
-            if constexpr (TREE) {
-              const int node = at + 32 * t + 16 * u + 4 * g + i - tree_key;
-              see = see && (node < 0 || (bits[n] >> (node & 63) & 1));
-            }
+            const int node = at + 32 * t + 16 * u + 4 * g + i - tree_key;
+            see = see && (node < 0 || (bits[n] >> (node & 63) & 1));
             x[u][i] = see ? acc[i] * a.scale_log2 : -__builtin_inff();
             mx = fmaxf(mx, x[u][i]);
           }
@@ -280,22 +219,20 @@ __global__ __launch_bounds__(64 * NW) void paged_rows_kernel(Args a) {
 #pragma unroll
         for (int n = 0; n < NQ; ++n) o[n][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(vf), as_bf16x8(pf[n]), o[n][c], 0, 0, 0);
       }
-      if constexpr (TREE) {
-        for (; odd; odd &= odd - 1) {      // what was taken out: key kk of the tile
-          const int kk = __ffs(odd) - 1, tok = 32 * t + kk, j = (kk >> 4) * 4 + (kk & 3);
-          const uint16_t* vp = a.v + ((((size_t)list[tok >> a.bs_log2].x * a.nkv + h) << a.bs_log2) + (tok & (bs - 1))) * HD + 4 * g;
+      for (; odd; odd &= odd - 1) {      // what was taken out: key kk of the tile
+        const int kk = __ffs(odd) - 1, tok = 32 * t + kk, j = (kk >> 4) * 4 + (kk & 3);
+        const uint16_t* vp = a.v + ((((size_t)list[tok >> a.bs_log2].x * a.nkv + h) << a.bs_log2) + (tok & (bs - 1))) * HD + 4 * g;
 #pragma unroll
-          for (int n = 0; n < NQ; ++n) {
-            const uint32_t two = __shfl(j & 4 ? (j & 2 ? pf[n][3] : pf[n][2]) : (j & 2 ? pf[n][1] : pf[n][0]), 16 * (kk >> 2 & 3) + qi, 64);
-            const float p = __uint_as_float(j & 1 ? two & 0xffff0000u : two << 16);
+        for (int n = 0; n < NQ; ++n) {
+          const uint32_t two = __shfl(j & 4 ? (j & 2 ? pf[n][3] : pf[n][2]) : (j & 2 ? pf[n][1] : pf[n][0]), 16 * (kk >> 2 & 3) + qi, 64);
+          const float p = __uint_as_float(j & 1 ? two & 0xffff0000u : two << 16);
 #pragma unroll
-            for (int c = 0; c < NC; ++c)
+          for (int c = 0; c < NC; ++c)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const uint16_t x = vp[16 * c + i];
-                if ((x & 0x7f80) == 0x7f80 && p != 0.f) o[n][c][i] += p * bf16_to_f32(x);
-              }
-          }
+            for (int i = 0; i < 4; ++i) {
+              const uint16_t x = vp[16 * c + i];
+              if ((x & 0x7f80) == 0x7f80 && p != 0.f) o[n][c][i] += p * bf16_to_f32(x);
+            }
         }
       }
     }
@@ -308,7 +245,7 @@ __global__ __launch_bounds__(64 * NW) void paged_rows_kernel(Args a) {
       ml[w * 32 * NQ + 16 * n + qi] = m_run[n];
       ml[w * 32 * NQ + 16 * NQ + 16 * n + qi] = l_run[n];
     }
-  const bool split_up = TREE ? tree_part(a, ctx) < ctx : a.splits > 1;
+  const bool split_up = part < ctx;
   const size_t slab = (((size_t)item * a.nkv + h) * a.splits + split) * 16 * NQ;
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
@@ -322,8 +259,8 @@ __global__ __launch_bounds__(64 * NW) void paged_rows_kernel(Args a) {
     for (int idx = tid; idx < 16 * HD; idx += NT) {
       const int qq = idx / HD, d = idx - qq * HD;
       const int r = first_node + 16 * n + qq;
-      const int node = TREE ? r / G : 0, head = h * G + (TREE ? r - node * G : r);
-      if (TREE ? node >= nodes : r >= G) continue;
+      const int node = r / G, head = h * G + r - node * G;
+      if (node >= nodes) continue;
       float M = -__builtin_inff();
 #pragma unroll
       for (int v = 0; v < NW; ++v) M = fmaxf(M, ml[v * 32 * NQ + 16 * n + qq]);
@@ -347,24 +284,15 @@ __global__ __launch_bounds__(64 * NW) void paged_rows_kernel(Args a) {
 }
 
 // Runs of the same columns: weighed by their sums.
-template <int HD, int NQ, bool TREE>
-__global__ __launch_bounds__(HD) void paged_rows_reduce_kernel(Args a) {
+template <int HD, int NQ>
+__global__ __launch_bounds__(HD) void tree_rows_reduce_kernel(Args a) {
   const int item = blockIdx.x / a.nkv, h = blockIdx.x - item * a.nkv, col = blockIdx.y, d = threadIdx.x, G = a.nh / a.nkv;
-  int row, head, runs = a.splits;
-  if constexpr (TREE) {
-    const int tiles = (a.max_nodes * G + 16 * NQ - 1) / (16 * NQ), seq = item / tiles;
-    const int r = (item - seq * tiles) * 16 * NQ + col, node = r / G;
-    if (a.cu[seq] < 0 || node >= min(min(a.cu[seq + 1], a.rows) - a.cu[seq], a.max_nodes)) return;
-    const int ctx = min(max(a.ctx[seq], 0), a.table_cols << a.bs_log2), part = tree_part(a, ctx);
-    if (part >= ctx) return;
-    runs = (ctx + part - 1) / part;
-    row = a.cu[seq] + node;
-    head = h * G + r - node * G;
-  } else {
-    if (col >= G) return;
-    row = item;
-    head = h * G + col;
-  }
+  const int tiles = (a.max_nodes * G + 16 * NQ - 1) / (16 * NQ), seq = item / tiles;
+  const int r = (item - seq * tiles) * 16 * NQ + col, node = r / G;
+  if (a.cu[seq] < 0 || node >= min(min(a.cu[seq + 1], a.rows) - a.cu[seq], a.max_nodes)) return;
+  const int ctx = min(max(a.ctx[seq], 0), a.table_cols << a.bs_log2), part = tree_part(a, ctx);
+  if (part >= ctx) return;
+  const int runs = (ctx + part - 1) / part, row = a.cu[seq] + node, head = h * G + r - node * G;
   const size_t base = ((size_t)item * a.nkv + h) * a.splits * 16 * NQ + col;
   float M = -__builtin_inff();
   for (int i = 0; i < runs; ++i) M = fmaxf(M, a.part_l[base + (size_t)i * 16 * NQ]);
@@ -379,24 +307,23 @@ __global__ __launch_bounds__(HD) void paged_rows_reduce_kernel(Args a) {
   a.out[(size_t)row * a.out_stride + head * HD + d] = f32_to_bf16(W == 0.f ? 0.f : acc / W);
 }
 
-template <int HD, int NQ, int NW, bool TREE>
+template <int HD, int NQ, int NW>
 int launch(const Args& a, int items, hipStream_t s) {
   const int lds = NW * wave_lds<HD>() + kList * 8 + NW * 32 * NQ * 4 + (NW + 1) * 4;
-  paged_rows_kernel<HD, NQ, NW, TREE><<<dim3(a.nkv * items, a.splits), 64 * NW, lds, s>>>(a);
+  tree_rows_kernel<HD, NQ, NW><<<dim3(a.nkv * items, a.splits), 64 * NW, lds, s>>>(a);
   DGI_CHECK_LAUNCH();
   if (a.splits > 1) {
-    const int G = a.nh / a.nkv, cols = TREE ? 16 * NQ : G;
-    paged_rows_reduce_kernel<HD, NQ, TREE><<<dim3(a.nkv * items, cols), HD, 0, s>>>(a);
+    tree_rows_reduce_kernel<HD, NQ><<<dim3(a.nkv * items, 16 * NQ), HD, 0, s>>>(a);
     DGI_CHECK_LAUNCH();
   }
   return 0;
 }
 
-template <int NQ, int NW, bool TREE>
+template <int NQ, int NW>
 int launch_dims(const Args& a, int items, int hd, hipStream_t s) {
-  if (hd == 64) return launch<64, NQ, NW, TREE>(a, items, s);
-  if (hd == 128) return launch<128, NQ, NW, TREE>(a, items, s);
-  if (hd == 256) return launch<256, NQ, NW, TREE>(a, items, s);
+  if (hd == 64) return launch<64, NQ, NW>(a, items, s);
+  if (hd == 128) return launch<128, NQ, NW>(a, items, s);
+  if (hd == 256) return launch<256, NQ, NW>(a, items, s);
   return -5;
 }
 
@@ -405,39 +332,7 @@ int launch_dims(const Args& a, int items, int hd, hipStream_t s) {
 // Query columns of a workgroup of a tree: 16 or 32 of its (node, head) pairs.
 extern "C" int dgi_tree_columns(int max_nodes, int G) { return max_nodes * G <= 16 ? 16 : 32; }
 
-extern "C" int dgi_paged_selected(const void* q, long long q_stride, const void* k, const void* v, const int* tables, int table_stride,
-                                  int table_cols, int n_seqs, int num_blocks, const int* ctx, const int* row_seq, const int* pages, int count,
-                                  void* out, long long out_stride, float* part_o, float* part_l, int splits, int T, int nh, int nkv, int hd,
-                                  int block_size, float scale, hipStream_t s) {
-  if (T == 0) return 0;
-  Args a{};
-  a.q = (const uint16_t*)q;
-  a.q_stride = q_stride;
-  a.k = (const uint16_t*)k;
-  a.v = (const uint16_t*)v;
-  a.tables = tables;
-  a.table_stride = table_stride;
-  a.table_cols = table_cols;
-  a.n_seqs = n_seqs;
-  a.num_blocks = num_blocks;
-  a.rows = T;
-  a.ctx = ctx;
-  a.out = (uint16_t*)out;
-  a.out_stride = out_stride;
-  a.part_o = part_o;
-  a.part_l = part_l;
-  a.splits = splits;
-  a.nh = nh;
-  a.nkv = nkv;
-  while ((1 << a.bs_log2) < block_size) ++a.bs_log2;
-  a.scale_log2 = scale * 1.4426950408889634f;
-  a.pages = pages;
-  a.row_seq = row_seq;
-  a.count = count;
-  return launch_dims<1, 4, false>(a, T, hd, s);
-}
-
-extern "C" int dgi_paged_tree(const void* q, long long q_stride, const void* k, const void* v, const int* tables, int table_stride,
+extern "C" int dgi_tree_rows(const void* q, long long q_stride, const void* k, const void* v, const int* tables, int table_stride,
                               int table_cols, int n_seqs, int num_blocks, int rows, const int* cu, const int* ctx, const void* mask,
                               int mask_stride, int max_nodes, void* out, long long out_stride, float* part_o, float* part_l, int splits,
                               int min_part, int nh, int nkv, int hd, int block_size, float scale, hipStream_t s) {
@@ -469,6 +364,6 @@ extern "C" int dgi_paged_tree(const void* q, long long q_stride, const void* k, 
   a.max_nodes = max_nodes;
   a.min_part = min_part;
   const int cols = dgi_tree_columns(max_nodes, nh / nkv), items = n_seqs * ((max_nodes * (nh / nkv) + cols - 1) / cols);
-  if (cols == 16) return launch_dims<1, 4, true>(a, items, hd, s);
-  return launch_dims<2, 4, true>(a, items, hd, s);
+  if (cols == 16) return launch_dims<1, 4>(a, items, hd, s);
+  return launch_dims<2, 4>(a, items, hd, s);
 }
