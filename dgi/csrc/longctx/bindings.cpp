@@ -21,8 +21,8 @@ int dgi_select_pages(const void* q, long long q_stride, const void* bounds, cons
                      int recent, void* keys, int key_stride, int* out, hipStream_t s);
 int dgi_paged_selected(const void* q, long long q_stride, const void* k, const void* v, const int* tables, int table_stride, int table_cols,
                        int n_seqs, int num_blocks, const int* ctx, const int* row_seq, const int* pages, int count, void* out,
-                       long long out_stride, float* part_o, float* part_l, int splits, int T, int nh, int nkv, int hd, int block_size,
-                       float scale, hipStream_t s);
+                       long long out_stride, float* part_o, float* part_l, int splits, void* plan, int* plan_total, int* plan_rows, int T, int nh,
+                       int nkv, int hd, int block_size, float scale, hipStream_t s);
 int dgi_tree_columns(int max_nodes, int G);
 int dgi_tree_rows(const void* q, long long q_stride, const void* k, const void* v, const int* tables, int table_stride, int table_cols,
                    int n_seqs, int num_blocks, int rows, const int* cu, const int* ctx, const void* mask, int mask_stride, int max_nodes,
@@ -214,7 +214,7 @@ void paged_selected(at::Tensor out, const at::Tensor& q, const at::Tensor& k, co
                     ": pages must be [rows, kv heads, count]");
   const int* rows = rows_of(row_seq, tables, T, at_.dev, op);
   const int64_t count = pages.size(2);
-  TORCH_CHECK_VALUE(T <= kInt / nkv, op, ": too many rows");
+  TORCH_CHECK_VALUE(T <= kInt / nkv - 16, op, ": too many rows");
   const c10::DeviceGuard guard(at_.dev);
   // runs of 256 keys at the least, as many as give the card two workgroups a compute unit
   const int64_t least = std::max<int64_t>(1, 256 / at_.page);
@@ -224,11 +224,19 @@ void paged_selected(at::Tensor out, const at::Tensor& q, const at::Tensor& k, co
     part_o = at::empty({T * nh * splits * at_.hd}, q.options().dtype(at::kFloat));
     part_l = at::empty({T * nh * splits}, q.options().dtype(at::kFloat));
   }
+  // more rows than sequences: neighbours that may read their pages together
+  at::Tensor plan, plan_n;
+  const bool together = rows && T > tables.size(0) && nh / nkv <= 8;
+  if (together) {
+    plan = at::empty({T * nkv * count * 2}, q.options().dtype(at::kLong));
+    plan_n = at::empty({T * (nkv + 1)}, q.options().dtype(at::kInt));
+  }
   check_rc(dgi_paged_selected(q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(), tables.data_ptr<int>(), (int)tables.stride(0),
                               (int)tables.size(1), (int)tables.size(0), (int)k.size(0), ctx.data_ptr<int>(), rows, pages.data_ptr<int>(),
                               (int)count, out.data_ptr(), out.stride(0), splits > 1 ? part_o.data_ptr<float>() : nullptr,
-                              splits > 1 ? part_l.data_ptr<float>() : nullptr, (int)splits, (int)T, (int)nh, (int)nkv, (int)at_.hd,
-                              (int)at_.page, (float)scale, cur_stream()), op);
+                              splits > 1 ? part_l.data_ptr<float>() : nullptr, (int)splits, together ? plan.data_ptr() : nullptr,
+                              together ? plan_n.data_ptr<int>() : nullptr, together ? plan_n.data_ptr<int>() + T * nkv : nullptr, (int)T, (int)nh,
+                              (int)nkv, (int)at_.hd, (int)at_.page, (float)scale, cur_stream()), op);
 }
 
 void paged_tree(at::Tensor out, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& tables,

@@ -5,14 +5,19 @@
 //
 // A workgroup owns the G heads of a kv head for one row or, where rows of one sequence follow each other, for as many of them as
 // make 16 query columns: neighbours of a prompt mostly select the same pages, which are then read once, and the columns of the matrix
-// instruction are used.  It reads the union of their lists (a bit per page and row in LDS), each column masked to its own row's.  Its waves
-// take tiles of 32 keys in turn and are merged through LDS; lists are cut between workgroups where rows are few, and added up
-// by a second launch.
+// instruction are used.  It reads the union of their lists (made by a launch of its own, a bit per page and row in LDS), each column
+// masked to its own row's.  Its waves take tiles of 32 keys in turn and are merged through LDS; lists are cut between workgroups where
+// rows are few, and added up by a second launch.
 //
 // Scores are formed transposed, S^T = K Q^T, so that a lane owns a query column and the weights stay in the registers that the product
-// O^T += V^T P^T takes them from; V is transposed on its way out of LDS.  Weights are rounded to bf16 for that product (as the cached
-// values are; their sum is taken before), everything else is fp32.  Decode rows are bound by the bytes of their pages, rows of prompts by
-// what a compute unit's L1 passes on: a tile's keys and values are asked for while the one before is multiplied.
+// O^T += V^T P^T takes them from.  Weights are rounded to bf16 for that product (as the cached values are; their sum is taken before),
+// everything else is fp32.  A tile's keys and values are asked for while the one before is multiplied, whole rows a load, and go
+// through LDS: operands of the key product loaded as they are needed touch every line twice, 64 bytes at a time.
+//
+// Decode rows are bound by the bytes of their pages: 64 rows of 64 heads on 8, 128 pages of 16 keys each, 97 us, 5.5 TB/s.  Rows of
+// prompts by the path from the L2 to a compute unit's registers: 2 x 509 rows of 28 heads on 4, 64 pages each, 100 us, 1.5 GB of keys
+// and values where row by row it is 2.1 GB (205 us; together with key operands straight from memory 133; without the loads 70).
+// Three workgroups a compute unit spill registers (104).
 #include "../common.h"
 
 #include <type_traits>
@@ -42,14 +47,18 @@ struct Args {
   float* part_l;
   int splits, nh, nkv, bs_log2;
   float scale_log2;
+  int4* plan;         // [rows][kv head][count] what the rows that begin with a row read: page, place, rows that selected it
+  int* plan_total;    // [rows][kv head] how many entries
+  int* plan_rows;     // [rows] how many rows go together, 0: the row goes with one before it
 };
 
+// Where 16-byte chunk ch of a row lies in LDS: keys are read 16 rows at one chunk (16 banks' worth apart), values transposed.
 template <int HD>
-__device__ __forceinline__ int v_lds_off(int row, int col) {
-  constexpr int NCH = HD / 8;
-  const int ch = (col >> 3) ^ (((row & 7) << 1) & (NCH - 1));
-  return row * HD + (ch << 3) + (col & 7);
-}
+__device__ __forceinline__ int k_lds_off(int row, int ch) { return row * HD + ((ch ^ (HD == 64 ? row >> 1 & 7 : row & 15)) << 3); }
+template <int HD>
+__device__ __forceinline__ int v_lds_chunk(int row, int ch) { return row * HD + ((ch ^ (((row & 7) << 1) & (HD / 8 - 1))) << 3); }
+template <int HD>
+__device__ __forceinline__ int v_lds_off(int row, int col) { return v_lds_chunk<HD>(row, col >> 3) + (col & 7); }
 
 template <int HD>
 constexpr int wave_lds() { return 64 * HD; }      // a tile of values (32 x HD bf16), then 16 rows of sums (fp32)
@@ -67,28 +76,115 @@ __device__ __forceinline__ int rows_from(const Args& a, int t, int most, int lan
   return __ffs(begins >> (at + 1));
 }
 
-template <int HD, bool WIDE>
+// What the workgroups of rows that go together read: the union of their lists, ascending, or, where a row names a page twice (it counts
+// twice) or the bits do not fit, one list after another.  A workgroup per (first row, kv head).
+__global__ __launch_bounds__(NT) void selected_plan_kernel(Args a) {
+  __shared__ unsigned bits[kBits];        // [rows][words] the pages that a row selected
+  __shared__ int before[kBits / 2];       // [words] pages of any row in the words before
+  __shared__ int s_n[NW];
+  const int G = a.nh / a.nkv, side = 16 / G, groups = (a.rows + side - 1) / side;
+  // the first rows of all groups, the second ones, ..: most of the others have nothing to do, and would leave every other XCD without work
+  const int unit = blockIdx.x / a.nkv, h = blockIdx.x - unit * a.nkv, place = unit / groups, t0 = (unit - place * groups) * side + place;
+  const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
+  if (t0 >= a.rows) return;
+  const int m = rows_from(a, t0, side, lane);
+  if (h == 0 && tid == 0) a.plan_rows[t0] = m;
+  if (m == 0) return;
+  const int seq = a.row_seq[t0];
+  const bool known = seq >= 0 && seq < a.n_seqs;
+  const int* table = a.tables + (size_t)(known ? seq : 0) * a.table_stride;
+  int most = known && lane < m ? a.ctx[t0 + lane] : 0;
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o, 64));
+  most = __shfl(most, 0, 64);
+  int4* list = a.plan + (size_t)t0 * a.nkv * a.count + (size_t)h * m * a.count;
+  auto entry = [&](int i) {      // entry e of row r; i = r count + e
+    const int r = i / a.count;
+    return a.pages[((size_t)(t0 + r) * a.nkv + h) * a.count + (i - r * a.count)];
+  };
+  auto fits = [&](int p) { return p >= 0 && p < a.table_cols && ((long long)p << a.bs_log2) < most; };
+  const int words = min((int)(((long long)most + (32ll << a.bs_log2) - 1) >> (a.bs_log2 + 5)), (a.table_cols + 31) >> 5), all = m * a.count;
+  bool together = m > 1 && m * words <= kBits;
+  if (together) {
+    for (int i = tid; i < m * words; i += NT) bits[i] = 0;
+    __syncthreads();
+    bool twice = false;
+    for (int i = tid; i < all; i += NT) {
+      const int p = entry(i);
+      if (fits(p)) twice = twice || (atomicOr(&bits[i / a.count * words + (p >> 5)], 1u << (p & 31)) >> (p & 31) & 1);
+    }
+    together = !__syncthreads_or(twice);
+  }
+  if (!together) {
+    for (int i = tid; i < all; i += NT) {
+      const int p = entry(i), id = fits(p) ? table[p] : -1;
+      const bool there = id >= 0 && id < a.num_blocks;
+      list[i] = int4{there ? id : 0, there ? p << a.bs_log2 : 0, there ? 1 << (i / a.count) : 0, 0};
+    }
+    if (tid == 0) a.plan_total[t0 * a.nkv + h] = all;
+    return;
+  }
+  const int per = (words + NT - 1) / NT, first = min(tid * per, words), last = min(first + per, words);
+  int n = 0;
+  for (int i = first; i < last; ++i) {
+    unsigned u = 0;
+    for (int r = 0; r < m; ++r) u |= bits[r * words + i];
+    before[i] = n;
+    n += __popc(u);
+  }
+  int sum = n;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int x = __shfl_up(sum, o, 64);
+    if (lane >= o) sum += x;
+  }
+  if (lane == 63) s_n[w] = sum;
+  __syncthreads();
+  int from = sum - n;
+  for (int v = 0; v < w; ++v) from += s_n[v];
+  if (tid == NT - 1) a.plan_total[t0 * a.nkv + h] = from + n;
+  for (int i = first; i < last; ++i) before[i] += from;
+  __syncthreads();
+  for (int i = tid; i < all; i += NT) {      // the first row that has a page writes it
+    const int p = entry(i), r = i / a.count, word = p >> 5;
+    if (!fits(p)) continue;
+    unsigned who = 0, u = 0;
+    for (int s = 0; s < m; ++s) {
+      const unsigned x = bits[s * words + word];
+      who |= (x >> (p & 31) & 1) << s;
+      u |= x;
+    }
+    if (who & ((1u << r) - 1)) continue;
+    const int id = table[p];
+    const bool there = id >= 0 && id < a.num_blocks;
+    list[before[word] + __popc(u & ((1u << (p & 31)) - 1))] = int4{there ? id : 0, there ? p << a.bs_log2 : 0, there ? (int)who : 0, 0};
+  }
+}
+
+// PLAN: rows that go together and their list come from the launch before; otherwise each row is by itself.
+template <int HD, bool WIDE, bool PLAN>
 __global__ __launch_bounds__(NT, HD == 256 ? 1 : 2) void selected_kernel(Args a) {
   constexpr int KS = HD / 32, NC = HD / 16, VCH = HD / 8;
   __shared__ __attribute__((aligned(16))) char smem[NW * wave_lds<HD>()];
-  __shared__ int2 list[kList];            // page, its first key's place in the sequence
-  __shared__ unsigned seen[kList];        // rows that selected it
-  __shared__ unsigned bits[kBits];        // [rows][words] the pages that a row selected; then [words] of any row, [words] how many before
+  __shared__ int4 list[kList];            // page, its first key's place in the sequence, rows that selected it
   __shared__ float ml[NW][2][16];
-  __shared__ int s_n[NW + 1];
+  __shared__ int s_n[NW];
 
-  const int G = a.nh / a.nkv, bs = 1 << a.bs_log2, side = 16 / G, groups = (a.rows + side - 1) / side;
-  // the first rows of all groups, the second ones, ..: most of the others have nothing to do, and would leave every other XCD without work
-  const int unit = blockIdx.x / a.nkv, h = blockIdx.x - unit * a.nkv, place = unit / groups, t0 = (unit - place * groups) * side + place;
+  const int G = a.nh / a.nkv, bs = 1 << a.bs_log2;
+  const int unit = blockIdx.x / a.nkv, h = blockIdx.x - unit * a.nkv;
+  int t0 = unit, m = 1;
+  if constexpr (PLAN) {      // in the plan's order of rows
+    const int side = 16 / G, groups = (a.rows + side - 1) / side, place = unit / groups;
+    t0 = (unit - place * groups) * side + place;
+    if (t0 >= a.rows) return;
+    m = a.plan_rows[t0];
+    if (m == 0) return;
+  }
   const int split = blockIdx.y, tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, qi = lane & 15, g = lane >> 4;
-  if (t0 >= a.rows) return;
-  const int m = __builtin_amdgcn_readfirstlane(rows_from(a, t0, side, lane));
-  if (m == 0) return;
   uint16_t* vt = reinterpret_cast<uint16_t*>(smem + w * wave_lds<HD>());
 
-  int seq = a.row_seq ? a.row_seq[t0] : t0;
+  const int seq = a.row_seq ? a.row_seq[t0] : t0;
   const bool known = seq >= 0 && seq < a.n_seqs;
-  const int* table = a.tables + (size_t)(known ? seq : 0) * a.table_stride;
   // column qi: head qi % G of row qi / G
   const int rr = qi / G, head = h * G + qi - rr * G;
   const bool live = rr < m;
@@ -98,127 +194,69 @@ __global__ __launch_bounds__(NT, HD == 256 ? 1 : 2) void selected_kernel(Args a)
 #pragma unroll
   for (int s = 0; s < KS; ++s) qf[s] = live ? *reinterpret_cast<const u32x4*>(qp + 32 * s) : u32x4{0, 0, 0, 0};
   int most = ctx, least = live ? ctx : 0x7fffffff;      // the longest and the shortest context of the rows
+  if constexpr (PLAN) {
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) {
-    most = max(most, __shfl_xor(most, o, 64));
-    least = min(least, __shfl_xor(least, o, 64));
+    for (int o = 8; o > 0; o >>= 1) {
+      most = max(most, __shfl_xor(most, o, 64));
+      least = min(least, __shfl_xor(least, o, 64));
+    }
+    least = __builtin_amdgcn_readfirstlane(least);
   }
-  most = __builtin_amdgcn_readfirstlane(most);
-  least = __builtin_amdgcn_readfirstlane(least);
-
-  // ---- the lists: entry e of row r; i = r count + e
-  auto entry = [&](int i) {
-    const int r = i / a.count;
-    return a.pages[((size_t)(t0 + r) * a.nkv + h) * a.count + (i - r * a.count)];
-  };
-  // a page that the rows may read: in the table and begun by the longest context
-  auto fits = [&](int p) { return p >= 0 && p < a.table_cols && ((long long)p << a.bs_log2) < most; };
-  const int words = min((int)(((long long)most + (32ll << a.bs_log2) - 1) >> (a.bs_log2 + 5)), (a.table_cols + 31) >> 5);
-  int total = m * a.count;
-  const int mine = m > 1 && tid < total ? entry(tid) : -1;      // the thread's first entry, and its page
-  const int mine_id = fits(mine) ? table[mine] : -1;
-  bool together = m > 1 && m * words <= kBits;
-  if (together) {
-    for (int i = tid; i < m * words; i += NT) bits[i] = 0;
-    __syncthreads();
-    bool twice = false;
-    for (int i = tid; i < total; i += NT) {
-      const int r = i / a.count, p = i == tid ? mine : entry(i);
-      if (fits(p)) twice = twice || (atomicOr(&bits[r * words + (p >> 5)], 1u << (p & 31)) >> (p & 31) & 1);
-    }
-    together = !__syncthreads_or(twice);      // a page named twice counts twice: then list by list
-  }
-  if (together) {
-    const int per = (words + NT - 1) / NT, first = min(tid * per, words), last = min(first + per, words);
-    int n = 0;
-    for (int i = first; i < last; ++i) {
-      unsigned u = 0;
-      for (int r = 0; r < m; ++r) u |= bits[r * words + i];
-      bits[i] = u;
-      n += __popc(u);
-    }
-    int sum = n;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int x = __shfl_up(sum, o, 64);
-      if (lane >= o) sum += x;
-    }
-    if (lane == 63) s_n[w] = sum;
-    __syncthreads();
-    int before = sum - n;
-    total = 0;
-    for (int v = 0; v < NW; ++v) {
-      if (v < w) before += s_n[v];
-      total += s_n[v];
-    }
-    for (int i = first; i < last; ++i) {
-      bits[words + i] = before;
-      before += __popc(bits[i]);
-    }
-  }
+  most = __builtin_amdgcn_readfirstlane(most);      // lane 0's column is live
+  if constexpr (!PLAN) least = most;
+  const int total = PLAN ? a.plan_total[t0 * a.nkv + h] : a.count;
   const int part = (total + a.splits - 1) / a.splits, lo = split * part, hi = most > 0 ? min(lo + part, total) : lo;
+  const int4* planned = PLAN ? a.plan + (size_t)t0 * a.nkv * a.count + (size_t)h * m * a.count : nullptr;
 
-  // what a wave works with
+  // where the lane's chunk of row i 64 / VCH + lane / VCH goes in LDS: the same for every P-th i, but for whole rows
+  constexpr int P = VCH / 4;      // 16 rows
+  int k_at[P], v_at[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    k_at[i] = k_lds_off<HD>(i * (64 / VCH) + lane / VCH, lane % VCH);
+    v_at[i] = v_lds_chunk<HD>(i * (64 / VCH) + lane / VCH, lane % VCH);
+  }
+  const int ctx_g = ctx - 4 * g;      // the lane's keys begin at 4 g
+
   float m_run, l_run;
   f32x4 o[NC];
-  int entries = 0;
-  auto fill = [&](int at) {      // the list of entries at .. of the union, or of one row's list after another's
-    __syncthreads();
-    if (together) {
-      entries = min(kList, hi - at);
-      for (int e = tid; e < entries; e += NT) seen[e] = 0;
-      __syncthreads();
-      for (int i = tid; i < m * a.count; i += NT) {
-        const int p = i == tid ? mine : entry(i);
-        if (!fits(p)) continue;
-        const int rank = bits[words + (p >> 5)] + __popc(bits[p >> 5] & ((1u << (p & 31)) - 1)) - at;
-        if (rank < 0 || rank >= entries) continue;
-        const int id = i == tid ? mine_id : table[p];
-        const bool there = id >= 0 && id < a.num_blocks;
-        list[rank] = int2{there ? id : 0, p << a.bs_log2};      // every row that has it writes the same
-        if (there) atomicOr(&seen[rank], 1u << (i / a.count));
-      }
-    } else {
-      const int e = at + tid;
-      int id = -1, p = -1;
-      if (tid < kList && e < hi) {
-        p = entry(e);
-        if (fits(p)) id = table[p];
-      }
-      const bool there = id >= 0 && id < a.num_blocks;
-      const unsigned long long b = __ballot(there);
-      if (lane == 0) s_n[w] = __popcll(b);
-      __syncthreads();
-      int from = 0;
-      entries = 0;
-      for (int v = 0; v < NW; ++v) {
-        if (v < w) from += s_n[v];
-        entries += s_n[v];
-      }
-      if (there) {
-        from += __popcll(b & ((1ull << lane) - 1));
-        list[from] = int2{id, p << a.bs_log2};
-        seen[from] = 1u << (e / a.count);
-      }
-    }
-    __syncthreads();
-  };
-
   // A pass over the keys for all rows.  Values that are infinite or no numbers reach the rows that see them alone, but zero times such a
   // value is no number: where rows go together and a result is not finite, each is done again by itself, the values that it does not
   // see as zeros.
   for (int turn = -1, turns = 0; turn < turns; ++turn) {
-    const bool alone = turn >= 0;
+    const bool alone = PLAN && turn >= 0;
     const unsigned who = alone ? 1u << turn : (1u << m) - 1;
+    const int limit = alone ? a.ctx[t0 + turn] : most;
     m_run = -__builtin_inff();
     l_run = 0.f;
 #pragma unroll
     for (int c = 0; c < NC; ++c) o[c] = f32x4{0, 0, 0, 0};
-    const int limit = alone ? a.ctx[t0 + turn] : most;
     for (int at = lo; at < hi; at += kList) {
-      fill(at);
+      int entries = min(kList, hi - at);
+      __syncthreads();
+      if constexpr (PLAN) {
+        if (tid < entries) list[tid] = planned[at + tid];
+      } else {      // entries without a page are left out
+        int id = -1, p = -1;
+        if (tid < entries) {
+          p = a.pages[((size_t)t0 * a.nkv + h) * a.count + at + tid];
+          if (p >= 0 && p < a.table_cols && ((long long)p << a.bs_log2) < most) id = a.tables[(size_t)seq * a.table_stride + p];
+        }
+        const bool there = id >= 0 && id < a.num_blocks;
+        const unsigned long long b = __ballot(there);
+        if (lane == 0) s_n[w] = __popcll(b);
+        __syncthreads();
+        int from = 0;
+        entries = 0;
+        for (int v = 0; v < NW; ++v) {
+          if (v < w) from += s_n[v];
+          entries += s_n[v];
+        }
+        if (there) list[from + __popcll(b & ((1ull << lane) - 1))] = int4{id, p << a.bs_log2, 1, 0};
+      }
+      __syncthreads();
       const int keys = entries << a.bs_log2, ntiles = (keys + 31) >> 5;
-      u32x4 kf[2][KS], vr[VCH / 2];
+      u32x4 kr[VCH / 2], vr[VCH / 2];
       // Sixteen keys of a tile lie side by side in one page (WIDE), or each lane finds its own: where they lie in the cache, in the
       // sequence, and who selected them.  Past the list: its last page, selected by nobody.
       struct Keys {
@@ -228,43 +266,47 @@ __global__ __launch_bounds__(NT, HD == 256 ? 1 : 2) void selected_kernel(Args a)
       };
       auto keys_at = [&](int tok) {
         const int e = min(tok >> a.bs_log2, entries - 1), off = tok & (bs - 1);
-        const int2 page = list[e];
-        return Keys{(((size_t)page.x * a.nkv + h) << a.bs_log2) + off, page.y + off, tok < keys ? (unsigned)seen[e] : 0u};
+        const int4 page = list[e];
+        return Keys{(((size_t)page.x * a.nkv + h) << a.bs_log2) + off, page.y + off, tok < keys ? (unsigned)page.z : 0u};
       };
       auto half = [&](int t, int u) {      // WIDE: in scalar registers
         const Keys x = keys_at(32 * t + 16 * u);
         return Keys{((size_t)__builtin_amdgcn_readfirstlane((int)(x.row >> 32)) << 32) | (unsigned)__builtin_amdgcn_readfirstlane((int)x.row),
                     __builtin_amdgcn_readfirstlane(x.base), (unsigned)__builtin_amdgcn_readfirstlane(x.who)};
       };
-      auto load_k = [&](int t, const Keys* x) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const uint16_t* p = WIDE ? a.k + x[u].row * HD + (qi * HD + 8 * g) : a.k + keys_at(32 * t + 16 * u + qi).row * HD + 8 * g;
-#pragma unroll
-          for (int s = 0; s < KS; ++s) kf[u][s] = *reinterpret_cast<const u32x4*>(p + 32 * s);
-        }
-      };
-      auto load_v = [&](int t, const Keys* x) {
+      // a tile's rows, whole lines a load
+      auto load = [&](int t, const Keys* x, const uint16_t* cache, u32x4* to) {
 #pragma unroll
         for (int i = 0; i < VCH / 2; ++i) {
           constexpr int R = 64 / VCH;      // rows a load
           const int u = i * R / 16;
-          const uint16_t* p = WIDE ? a.v + x[u].row * HD + ((i * R - 16 * u) * HD + lane * 8) : a.v + keys_at(32 * t + i * R + lane / VCH).row * HD + lane % VCH * 8;
-          vr[i] = *reinterpret_cast<const u32x4*>(p);
+          to[i] = *reinterpret_cast<const u32x4*>(WIDE ? cache + x[u].row * HD + ((i * R - 16 * u) * HD + lane * 8)
+                                                       : cache + keys_at(32 * t + i * R + lane / VCH).row * HD + lane % VCH * 8);
         }
       };
+      // and into LDS, behind the reads of what was there
+      auto stage = [&](const u32x4* from, const int* at) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < VCH / 2; ++i) *reinterpret_cast<u32x4*>(vt + at[i % P] + i / P * (64 / VCH * P * HD)) = from[i];
+      };
       auto tile = [&](int t, Keys* now, Keys* next, auto LAST) {
+        stage(kr, k_at);
+        if constexpr (!LAST.value) {
+          __builtin_amdgcn_sched_barrier(0);
+          load(t + NW, next, a.k, kr);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
         f32x4 sc[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           sc[u] = f32x4{0, 0, 0, 0};
 #pragma unroll
-          for (int s = 0; s < KS; ++s) sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(kf[u][s]), as_bf16x8(qf[s]), sc[u], 0, 0, 0);
-        }
-        if constexpr (!LAST.value) {
-          __builtin_amdgcn_sched_barrier(0);
-          load_k(t + NW, next);        // into the registers that the products have read
-          __builtin_amdgcn_sched_barrier(0);
+          for (int s = 0; s < KS; ++s)
+            sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(*reinterpret_cast<const u32x4*>(vt + k_lds_off<HD>(16 * u + qi, 4 * s + g))),
+                                                            as_bf16x8(qf[s]), sc[u], 0, 0, 0);
         }
         const int end = max(now[0].base, now[1].base) + 16;
         // values that no row (alone: not this one) sees are zeros: their weight is zero, but what lies there may be no number
@@ -272,17 +314,15 @@ __global__ __launch_bounds__(NT, HD == 256 ? 1 : 2) void selected_kernel(Args a)
 #pragma unroll
           for (int i = 0; i < VCH / 2; ++i) {
             constexpr int R = 64 / VCH;
-            const int row = i * R + lane / VCH, u = i * R / 16;
-            const Keys x = WIDE ? Keys{0, now[u].base + row - 16 * u, now[u].who} : keys_at(32 * t + row);
-            if (x.base >= limit || !(x.who & who)) vr[i] = u32x4{0, 0, 0, 0};
+            const int u = i * R / 16;
+            const Keys x = WIDE ? Keys{0, now[u].base + i * R - 16 * u, now[u].who} : keys_at(32 * t + i * R + lane / VCH);
+            if (x.base >= limit - (WIDE ? lane / VCH : 0) || !(x.who & who)) vr[i] = u32x4{0, 0, 0, 0};
           }
         }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // the previous tile's transposed reads
-#pragma unroll
-        for (int i = 0; i < VCH / 2; ++i) *reinterpret_cast<u32x4*>(vt + v_lds_off<HD>(i * (64 / VCH) + lane / VCH, lane % VCH * 8)) = vr[i];
+        stage(vr, v_at);
         if constexpr (!LAST.value) {
           __builtin_amdgcn_sched_barrier(0);
-          load_v(t + NW, next);
+          load(t + NW, next, a.v, vr);
           __builtin_amdgcn_sched_barrier(0);
         }
         // ---- online softmax; the lane's keys are 16 u + 4 g + i
@@ -296,8 +336,8 @@ __global__ __launch_bounds__(NT, HD == 256 ? 1 : 2) void selected_kernel(Args a)
           for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const Keys k = WIDE ? Keys{0, now[u].base + 4 * g + i, now[u].who} : keys_at(32 * t + 16 * u + 4 * g + i);
-              if (!((k.who & who) >> rr & 1) || k.base >= ctx) x[u][i] = -__builtin_inff();
+              const Keys k = WIDE ? Keys{0, now[u].base + i, now[u].who} : keys_at(32 * t + 16 * u + 4 * g + i);
+              if (!((k.who & who) >> rr & 1) || k.base >= (WIDE ? ctx_g : ctx)) x[u][i] = -__builtin_inff();
             }
         }
 #pragma unroll
@@ -349,8 +389,8 @@ __global__ __launch_bounds__(NT, HD == 256 ? 1 : 2) void selected_kernel(Args a)
           }
         };
         find(now, w);
-        load_k(w, now);
-        load_v(w, now);
+        load(w, now, a.k, kr);
+        load(w, now, a.v, vr);
         int t = w;
         for (; t + NW < ntiles; t += NW) {
           find(next, t + NW);
@@ -405,7 +445,7 @@ __global__ __launch_bounds__(NT, HD == 256 ? 1 : 2) void selected_kernel(Args a)
         if (d == 0) a.part_l[slab] = L == 0.f ? -__builtin_inff() : M + __builtin_amdgcn_logf(L);
       }
     }
-    if (m > 1 && !alone && __syncthreads_or(odd)) turns = m;
+    if (PLAN && m > 1 && !alone && __syncthreads_or(odd)) turns = m;
   }
 }
 
@@ -454,10 +494,18 @@ __global__ __launch_bounds__(256) void selected_runs_kernel(Args a) {
 
 template <int HD>
 int launch(const Args& a, hipStream_t s) {
-  const int side = 16 / (a.nh / a.nkv);
-  const dim3 grid(a.nkv * ((a.rows + side - 1) / side * side), a.splits);
-  if (a.bs_log2 >= 4) selected_kernel<HD, true><<<grid, NT, 0, s>>>(a);
-  else selected_kernel<HD, false><<<grid, NT, 0, s>>>(a);
+  if (a.plan) {
+    const int side = 16 / (a.nh / a.nkv), rows = (a.rows + side - 1) / side * side;
+    selected_plan_kernel<<<a.nkv * rows, NT, 0, s>>>(a);
+    DGI_CHECK_LAUNCH();
+    const dim3 grid(a.nkv * rows, a.splits);
+    if (a.bs_log2 >= 4) selected_kernel<HD, true, true><<<grid, NT, 0, s>>>(a);
+    else selected_kernel<HD, false, true><<<grid, NT, 0, s>>>(a);
+  } else {
+    const dim3 grid(a.nkv * a.rows, a.splits);
+    if (a.bs_log2 >= 4) selected_kernel<HD, true, false><<<grid, NT, 0, s>>>(a);
+    else selected_kernel<HD, false, false><<<grid, NT, 0, s>>>(a);
+  }
   DGI_CHECK_LAUNCH();
   if (a.splits > 1) {
     selected_runs_kernel<HD><<<(unsigned)(((long long)a.rows * a.nh * (HD / 4) + 255) / 256), 256, 0, s>>>(a);
@@ -470,11 +518,12 @@ int launch(const Args& a, hipStream_t s) {
 
 extern "C" int dgi_paged_selected(const void* q, long long q_stride, const void* k, const void* v, const int* tables, int table_stride,
                                   int table_cols, int n_seqs, int num_blocks, const int* ctx, const int* row_seq, const int* pages, int count,
-                                  void* out, long long out_stride, float* part_o, float* part_l, int splits, int T, int nh, int nkv, int hd,
-                                  int block_size, float scale, hipStream_t s) {
+                                  void* out, long long out_stride, float* part_o, float* part_l, int splits, void* plan, int* plan_total,
+                                  int* plan_rows, int T, int nh, int nkv, int hd, int block_size, float scale, hipStream_t s) {
   if (T == 0) return 0;
   Args a{(const uint16_t*)q, q_stride, (const uint16_t*)k, (const uint16_t*)v, tables, table_stride, table_cols, n_seqs, num_blocks, T, ctx,
-         row_seq, pages, count, (uint16_t*)out, out_stride, part_o, part_l, splits, nh, nkv, 0, scale * 1.4426950408889634f};
+         row_seq, pages, count, (uint16_t*)out, out_stride, part_o, part_l, splits, nh, nkv, 0, scale * 1.4426950408889634f,
+         (int4*)plan, plan_total, plan_rows};
   while ((1 << a.bs_log2) < block_size) ++a.bs_log2;
   if (hd == 64) return launch<64>(a, s);
   if (hd == 128) return launch<128>(a, s);
