@@ -117,7 +117,7 @@ void rope_cache_bounds(at::Tensor q_out, const at::Tensor& qkv, const at::Tensor
   const int64_t T = qkv.size(0);
   check_int(positions, dev, at::kInt, op, "positions");
   check_int(slots, dev, at::kInt, op, "slot_mapping");
-  TORCH_CHECK_VALUE(positions.numel() == T && slots.numel() == T, op, ": positions and slot_mapping must have a number for each row");
+  TORCH_CHECK_VALUE(positions.numel() == T && slots.numel() == T && T <= (1 << 29), op, ": positions and slot_mapping must have a number for each row");
   TORCH_CHECK_VALUE(cos_sin.is_cuda() && cos_sin.device() == dev && cos_sin.scalar_type() == at::kFloat && cos_sin.is_contiguous() &&
                         cos_sin.dim() == 2 && cos_sin.size(0) > 0 && cos_sin.size(0) <= kInt && aligned(cos_sin),
                     op, ": cos_sin must be contiguous fp32 [positions, rotated dims]");

@@ -23,122 +23,160 @@ __device__ __forceinline__ void widen8(float* lo, float* hi, const float* x) {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 
-// Chunk c (8 dims) of a head at `hp`, rotated by the row's [cos | sin] at cs: the pairs of mode 0 are (i, i + rd / 2), of mode 1
-// (2 i, 2 i + 1); chunks beyond the rotated dims pass through.
-__device__ __forceinline__ void rotated_chunk(const uint16_t* __restrict__ hp, int c, const float* __restrict__ cs, int rd, int mode, float* o) {
-  float a[8];
-  unpack8(*reinterpret_cast<const u32x4*>(hp + c * 8), a);
-  if (c * 8 >= rd) {
+// A head's dims as tasks of one lane: a pair of 16-byte chunks that rotate with each other (mode 0: dims i and i + rd / 2), a chunk
+// that rotates in itself (mode 1: dims 2 i and 2 i + 1), or one behind the rotated dims that stays.
+struct Task {
+  int at, other;      // dims of the chunk and of the one that it rotates with (-1: none)
+  bool turns;
+  float c[8], s[8];   // cos and sin; mode 1: four of them
+};
+__device__ __forceinline__ int tasks_of(int hd, int rd, int mode) { return (mode == 0 ? rd >> 4 : rd >> 3) + ((hd - rd) >> 3); }
+__device__ __forceinline__ Task task_of(int i, int rd, int mode) {
+  const int turning = mode == 0 ? rd >> 4 : rd >> 3;
+  Task x;
+  x.turns = i < turning;
+  x.at = x.turns ? i * 8 : rd + (i - turning) * 8;
+  x.other = x.turns && mode == 0 ? x.at + (rd >> 1) : -1;
+  return x;
+}
+__device__ __forceinline__ void angles(Task& x, const float* __restrict__ cs, int rd, int mode) {
+  if (!x.turns) return;
+  const float *c = cs + (mode == 0 ? x.at : x.at >> 1), *s = c + (rd >> 1);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] = a[j];
-    return;
-  }
-  const int half = rd >> 1;
-  if (mode == 0) {
-    const bool second = c * 8 >= half;
-    const int p = second ? c * 8 - half : c * 8;
-    float b[8], cv[8], sv[8];
-    unpack8(*reinterpret_cast<const u32x4*>(hp + (second ? p : p + half)), b);
-    *reinterpret_cast<float4*>(cv) = *reinterpret_cast<const float4*>(cs + p);
-    *reinterpret_cast<float4*>(cv + 4) = *reinterpret_cast<const float4*>(cs + p + 4);
-    *reinterpret_cast<float4*>(sv) = *reinterpret_cast<const float4*>(cs + half + p);
-    *reinterpret_cast<float4*>(sv + 4) = *reinterpret_cast<const float4*>(cs + half + p + 4);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] = second ? a[j] * cv[j] + b[j] * sv[j] : a[j] * cv[j] - b[j] * sv[j];
-  } else {
-    const float4 cv = *reinterpret_cast<const float4*>(cs + c * 4);
-    const float4 sv = *reinterpret_cast<const float4*>(cs + half + c * 4);
-    const float cc[4] = {cv.x, cv.y, cv.z, cv.w}, ss[4] = {sv.x, sv.y, sv.z, sv.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      o[2 * j] = a[2 * j] * cc[j] - a[2 * j + 1] * ss[j];
-      o[2 * j + 1] = a[2 * j + 1] * cc[j] + a[2 * j] * ss[j];
-    }
+  for (int j = 0; j < 8; j += 4) {
+    if (mode == 1 && j) break;
+    *reinterpret_cast<float4*>(x.c + j) = *reinterpret_cast<const float4*>(c + j);
+    *reinterpret_cast<float4*>(x.s + j) = *reinterpret_cast<const float4*>(s + j);
   }
 }
+// a (and b, the chunk it rotates with) turned
+__device__ __forceinline__ void turn(const Task& x, u32x4& a, u32x4& b) {
+  if (!x.turns) return;
+  float p[8], q[8], u[8], v[8];
+  unpack8(a, p);
+  if (x.other >= 0) {
+    unpack8(b, q);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      u[j] = p[j] * x.c[j] - q[j] * x.s[j];
+      v[j] = q[j] * x.c[j] + p[j] * x.s[j];
+    }
+    b = pack8(v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      u[2 * j] = p[2 * j] * x.c[j] - p[2 * j + 1] * x.s[j];
+      u[2 * j + 1] = p[2 * j + 1] * x.c[j] + p[2 * j] * x.s[j];
+    }
+  }
+  a = pack8(u);
+}
 
-// A workgroup per row: its queries and values, and, where the row is the first of the step in its page, the keys and bounds of all
-// rows that follow it there (rows of rising slots, one page's side by side: at most a page of them).  So every page has one writer.
+// The first T workgroups are for the keys, the others for queries and values of a row.
+//
+// A row that is the first of the step in its page takes the keys of all rows that follow it there (rows of rising slots, side by
+// side: a page of them at most) and the page's bounds, so that every page has one writer; its waves take a row each in turn, the same task of a
+// row each lane, and are joined in LDS.  The workgroups of the rows behind it end at once.
+//
+// A lane has the same task of every head that it takes, and so one read of the angles.
 __global__ __launch_bounds__(kThreads) void rope_cache_bounds_kernel(
     const uint16_t* __restrict__ qkv, long long ld, int T, const int* __restrict__ positions, int max_pos,
     const float* __restrict__ cos_sin, int nh, int nkv, int hd, int rd, int mode, const int* __restrict__ slots, long long n_slots,
     uint16_t* __restrict__ q_out, uint16_t* __restrict__ k_cache, uint16_t* __restrict__ v_cache, uint16_t* __restrict__ bounds,
     int block_size) {
-  const int t = blockIdx.x, tid = threadIdx.x;
-  const int chunks = hd >> 3;
-  const uint16_t* row = qkv + t * ld;
-  const float* cs = cos_sin + (size_t)min(max(positions[t], 0), max_pos - 1) * rd;
-  const int slot = slots[t];
+  const bool keys = blockIdx.x < T;
+  const int t = keys ? blockIdx.x : blockIdx.x - T, tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
+  const int tasks = tasks_of(hd, rd, mode), slot = slots[t];
   const bool cached = slot >= 0 && slot < n_slots;
   const int blk = cached ? slot / block_size : 0, off = cached ? slot - blk * block_size : 0;
+  auto angles_at = [&](int row) { return cos_sin + (size_t)min(max(positions[row], 0), max_pos - 1) * rd; };
 
-  for (int it = tid; it < (nh + nkv) * chunks; it += kThreads) {
-    const int head = it / chunks, c = it - head * chunks;
-    if (head < nh) {
-      float o[8];
-      rotated_chunk(row + head * hd, c, cs, rd, mode, o);
-      *reinterpret_cast<u32x4*>(q_out + ((size_t)t * nh + head) * hd + c * 8) = pack8(o);
-    } else if (cached) {
-      const int h = head - nh;
-      *reinterpret_cast<u32x4*>(v_cache + (((size_t)blk * nkv + h) * block_size + off) * hd + c * 8) =
-          *reinterpret_cast<const u32x4*>(row + (size_t)(nh + nkv + h) * hd + c * 8);
+  if (!keys) {
+    const uint16_t* row = qkv + t * ld;
+    const int side = kThreads / tasks;      // heads at a time
+    Task x = task_of(tid % tasks, rd, mode);
+    if (tid < side * tasks) {
+      angles(x, angles_at(t), rd, mode);
+#pragma unroll 4
+      for (int head = tid / tasks; head < nh; head += side) {
+        const uint16_t* qp = row + head * hd;
+        uint16_t* op = q_out + ((size_t)t * nh + head) * hd;
+        u32x4 a = *reinterpret_cast<const u32x4*>(qp + x.at), b = *reinterpret_cast<const u32x4*>(qp + max(x.other, 0));
+        turn(x, a, b);
+        *reinterpret_cast<u32x4*>(op + x.at) = a;
+        if (x.other >= 0) *reinterpret_cast<u32x4*>(op + x.other) = b;
+      }
     }
+    if (cached)
+      for (int it = tid; it < nkv * (hd >> 3); it += kThreads) {
+        const int h = it / (hd >> 3), c = it - h * (hd >> 3);
+        *reinterpret_cast<u32x4*>(v_cache + (((size_t)blk * nkv + h) * block_size + off) * hd + c * 8) =
+            *reinterpret_cast<const u32x4*>(row + (size_t)(nh + nkv + h) * hd + c * 8);
+      }
+    return;
   }
 
-  if (!cached || (off > 0 && t > 0 && slots[t - 1] == slot - 1)) return;      // the whole workgroup: no keys of its own
-  int run = 1;
-  while (off + run < block_size && t + run < T && slots[t + run] == slot + run) ++run;
-
-  __shared__ __attribute__((aligned(16))) u32x4 part[2][kWaves][64];
-  const int w = tid >> 6, lane = tid & 63;
-  for (int base = 0; base < nkv * chunks; base += 64) {
+  if (!cached || (off > 0 && t > 0 && slots[t - 1] == slot - 1)) return;
+  int run = 0;      // rows of the page from here on
+  for (bool on = true; on; run += 64) {
+    const int r = run + lane;
+    const bool in = off + r < block_size && t + r < T && slots[min(t + r, T - 1)] == slot + r;
+    const unsigned long long out = ~__ballot(in);
+    if (out) {
+      run += __ffsll(out) - 1 - 64;
+      on = false;
+    }
+  }
+  __shared__ __attribute__((aligned(16))) u32x4 part[4][kWaves][64];
+  for (int base = 0; base < nkv * tasks; base += 64) {
     const int it = base + lane;
-    const bool live = it < nkv * chunks;
-    const int h = live ? it / chunks : 0, c = live ? it - h * chunks : 0;
-    float lo[8], hi[8];
+    const bool live = it < nkv * tasks;
+    const int h = live ? it / tasks : 0;
+    Task x = task_of(live ? it - h * tasks : 0, rd, mode);
+    float lo[2][8], hi[2][8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      lo[j] = __builtin_inff();
-      hi[j] = -__builtin_inff();
+      lo[0][j] = lo[1][j] = __builtin_inff();
+      hi[0][j] = hi[1][j] = -__builtin_inff();
     }
     if (live)
+#pragma unroll 2
       for (int r = w; r < run; r += kWaves) {
-        const float* csr = cos_sin + (size_t)min(max(positions[t + r], 0), max_pos - 1) * rd;
-        float o[8], x[8];
-        rotated_chunk(qkv + (t + r) * ld + (nh + h) * hd, c, csr, rd, mode, o);
-        const u32x4 k = pack8(o);
-        *reinterpret_cast<u32x4*>(k_cache + (((size_t)blk * nkv + h) * block_size + off + r) * hd + c * 8) = k;
-        unpack8(k, x);      // what attention will read
-        widen8(lo, hi, x);
+        const uint16_t* kp = qkv + (t + r) * ld + (nh + h) * hd;
+        uint16_t* op = k_cache + (((size_t)blk * nkv + h) * block_size + off + r) * hd;
+        u32x4 a = *reinterpret_cast<const u32x4*>(kp + x.at), b = *reinterpret_cast<const u32x4*>(kp + max(x.other, 0));
+        angles(x, angles_at(t + r), rd, mode);
+        turn(x, a, b);
+        float v[8];      // what attention will read
+        *reinterpret_cast<u32x4*>(op + x.at) = a;
+        unpack8(a, v);
+        widen8(lo[0], hi[0], v);
+        if (x.other >= 0) {
+          *reinterpret_cast<u32x4*>(op + x.other) = b;
+          unpack8(b, v);
+          widen8(lo[1], hi[1], v);
+        }
       }
-    part[0][w][lane] = pack8(lo);      // exact: the values are bf16
-    part[1][w][lane] = pack8(hi);
+    part[0][w][lane] = pack8(lo[0]);      // exact: the values are bf16
+    part[1][w][lane] = pack8(hi[0]);
+    part[2][w][lane] = pack8(lo[1]);
+    part[3][w][lane] = pack8(hi[1]);
     __syncthreads();
-    if (w == 0 && live) {
-      uint16_t* bp = bounds + ((size_t)blk * nkv + h) * 2 * hd + c * 8;
+    // wave w: the least (w even) or largest of the task's first or second chunk
+    const int at = w < 2 ? x.at : x.other;
+    if (live && at >= 0) {
+      uint16_t* bp = bounds + (((size_t)blk * nkv + h) * 2 + (w & 1)) * hd + at;
+      float m[8], v[8];
+      unpack8(part[w][0][lane], m);
+      auto join = [&](const u32x4& from) {
+        unpack8(from, v);
 #pragma unroll
-      for (int v = 1; v < kWaves; ++v) {
-        float x[8], y[8];
-        unpack8(part[0][v][lane], x);
-        unpack8(part[1][v][lane], y);
+        for (int j = 0; j < 8; ++j) m[j] = w & 1 ? __builtin_elementwise_maximum(m[j], v[j]) : __builtin_elementwise_minimum(m[j], v[j]);
+      };
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          lo[j] = __builtin_elementwise_minimum(lo[j], x[j]);
-          hi[j] = __builtin_elementwise_maximum(hi[j], y[j]);
-        }
-      }
-      if (off > 0) {
-        float x[8], y[8];
-        unpack8(*reinterpret_cast<const u32x4*>(bp), x);
-        unpack8(*reinterpret_cast<const u32x4*>(bp + hd), y);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          lo[j] = __builtin_elementwise_minimum(lo[j], x[j]);
-          hi[j] = __builtin_elementwise_maximum(hi[j], y[j]);
-        }
-      }
-      *reinterpret_cast<u32x4*>(bp) = pack8(lo);
-      *reinterpret_cast<u32x4*>(bp + hd) = pack8(hi);
+      for (int i = 1; i < kWaves; ++i) join(part[w][i][lane]);
+      if (off > 0) join(*reinterpret_cast<const u32x4*>(bp));
+      *reinterpret_cast<u32x4*>(bp) = pack8(m);
     }
     __syncthreads();
   }
@@ -187,7 +225,7 @@ extern "C" int dgi_rope_cache_bounds(const void* qkv, long long ld, int T, const
                                      int nkv, int hd, int rd, int mode, const int* slots, long long n_slots, void* q_out, void* k_cache,
                                      void* v_cache, void* bounds, int block_size, hipStream_t s) {
   if (T == 0) return 0;
-  rope_cache_bounds_kernel<<<T, kThreads, 0, s>>>((const uint16_t*)qkv, ld, T, positions, max_pos, cos_sin, nh, nkv, hd, rd, mode, slots,
+  rope_cache_bounds_kernel<<<2 * T, kThreads, 0, s>>>((const uint16_t*)qkv, ld, T, positions, max_pos, cos_sin, nh, nkv, hd, rd, mode, slots,
                                                   n_slots, (uint16_t*)q_out, (uint16_t*)k_cache, (uint16_t*)v_cache, (uint16_t*)bounds,
                                                   block_size);
   DGI_CHECK_LAUNCH();
