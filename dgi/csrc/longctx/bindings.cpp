@@ -23,7 +23,6 @@ int dgi_paged_selected(const void* q, long long q_stride, const void* k, const v
                        int n_seqs, int num_blocks, const int* ctx, const int* row_seq, const int* pages, int count, void* out,
                        long long out_stride, float* part_o, float* part_l, int splits, void* plan, int* plan_total, int* plan_rows, int T, int nh,
                        int nkv, int hd, int block_size, float scale, hipStream_t s);
-int dgi_tree_columns(int max_nodes, int G);
 int dgi_tree_rows(const void* q, long long q_stride, const void* k, const void* v, const int* tables, int table_stride, int table_cols,
                    int n_seqs, int num_blocks, int rows, const int* cu, const int* ctx, const void* mask, int mask_stride, int max_nodes,
                    void* out, long long out_stride, float* part_o, float* part_l, int splits, int min_part, int nh, int nkv, int hd,
@@ -253,9 +252,12 @@ void paged_tree(at::Tensor out, const at::Tensor& q, const at::Tensor& k, const 
   TORCH_CHECK_VALUE(mask.dim() == 2 && mask.size(0) >= S && mask.size(1) >= max_nodes && mask.size(1) <= kInt, op,
                     ": tree_mask must be [sequences, nodes]");
   const c10::DeviceGuard guard(at_.dev);
-  const int64_t G = nh / nkv, width = tables.size(1) * at_.page;
-  if (max_nodes * G > 32 && at_.hd <= 128) {
-    const int64_t tiles = (max_nodes * G + 127) / 128, least = 4;
+  // Columns of 16 pairs a workgroup (tree_rows) or row tiles of 128 (tree_tiles), us at 32 heads on 8: one sequence of 10 / 32 nodes, 600 keys 10, 16 /
+  // 12, 18; of 8000 keys 20, 25 / 25, 28; eight of 2000 keys, 10 / 16 / 24 nodes 25, 25 / 26, 27 / 33, 30; 32 of 4000, 8 / 10 / 16 100, - / 143, 116 /
+  // 148, 122; 64 heads, one of 32 / 64 nodes, 600 keys 12, 20 / 15, 22, but of 8000 38, 34 / 60, 41.
+  const int64_t G = nh / nkv, width = tables.size(1) * at_.page, pairs = max_nodes * G, few = S * nkv * ((pairs + 15) / 16);
+  if (pairs > 32 && at_.hd <= 128 && !(few <= 256 && (pairs <= 128 || width <= 1024))) {
+    const int64_t tiles = (pairs + 127) / 128, least = 4;
     const int64_t shares = std::max<int64_t>(1, std::min<int64_t>(512 / nkv, (S * tiles * ((width + 63) / 64) + least - 1) / least));
     TORCH_CHECK_VALUE(S * tiles * nkv <= kInt, op, ": too many sequences");
     at::Tensor part_o, part_l;
@@ -270,7 +272,7 @@ void paged_tree(at::Tensor out, const at::Tensor& q, const at::Tensor& k, const 
                             (int)least, (int)nh, (int)nkv, (int)at_.hd, (int)at_.page, (float)scale, cur_stream()), op);
     return;
   }
-  const int64_t cols = dgi_tree_columns((int)max_nodes, (int)G), tiles = (max_nodes * G + cols - 1) / cols;
+  const int64_t cols = 16, tiles = (pairs + cols - 1) / cols;
   TORCH_CHECK_VALUE(S <= kInt / (nkv * tiles), op, ": too many sequences");
   const int64_t items = S * tiles * nkv, min_part = 128;
   const int64_t splits = std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(1, items), (width + min_part - 1) / min_part, 64}));
