@@ -18,7 +18,7 @@ int dgi_page_bounds(const void* k_cache, void* bounds, const int* pages, const i
                     int block_size, hipStream_t s);
 int dgi_select_pages(const void* q, long long q_stride, const void* bounds, const int* tables, int table_stride, int table_cols, int n_seqs,
                      int num_blocks, const int* ctx, const int* row_seq, int T, int nh, int nkv, int hd, int page, int count, int first,
-                     int recent, void* keys, int key_stride, int* out, hipStream_t s);
+                     int recent, void* keys, int key_stride, int key_rows, int* out, hipStream_t s);
 int dgi_paged_selected(const void* q, long long q_stride, const void* k, const void* v, const int* tables, int table_stride, int table_cols,
                        int n_seqs, int num_blocks, const int* ctx, const int* row_seq, const int* pages, int count, void* out,
                        long long out_stride, float* part_o, float* part_l, int splits, void* plan, int* plan_total, int* plan_rows, int T, int nh,
@@ -170,11 +170,13 @@ void select_pages(at::Tensor out, const at::Tensor& q, const at::Tensor& bounds,
   const int* rows = rows_of(row_seq, tables, T, dev, op);
   TORCH_CHECK_VALUE(T <= kInt / nkv && tables.size(1) <= (1 << 24), op, ": too many rows or pages");
   const c10::DeviceGuard guard(dev);
-  const int64_t stride = tables.size(1);
-  const at::Tensor keys = at::empty({stride > count ? T * nkv * stride : 0}, q.options().dtype(at::kLong));
+  // scores of as many rows at a time (by 16) as 256 MB hold
+  const int64_t stride = tables.size(1), rows_16 = std::max<int64_t>((1 << 25) / (16 * nkv * std::max<int64_t>(stride, 1)), 1);
+  const int64_t at_once = stride > count ? std::min(T, 16 * rows_16) : T;
+  const at::Tensor keys = at::empty({stride > count ? at_once * nkv * stride : 0}, q.options().dtype(at::kLong));
   check_rc(dgi_select_pages(q.data_ptr(), q.stride(0), bounds.data_ptr(), tables.data_ptr<int>(), (int)tables.stride(0), (int)tables.size(1),
                             (int)tables.size(0), (int)bounds.size(0), ctx.data_ptr<int>(), rows, (int)T, (int)nh, (int)nkv, (int)hd,
-                            (int)page, (int)count, (int)first, (int)recent, keys.data_ptr(), (int)stride, out.data_ptr<int>(), cur_stream()), op);
+                            (int)page, (int)count, (int)first, (int)recent, keys.data_ptr(), (int)stride, (int)at_once, out.data_ptr<int>(), cur_stream()), op);
 }
 
 struct Attention {

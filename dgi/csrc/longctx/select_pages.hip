@@ -4,12 +4,17 @@
 // the largest q . k that a key within the page's bounds can have.  Kept are the first and last pages (as many as the caller says) and the
 // best of the others, ties to the lowest.
 //
-// Scores are summed in 64 bits: which page is kept is a whole number, and may not depend on the order in which a sum was taken.
-// They go as integers of the same order into a workspace [T, n_kv, pages]; a second launch chooses by digits of these integers
-// taken from the top.
+// Which page is kept is a whole number, and may not depend on the order in which a sum was taken: pages are compared by sums in 64 bits.
+// What they are compared by goes into a workspace [T, n_kv, pages], and another launch chooses.
 //
-// Decode rows each have bounds of their own, which is what bounds them (a lane multiplies what it loads).  Rows of a prompt share
-// their sequence's: 16 of them are the rows of matrix instructions in 64 bits, whose rate is the bound.
+// Decode rows each have bounds of their own: the scores in 64 bits as a lane multiplies what it loads, as integers of the same order, whose
+// digits from the top are counted until the threshold is found.  What bounds this is the bounds' bytes (64 rows over 4096 to 65536 keys,
+// 8 kv heads of 128, 303 MB: 72 us at 4.2 TB/s, and 7 us for the choice).
+//
+// Rows of a prompt share their sequence's bounds: 16 of them are the rows of bf16 matrix instructions, which give each score in 32 bits and
+// a bound for its error; pages that the error leaves open are scored in 64 bits (1018 rows of 28 heads over 730 to 1000 pages of 4 kv heads
+// of 128: 55 us, of which scores 31, those of rows that do not go together 4, the choice 21; with the products in 64 bits on the matrix
+// cores, whose rate alone is 24 us, 88 us).  What bounds this is latency: of the weights ahead of 4 steps of 64 pages, and of the choice.
 #include "../common.h"
 
 using namespace dgi;
@@ -34,11 +39,12 @@ struct Args {
   int table_stride, table_cols, n_seqs, num_blocks;
   const int* ctx;
   const int* row_seq;
-  int T, nh, nkv, page, count, first, recent;
+  int T, nh, nkv, hd, page, count, first, recent;
   u64* keys;
   int key_stride;
   int* out;
   int chunk;      // pages of a workgroup
+  int row_chunk;  // of one that scores a single row
 };
 
 __device__ __forceinline__ int pages_of(const Args& a, int t) {
@@ -47,41 +53,53 @@ __device__ __forceinline__ int pages_of(const Args& a, int t) {
 }
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr float kLeast = 0x1p-110f;      // the least error: products too small for 32 bits
 constexpr int kRows = 16, kRuns = 4;      // rows of an aligned group; it goes together if they are of so many sequences at most
 
 __device__ __forceinline__ bool together(unsigned begins) { return __popc(begins & ((1u << kRows) - 1)) <= kRuns; }
 
 // The aligned group of row t: bit i says that row i begins another sequence than the row before it (or is behind the last row).
-__device__ __forceinline__ unsigned begins_of(const Args& a, int t, int lane) {
+__device__ __forceinline__ unsigned begins_of(const Args& a, int t, int lane, int& seq) {
   const int row = t / kRows * kRows + lane;
-  const int seq = lane < kRows && row < a.T ? a.row_seq[row] : -1;
+  seq = lane < kRows && row < a.T ? a.row_seq[row] : -1;
   const int prev = __shfl_up(seq, 1, 64);
   return (unsigned)__ballot(lane < kRows && (lane == 0 || row == a.T || (row < a.T && seq != prev))) | 1u << kRows;
 }
 
-// up += max(q, 0), down += min(q, 0) of eight channels over a group's G heads, HD apart; four of them under way at a time.
-template <int HD>
-__device__ __forceinline__ void add_heads(double* up, double* down, const uint16_t* q, int G) {
-  for (int g0 = 0; g0 < G; g0 += 4) {
-    u32x4 v[4];
+// Eight channels of eight of a group's G heads, hd apart.
+__device__ __forceinline__ void load_heads(u32x4* v, const uint16_t* q, int hd, int g0, int G) {
 #pragma unroll
-    for (int g = 0; g < 4; ++g) v[g] = *reinterpret_cast<const u32x4*>(q + min(g0 + g, G - 1) * HD);
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
+  for (int g = 0; g < 8; ++g) v[g] = *reinterpret_cast<const u32x4*>(q + min(g0 + g, G - 1) * hd);
+}
+
+// P and N of a group in 64 bits by N threads, [N | P] into LDS.
+template <int N>
+__device__ __forceinline__ void weigh(double* wgt, const uint16_t* q, int hd, int G) {
+  for (int d = threadIdx.x % N; d < hd; d += N) {
+    double up = 0., down = 0.;
+    for (int g0 = 0; g0 < G; g0 += 8) {
       float x[8];
-      unpack8(v[g], x);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (g0 + g >= G) x[j] = 0.f;
-        up[j] += x[j] < 0.f ? 0.f : x[j];        // no number stays none
-        down[j] += x[j] > 0.f ? 0.f : x[j];
+      for (int g = 0; g < 8; ++g) x[g] = bf16_to_f32(q[min(g0 + g, G - 1) * hd + d]);
+#pragma unroll
+      for (int g = 0; g < 8; ++g) {
+        if (g0 + g >= G) x[g] = 0.f;
+        up += x[g] < 0.f ? 0.f : x[g];        // no number stays none
+        down += x[g] > 0.f ? 0.f : x[g];
       }
     }
+    wgt[d] = down;
+    wgt[hd + d] = up;
   }
 }
 
+__device__ __forceinline__ unsigned begins_of(const Args& a, int t, int lane) {
+  int seq;
+  return begins_of(a, t, lane, seq);
+}
+
 // Row by row.  Four 16-byte chunks of a page's [lo | hi] a lane, HD / 16 lanes a page; the next pages' bounds are under way
-// while these are multiplied.  GROUPS: not the rows that page_scores_tiles_kernel takes.
+// while these are multiplied.  GROUPS: not the rows that page_screen_kernel takes, and scores with a bound for the error as it has them.
 template <int HD, bool GROUPS>
 __global__ __launch_bounds__(kThreads) void page_scores_kernel(Args a) {
   constexpr int LP = HD / 16, PW = 64 / LP, STEP = kWaves * PW;      // lanes a page, pages a wave and a workgroup at a time
@@ -89,19 +107,10 @@ __global__ __launch_bounds__(kThreads) void page_scores_kernel(Args a) {
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, l = lane % LP, p0 = lane / LP;
   if (GROUPS && together(begins_of(a, t, lane))) return;
   const int n = pages_of(a, t);
-  const int begin = a.first + blockIdx.y * a.chunk, end = min(begin + a.chunk, n - a.recent);
+  const int begin = a.first + blockIdx.y * a.row_chunk, end = min(begin + a.row_chunk, n - a.recent);
   if (n <= a.count || begin >= end) return;
   const int G = a.nh / a.nkv;
   __shared__ double wgt_s[2 * HD];      // of lo, of hi
-  if (threadIdx.x < HD / 8) {
-    double up[8] = {}, down[8] = {};
-    add_heads<HD>(up, down, a.q + t * a.q_stride + h * G * HD + threadIdx.x * 8, G);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      wgt_s[threadIdx.x * 8 + j] = down[j];
-      wgt_s[HD + threadIdx.x * 8 + j] = up[j];
-    }
-  }
   const int seq = a.row_seq ? a.row_seq[t] : t;
   const bool known = seq >= 0 && seq < a.n_seqs;
   const int* table = a.tables + (size_t)(known ? seq : 0) * a.table_stride;
@@ -118,6 +127,7 @@ __global__ __launch_bounds__(kThreads) void page_scores_kernel(Args a) {
   };
   int base = begin + w * PW, id = id_of(base), id_next = id_of(base + STEP);
   load(v[0], id);
+  weigh<kThreads>(wgt_s, a.q + t * a.q_stride + h * G * HD, HD, G);
   __syncthreads();
   // chunk l + LP i: the lo half for i < 2, the hi half behind it
   double wgt[4][8];
@@ -125,6 +135,7 @@ __global__ __launch_bounds__(kThreads) void page_scores_kernel(Args a) {
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 8; ++j) wgt[i][j] = wgt_s[(l + LP * i) * 8 + j];
+  float largest = 0.f;
   auto score = [&](const u32x4* x4, int base, int id) {
     double sum[4] = {};
 #pragma unroll
@@ -137,8 +148,16 @@ __global__ __launch_bounds__(kThreads) void page_scores_kernel(Args a) {
     double s = (sum[0] + sum[1]) + (sum[2] + sum[3]);
 #pragma unroll
     for (int o = 1; o < LP; o <<= 1) s += __shfl_xor(s, o, 64);
-    if (l == 0 && base + p0 < end) keys[base + p0] = key_of(id >= 0 ? s : -__builtin_inf());
+    if (l != 0 || base + p0 >= end) return;
+    if constexpr (GROUPS) {
+      const float x = id < 0 ? -__builtin_inff() : fabs(s) <= 0x1p126 ? (float)s : __builtin_nanf("");
+      if (id >= 0) largest = fmaxf(largest, fabsf(x));
+      reinterpret_cast<float*>(keys)[base + p0] = x;
+    } else {
+      keys[base + p0] = key_of(id >= 0 ? s : -__builtin_inf());
+    }
   };
+  const int begin_w = base;
   for (; base < end; base += 2 * STEP) {
     int id2 = id_of(base + 2 * STEP);
     load(v[1], id_next);
@@ -150,101 +169,230 @@ __global__ __launch_bounds__(kThreads) void page_scores_kernel(Args a) {
     score(v[1], base + STEP, id_next);
     id_next = id2;
   }
+  if constexpr (GROUPS) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor(largest, o, 64));
+    if (lane == 0 && begin_w < end) reinterpret_cast<float*>(keys)[a.key_stride + blockIdx.y * kWaves + w] = largest * 0x1p-23f + kLeast;
+  }
 }
 
-// Rows that go together: 16 x 16 (rows, pages) at a time, four channels an instruction.  A lane has row lane % 16's weights and page
-// lane % 16's bounds of the chunks 4 j + lane / 16 of [lo | hi], eight values each.
+// Rows that go together: 16 x 16 (rows, pages) at a time, 32 channels an instruction, in fewer bits than the choice needs: a weight w
+// is the sum of two bf16 numbers to |w| 2^-16, their products with the bounds are exact in 32 bits, and each of the 4 HD additions is
+// off by no more than two steps of the last place, 2^-22 of S = sum |w| |bound|; G heads are added up for a weight, each to 2^-24.  A third
+// product gives S (of the weights' first numbers, no less than 1 - 2^-8 of it).  Written are the score and, for a wave's pages of a
+// row, the largest error; what no such bound holds for (infinite or no numbers) is written as none.
+// A lane has row lane % 16's weights and page lane % 16's bounds of the chunks 4 j + lane / 16 of [lo | hi], eight values each.
 template <int HD>
-__global__ __launch_bounds__(kThreads, 2) void page_scores_tiles_kernel(Args a) {
+__global__ __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) void page_screen_kernel(Args a) {
   constexpr int CH = HD / 4, J = CH / 4;      // chunks of a row of bounds, of them a lane's
-  constexpr int LD = 2 * HD + 2;              // doubles between rows in LDS: reads of 16 rows hit other banks
-  __shared__ __attribute__((aligned(16))) double wgt_s[kRows * LD];
+  constexpr int LD = 2 * HD + 8;              // numbers between rows in LDS: reads of 16 rows hit other banks
+  __shared__ __attribute__((aligned(16))) uint16_t wgt_s[2][kRows * LD];
   const int group = blockIdx.x / a.nkv, h = blockIdx.x - group * a.nkv, t0 = group * kRows;
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n16 = lane & 15, kq = lane >> 4;
-  const unsigned begins = begins_of(a, t0, lane);
+  int seqs;
+  const unsigned begins = begins_of(a, t0, lane, seqs);
   if (!together(begins)) return;
   const int G = a.nh / a.nkv;
-  // the workgroup's run: rows r0 .. r1 of the group
-  const int chunks = gridDim.y / kRuns, run = blockIdx.y / chunks;
-  unsigned rest = begins;
-  for (int i = 0; i < run; ++i) rest &= rest - 1;
-  const int r0 = __ffs(rest) - 1, r1 = __ffs(begins >> (r0 + 1)) + r0;
-  if (r0 >= kRows || t0 + r0 >= a.T) return;
-  // weights of the group's rows
-  for (int i = tid; i < kRows * (HD / 8); i += kThreads) {
-    const int row = i / (HD / 8), c = i - row * (HD / 8), t = min(t0 + row, a.T - 1);
-    double up[8] = {}, down[8] = {};
-    add_heads<HD>(up, down, a.q + t * a.q_stride + h * G * HD + c * 8, G);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      wgt_s[row * LD + c * 8 + j] = down[j];
-      wgt_s[row * LD + HD + c * 8 + j] = up[j];
-    }
-  }
-  int stop = 0;      // pages that row n16 needs scores of end here
-  if (n16 >= r0 && n16 < r1) {
-    const int n = pages_of(a, t0 + n16);
-    stop = n > a.count ? n - a.recent : 0;
-  }
-  int last = stop;
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) last = max(last, __shfl_xor(last, o, 64));
-  const int begin = a.first + (blockIdx.y - run * chunks) * a.chunk, end = __builtin_amdgcn_readfirstlane(min(begin + a.chunk, last));
-  if (begin >= end) return;
-  const int seq = a.row_seq[t0 + r0];
-  const bool known = seq >= 0 && seq < a.n_seqs;
-  const int* table = a.tables + (size_t)(known ? seq : 0) * a.table_stride;
-  auto id_of = [&](int base) {
-    const int p = base + n16, id = known && p < end ? table[p] : -1;
+  const float error = 1.02f * (HD * 0x1p-20f + 0x1p-16f + G * 0x1p-24f);
+  // contexts, the first run's ids and queries are loaded together
+  constexpr int STEP = kWaves * 16, TASKS = kRows * (HD / 8);
+  const int begin = a.first + blockIdx.y * a.chunk, begin_w = begin + 16 * w;
+  const int ctx = t0 + n16 < a.T ? a.ctx[t0 + n16] : 0;
+  const int* table = nullptr;
+  auto id_of = [&](int base, int end) {
+    const int p = base + n16, id = table && p < end ? table[p] : -1;
     return id >= 0 && id < a.num_blocks ? id : -1;
   };
-  u32x4 v[J];
-  auto load = [&](int id) {
+  auto table_of = [&](int r) {
+    const int seq = __builtin_amdgcn_readlane(seqs, r);
+    return seq >= 0 && seq < a.n_seqs ? a.tables + (size_t)seq * a.table_stride : nullptr;
+  };
+  table = table_of(0);
+  int id = id_of(begin_w, a.table_cols), id_next = id_of(begin_w + STEP, a.table_cols);
+  u32x4 qv[8];
+  auto q_of = [&](int i) { return a.q + min(t0 + i / (HD / 8), a.T - 1) * a.q_stride + h * G * HD + i % (HD / 8) * 8; };
+  load_heads(qv, q_of(tid % TASKS), HD, 0, G);
+  const int n = ctx <= 0 ? 0 : min((ctx - 1) / a.page + 1, a.table_cols);
+  const int stop_n16 = n > a.count ? n - a.recent : 0;      // pages that row n16 needs scores of end here
+  u32x4 v[2][J];
+  auto load = [&](u32x4* v, int id) {
     const uint16_t* bp = a.bounds + ((size_t)max(id, 0) * a.nkv + h) * 2 * HD + kq * 8;
 #pragma unroll
     for (int j = 0; j < J; ++j) v[j] = *reinterpret_cast<const u32x4*>(bp + j * 32);
   };
-  constexpr int STEP = kWaves * 16;
-  int base = begin + 16 * w, id = id_of(base), id_next = id_of(base + STEP);
-  load(id);
-  __syncthreads();
-  double wgt[J][8];
+  bf16x8 wgt[2][J];
+  bool ready = false;
+  // the runs of rows of one sequence
+  for (int r0 = 0; r0 < kRows && t0 + r0 < a.T;) {
+    const int r1 = __ffs(begins >> (r0 + 1)) + r0;
+    const int stop = n16 >= r0 && n16 < r1 ? stop_n16 : 0;
+    int last = stop;
 #pragma unroll
-  for (int j = 0; j < J; ++j)
-#pragma unroll
-    for (int s = 0; s < 8; ++s) wgt[j][s] = wgt_s[n16 * LD + (4 * j + kq) * 8 + s];
-  for (; base < end; base += STEP) {
-    d4 acc[2] = {};
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-      float x[8];
-      unpack8(v[j], x);
-#pragma unroll
-      for (int s = 0; s < 8; ++s) acc[s & 1] = __builtin_amdgcn_mfma_f64_16x16x4f64(wgt[j][s], (double)x[s], acc[s & 1], 0, 0, 0);
+    for (int o = 8; o > 0; o >>= 1) last = max(last, __shfl_xor(last, o, 64));
+    const int end = __builtin_amdgcn_readfirstlane(min(begin + a.chunk, last));
+    if (begin >= end) {
+      r0 = r1;
+      continue;
     }
-    const int now = id;
-    id = id_next;
-    load(id);
-    id_next = id_of(base + 2 * STEP);
-    // the lane has page n16 of rows 4 i + lane / 16
+    if (r0 > 0) {
+      table = table_of(r0);
+      id = id_of(begin_w, end);
+      id_next = id_of(begin_w + STEP, end);
+    }
+    load(v[0], id);
+    if (!ready) {
+      // weights of the group's rows
+      for (int i = tid; i < TASKS; i += kThreads) {
+        const int row = i / (HD / 8), c = i - row * (HD / 8);
+        if (i > tid) load_heads(qv, q_of(i), HD, 0, G);
+        float both[2][8] = {};
+        for (int g0 = 0; g0 < G; g0 += 8) {
+          if (g0 > 0) load_heads(qv, q_of(i), HD, g0, G);
+#pragma unroll
+          for (int g = 0; g < 8; ++g) {
+            if (g0 + g >= G) break;
+            float x[8];
+            unpack8(qv[g], x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              both[0][j] += x[j] - fabsf(x[j]);      // twice the smaller of x and 0
+              both[1][j] += x[j] + fabsf(x[j]);
+            }
+          }
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          float x[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) both[half][j] *= 0.5f;
+          const u32x4 high = pack8(both[half]);
+          unpack8(high, x);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = both[half][j] - x[j];
+          *reinterpret_cast<u32x4*>(&wgt_s[0][row * LD + half * HD + c * 8]) = high;
+          *reinterpret_cast<u32x4*>(&wgt_s[1][row * LD + half * HD + c * 8]) = pack8(x);
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) wgt[s][j] = *reinterpret_cast<const bf16x8*>(&wgt_s[s][n16 * LD + (4 * j + kq) * 8]);
+      ready = true;
+    }
+    // the lane has page n16 of rows 4 kq + i
+    int stops[4];
+    float largest[4] = {}, *to[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int row = 4 * i + kq, p = base + n16;
-      if (p < __shfl(stop, row, 64)) a.keys[((size_t)(t0 + row) * a.nkv + h) * a.key_stride + p] = key_of(now >= 0 ? acc[0][i] + acc[1][i] : -__builtin_inf());
+      stops[i] = __shfl(stop, 4 * kq + i, 64);
+      to[i] = reinterpret_cast<float*>(a.keys + ((size_t)(t0 + 4 * kq + i) * a.nkv + h) * a.key_stride);
     }
+    auto score = [&](const u32x4* v, int base, int id) {
+      f32x4 acc[2] = {}, sum = {};
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wgt[0][j], as_bf16x8(v[j]), acc[0], 0, 0, 0);
+        acc[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wgt[1][j], as_bf16x8(v[j]), acc[1], 0, 0, 0);
+        // the weights of lo are none above zero, those of hi none below it
+        const u32x4 size = j < J / 2 ? v[j] | 0x80008000u : v[j] & 0x7fff7fffu;
+        sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wgt[0][j], as_bf16x8(size), sum, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int p = base + n16;
+        if (p >= stops[i]) continue;
+        float x = acc[0][i] + acc[1][i];
+        if (!(fabsf(x) <= 0x1p126f && sum[i] <= 0x1p126f)) x = __builtin_nanf("");
+        if (id < 0) x = -__builtin_inff();
+        else largest[i] = fmaxf(largest[i], sum[i]);
+        to[i][p] = x;
+      }
+    };
+    for (int base = begin_w; base < end; base += 2 * STEP) {
+      int id2 = id_of(base + 2 * STEP, end);
+      load(v[1], id_next);
+      score(v[0], base, id);
+      if (base + STEP >= end) break;
+      id = id2;
+      load(v[0], id);
+      id2 = id_of(base + 3 * STEP, end);
+      score(v[1], base + STEP, id_next);
+      id_next = id2;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) largest[i] = fmaxf(largest[i], __shfl_xor(largest[i], o, 64));
+      if (n16 == 0 && begin_w < stops[i]) to[i][a.key_stride + blockIdx.y * kWaves + w] = largest[i] * error + kLeast;
+    }
+    r0 = r1;
   }
 }
 
 // A workgroup per (row, kv head).  The threshold is found by digits of 8 bits within the window that still holds it, the first one
 // cut from the range of the keys; then the kept pages are written in order.  R > 0: a thread has R of the keys in registers.
+struct Long {
+  u64 lo[kWaves], hi[kWaves];
+  int hist[256];
+  int eq[kWaves], kept[kWaves], digit, above, in;
+};
+
 struct Shared {
   u64 lo[kWaves], hi[kWaves];
   int hist[3][256];
   int eq[32][kWaves], kept[32][kWaves];
+  Long any;
 };
 
+// The digit of the need-th largest; `need` becomes what is needed of it and `in` what has it.  Every wave does this for itself.
+__device__ __forceinline__ int digit_of(const int* hist, int lane, int& need, int& in) {
+  // a lane's digits are 4 lane .. 4 lane + 3; how many keys lie above each
+  const int4 c = reinterpret_cast<const int4*>(hist)[lane];
+  const int own = c.x + c.y + c.z + c.w;
+  int above = own;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int x = __shfl_down(above, o, 64);
+    if (lane + o < 64) above += x;
+  }
+  above -= own;
+  int digit = -1, over = 0, has = 0;
+  const int cs[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+  for (int j = 3; j >= 0; --j) {
+    if (above < need && above + cs[j] >= need) {
+      digit = 4 * lane + j;
+      over = above;
+      has = cs[j];
+    }
+    above += cs[j];
+  }
+  const int src = __ffsll((u64)__ballot(digit >= 0)) - 1;      // one lane has it
+  need -= __shfl(over, src, 64);
+  in = __shfl(has, src, 64);
+  return __shfl(digit, src, 64);
+}
+
+// The kept of R * 256 in order; sh.kept has their numbers by turn and wave.
 template <int R>
-__device__ __forceinline__ void pick(const Args& a, const u64* keys, int begin, int end, int need, int* out, Shared& sh) {
+__device__ __forceinline__ void write_kept(const u64* kept, int begin, int* out, const Shared& sh) {
+  const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
+  int at = 0;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    int mine = at;
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) {
+      if (v < w) mine += sh.kept[r][v];
+      at += sh.kept[r][v];
+    }
+    if (kept[r] >> lane & 1) out[mine + __popcll(kept[r] & ((1ull << lane) - 1))] = begin + r * kThreads + tid;
+  }
+}
+
+template <int R>
+__device__ __forceinline__ void pick(const u64* keys, int begin, int end, int need, int* out, Shared& sh) {
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
   u64 k[R];
   u64 lo = ~0ull, hi = 0;
@@ -284,31 +432,9 @@ __device__ __forceinline__ void pick(const Args& a, const u64* keys, int begin, 
       if (there(r) && k[r] >= lo && k[r] <= hi) atomicAdd(&hist[(int)((k[r] - lo) >> shift)], 1);
     sh.hist[(turn + 1) % 3][tid] = 0;      // its last readers are before the last barrier
     __syncthreads();
-    // every wave: lane's digits are 4 lane .. 4 lane + 3; how many keys lie above each
-    const int4 c = reinterpret_cast<const int4*>(hist)[lane];
-    int above = c.x + c.y + c.z + c.w;
-    const int own = above;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int x = __shfl_down(above, o, 64);
-      if (lane + o < 64) above += x;
-    }
-    above -= own;
-    int digit = -1, over = 0, in = 0;
-    const int cs[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-    for (int j = 3; j >= 0; --j) {
-      if (above < need && above + cs[j] >= need) {
-        digit = 4 * lane + j;
-        over = above;
-        in = cs[j];
-      }
-      above += cs[j];
-    }
-    const int src = __ffsll((u64)__ballot(digit >= 0)) - 1;      // one lane has it
-    digit = __shfl(digit, src, 64);
-    need -= __shfl(over, src, 64);
-    whole = __shfl(in, src, 64) == need;
+    int in;
+    const int digit = digit_of(hist, lane, need, in);
+    whole = in == need;
     lo += (u64)digit << shift;
     hi = lo + min(hi - lo, (u64)((1ull << shift) - 1));      // lo + 2^shift may not fit
   }
@@ -341,48 +467,28 @@ __device__ __forceinline__ void pick(const Args& a, const u64* keys, int begin, 
   for (int r = 0; r < R; ++r)
     if (lane == 0) sh.kept[r][w] = __popcll(kept[r]);
   __syncthreads();
-  int at = 0;
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    int mine = at;
-#pragma unroll
-    for (int v = 0; v < kWaves; ++v) {
-      if (v < w) mine += sh.kept[r][v];
-      at += sh.kept[r][v];
-    }
-    if (kept[r] >> lane & 1) out[mine + __popcll(kept[r] & ((1ull << lane) - 1))] = begin + r * kThreads + tid;
+  write_kept<R>(kept, begin, out, sh);
+}
+
+// W waves together: all of a workgroup's, or one by itself.
+template <int W>
+__device__ __forceinline__ void sync() {
+  if constexpr (W > 1) {
+    __syncthreads();
+  } else {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   }
 }
 
-// MOST: keys of a thread in registers at most (their number is the kernel's registers, and so how many workgroups share a compute unit)
-template <int MOST>
-__global__ __launch_bounds__(kThreads) void pick_pages_kernel(Args a) {
-  const int t = blockIdx.x / a.nkv, h = blockIdx.x - t * a.nkv, tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
-  const int n = pages_of(a, t);
-  int* out = a.out + ((size_t)t * a.nkv + h) * a.count;
-  if (n <= a.count) {
-    for (int i = tid; i < a.count; i += kThreads) out[i] = i < n ? i : -1;
-    return;
-  }
-  const u64* keys = a.keys + ((size_t)t * a.nkv + h) * a.key_stride;
-  const int begin = a.first, end = n - a.recent;
-  int need = a.count - a.first - a.recent;
-  for (int i = tid; i < a.first; i += kThreads) out[i] = i;
-  for (int i = tid; i < a.recent; i += kThreads) out[a.count - a.recent + i] = n - a.recent + i;
-  if (need == 0) return;
-  __shared__ __attribute__((aligned(16))) Shared sh;
-  out += a.first;
-  if (end - begin <= 2 * kThreads) return pick<2>(a, keys, begin, end, need, out, sh);
-  if (end - begin <= 4 * kThreads) return pick<4>(a, keys, begin, end, need, out, sh);
-  if constexpr (MOST > 4) {
-    if (end - begin <= 8 * kThreads) return pick<8>(a, keys, begin, end, need, out, sh);
-    if (end - begin <= 16 * kThreads) return pick<16>(a, keys, begin, end, need, out, sh);
-    if (end - begin <= 32 * kThreads) return pick<32>(a, keys, begin, end, need, out, sh);
-  }
-
-  // longer ones read their keys anew each time: the same in loops
+// The same for any number of keys, read anew each time, by W waves.
+template <int W>
+__device__ void pick_long(const u64* keys, int begin, int end, int need, int* out, Long& sh) {
+  constexpr int N = 64 * W;
+  const int tid = threadIdx.x % N, w = tid >> 6, lane = tid & 63;
   u64 lo = ~0ull, hi = 0;
-  for (int i = begin + tid; i < end; i += kThreads) {
+  for (int i = begin + tid; i < end; i += N) {
     lo = min(lo, keys[i]);
     hi = max(hi, keys[i]);
   }
@@ -395,110 +501,380 @@ __global__ __launch_bounds__(kThreads) void pick_pages_kernel(Args a) {
     sh.lo[w] = lo;
     sh.hi[w] = hi;
   }
-  __syncthreads();
-  for (int v = 0; v < kWaves; ++v) {
+  sync<W>();
+  for (int v = 0; v < W; ++v) {
     lo = min(lo, sh.lo[v]);
     hi = max(hi, sh.hi[v]);
   }
-  __shared__ int s_digit, s_above, s_in;
   bool whole = false;
   while (lo < hi) {
-    int* hist = sh.hist[0];
     const int shift = max(64 - __clzll(hi - lo) - 8, 0);
-    hist[tid] = 0;
-    __syncthreads();
-    for (int i = begin + tid; i < end; i += kThreads) {
+    for (int i = tid; i < 256; i += N) sh.hist[i] = 0;
+    sync<W>();
+    for (int i = begin + tid; i < end; i += N) {
       const u64 k = keys[i];
-      if (k >= lo && k <= hi) atomicAdd(&hist[(int)((k - lo) >> shift)], 1);
+      if (k >= lo && k <= hi) atomicAdd(&sh.hist[(int)((k - lo) >> shift)], 1);
     }
-    __syncthreads();
+    sync<W>();
     if (tid == 0) {
       int above = 0, d = 255;
-      for (; above + hist[d] < need; --d) above += hist[d];
-      s_digit = d;
-      s_above = above;
-      s_in = hist[d];
+      for (; above + sh.hist[d] < need; --d) above += sh.hist[d];
+      sh.digit = d;
+      sh.above = above;
+      sh.in = sh.hist[d];
     }
-    __syncthreads();
-    need -= s_above;
-    lo += (u64)s_digit << shift;
+    sync<W>();
+    need -= sh.above;
+    lo += (u64)sh.digit << shift;
     hi = lo + min(hi - lo, (u64)((1ull << shift) - 1));
-    if (s_in == need) {
+    if (sh.in == need) {
       whole = true;
       break;
     }
-    __syncthreads();
+    sync<W>();
   }
   int done = 0, ties = 0;
-  for (int base = begin; base < end; base += kThreads) {
+  for (int base = begin; base < end; base += N) {
     const int i = base + tid;
     const u64 k = i < end ? keys[i] : 0;
     const bool in = i < end && k >= lo && k <= hi;
     const u64 eq = __ballot(in);
-    __syncthreads();
-    if (lane == 0) sh.eq[0][w] = __popcll(eq);
-    __syncthreads();
+    sync<W>();
+    if (lane == 0) sh.eq[w] = __popcll(eq);
+    sync<W>();
     int before = ties;
-    for (int v = 0; v < kWaves; ++v) {
-      if (v < w) before += sh.eq[0][v];
-      ties += sh.eq[0][v];
+    for (int v = 0; v < W; ++v) {
+      if (v < w) before += sh.eq[v];
+      ties += sh.eq[v];
     }
     const bool kept = i < end && (k > hi || (in && (whole || before + __popcll(eq & ((1ull << lane) - 1)) < need)));
     const u64 b = __ballot(kept);
-    if (lane == 0) sh.kept[0][w] = __popcll(b);
-    __syncthreads();
+    if (lane == 0) sh.kept[w] = __popcll(b);
+    sync<W>();
     int at = done;
-    for (int v = 0; v < kWaves; ++v) {
-      if (v < w) at += sh.kept[0][v];
-      done += sh.kept[0][v];
+    for (int v = 0; v < W; ++v) {
+      if (v < w) at += sh.kept[v];
+      done += sh.kept[v];
     }
     if (kept) out[at + __popcll(b & ((1ull << lane) - 1))] = i;
   }
 }
 
+// 32-bit integers of the order of the floats; no number is the largest.
+__device__ __forceinline__ unsigned key_of(float x) {
+  const unsigned b = __float_as_uint(x + 0.f);
+  return x != x ? ~0u : b >> 31 ? ~b : b | 1u << 31;
+}
+__device__ __forceinline__ float float_of(unsigned k) { return __uint_as_float(k >> 31 ? k ^ 1u << 31 : ~k); }
+
+// A page's score in 64 bits by 16 lanes; `l` is the lane's place among them.
+__device__ __forceinline__ u64 score_of(const Args& a, const double* wgt, const int* table, int h, int p, int l) {
+  const int id = table ? table[p] : -1;
+  if (id < 0 || id >= a.num_blocks) return key_of(-__builtin_inf());
+  const uint16_t* b = a.bounds + ((size_t)id * a.nkv + h) * 2 * a.hd;
+  double sum[2] = {};
+  for (int c = l; c < a.hd / 4; c += 16) {
+    float x[8];
+    unpack8(*reinterpret_cast<const u32x4*>(b + c * 8), x);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum[j & 1] = fma(wgt[c * 8 + j], (double)x[j], sum[j & 1]);
+  }
+  double s = sum[0] + sum[1];
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) s += __shfl_xor(s, o, 64);
+  return key_of(s);
+}
+
+// From scores that are off by an error E at most.  With the threshold of these scores in [lo, hi], that of the true ones is in
+// [lo - E, hi + E]: pages above hi + 2 E are kept, those below lo - 2 E are not, and those between (1 to 8 of 1000 where bounds are normal) are scored again in
+// 64 bits and take the places that are left.  Where there are too many of them, or scores without a bound, all are.
+// W waves a row: one for up to 1024 pages (1018 rows over 730 to 1000 pages of 4 heads: 21 us, by all four of a workgroup 45), four for
+// more.  A wave has turns * 64 pages in a row, R > 0: R of them at most a lane, in registers; 0: they are read anew each time.
+template <int R, int W>
+struct Screened {
+  static constexpr int kBand = 64 * W;      // pages scored again at most: a thread each
+  Long any;
+  unsigned lo[W], hi[W];
+  float error[W];
+  int sure[W], band, page[kBand];
+  u64 key[kBand];
+  u64 kept[R ? R * W : 1];      // of the pages scored again: a bit a page
+};
+
+template <int R, int W>
+__global__ __launch_bounds__(kThreads) void pick_screened_kernel(Args a) {
+  constexpr int N = 64 * W;
+  typedef Screened<R, W> S;
+  extern __shared__ __attribute__((aligned(16))) double wgt_s[];      // 2 hd a row: of lo, of hi
+  __shared__ __attribute__((aligned(16))) S teams[kWaves / W];
+  const int team = __builtin_amdgcn_readfirstlane(threadIdx.x / N), tid = threadIdx.x % N, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int item = blockIdx.x * (kWaves / W) + team, t = item / a.nkv, h = item - t * a.nkv, G = a.nh / a.nkv;
+  if (t >= a.T) return;
+  S& s = teams[team];
+  double* wgt = wgt_s + team * 2 * a.hd;
+  u64* row = a.keys + ((size_t)t * a.nkv + h) * a.key_stride;
+  float* scores = reinterpret_cast<float*>(row);
+  // all that is read is under way together; a wave by itself reads scores before it knows how many there are
+  int seqs;
+  const bool tiles = together(begins_of(a, t, lane, seqs));
+  const int ctx = a.ctx[t], begin = a.first;
+  float raw[R ? R : 1], E_first = tid < a.table_cols ? scores[a.key_stride + tid] : 0.f;
+  if constexpr (W == 1) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int i = begin + r * 64 + lane;
+      raw[r] = i < a.table_cols ? scores[i] : 0.f;
+    }
+  }
+  weigh<N>(wgt, a.q + t * a.q_stride + h * G * a.hd, a.hd, G);
+  const int n = ctx <= 0 ? 0 : min((ctx - 1) / a.page + 1, a.table_cols), seq = __builtin_amdgcn_readlane(seqs, t % kRows);
+  int* out = a.out + ((size_t)t * a.nkv + h) * a.count;
+  if (n <= a.count) {
+    for (int i = tid; i < a.count; i += N) out[i] = i < n ? i : -1;
+    return;
+  }
+  const int end = n - a.recent, need = a.count - a.first - a.recent;
+  for (int i = tid; i < a.first; i += N) out[i] = i;
+  for (int i = tid; i < a.recent; i += N) out[a.count - a.recent + i] = end + i;
+  if (need == 0) return;
+  out += a.first;
+  const int turns = (end - begin + N - 1) / N, begin_w = begin + w * turns * 64;
+  unsigned k[R ? R : 1];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int i = begin_w + r * 64 + lane;
+    const bool there = r < turns && i < end;
+    if constexpr (W > 1) raw[r] = there ? scores[i] : 0.f;
+    k[r] = there ? key_of(raw[r]) : 0;      // below any score's
+  }
+  // `f` of the turns' keys
+  auto each = [&](auto f) {
+    if constexpr (R > 0) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (r < turns) f(r, k[r]);
+    } else {
+      for (int r = 0; r < turns; ++r) {
+        const int i = begin_w + r * 64 + lane;
+        f(r, i < end ? key_of(scores[i]) : 0u);
+      }
+    }
+  };
+  // errors are those of chunks of pages, 16 or 1024 / hd of them a wave at a time
+  const int chunk = tiles ? a.chunk : a.row_chunk, width = tiles ? 16 : 1024 / a.hd;
+  float E = 0.f;
+  for (int i = tid; (i / kWaves) * chunk + width * (i % kWaves) < end - begin; i += N)
+    if (width * (i % kWaves) < chunk) E = fmaxf(E, i == tid ? E_first : scores[a.key_stride + i]);
+  unsigned lo = ~0u, hi = 0;
+  each([&](int, unsigned x) {
+    lo = min(lo, x ? x : ~0u);
+    hi = max(hi, x);
+  });
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    lo = min(lo, (unsigned)__shfl_xor((int)lo, o, 64));
+    hi = max(hi, (unsigned)__shfl_xor((int)hi, o, 64));
+    E = fmaxf(E, __shfl_xor(E, o, 64));
+  }
+  if constexpr (R > 0) {
+    for (int i = tid; i < R * W; i += N) s.kept[i] = 0;
+  }
+  if (tid == 0) s.band = 0;
+  if constexpr (W > 1) {
+    if (lane == 0) {
+      s.lo[w] = lo;
+      s.hi[w] = hi;
+      s.error[w] = E;
+    }
+    sync<W>();
+#pragma unroll
+    for (int v = 0; v < W; ++v) {
+      lo = min(lo, s.lo[v]);
+      hi = max(hi, s.hi[v]);
+      E = fmaxf(E, s.error[v]);
+    }
+  }
+  const int* table = seq >= 0 && seq < a.n_seqs ? a.tables + (size_t)seq * a.table_stride : nullptr;
+  const int l16 = lane & 15, p16 = tid >> 4;
+  if (hi != ~0u) {
+    int left = need;      // places for the pages of the window [lo, hi]
+    while (lo < hi && !(float_of(hi) - float_of(lo) <= E)) {
+      const int shift = max(32 - __clz(hi - lo) - 8, 0);
+      for (int i = tid; i < 256; i += N) s.any.hist[i] = 0;
+      sync<W>();
+      each([&](int, unsigned x) {
+        if (x >= lo && x <= hi) atomicAdd(&s.any.hist[(x - lo) >> shift], 1);
+      });
+      sync<W>();
+      int in;
+      const int digit = digit_of(s.any.hist, lane, left, in);
+      lo += (unsigned)digit << shift;
+      hi = lo + min(hi - lo, (1u << shift) - 1);
+      sync<W>();
+    }
+    const float from = float_of(lo) - 2.01f * E, above = float_of(hi) + 2.01f * E;
+    const unsigned from_k = key_of(from), above_k = key_of(above);
+    int sure = 0;
+    sync<W>();
+    each([&](int r, unsigned x) {
+      const u64 over = __ballot(x > above_k), between = __ballot(x >= from_k && x <= above_k);
+      sure += __popcll(over);
+      if (!between) return;
+      int at = 0;
+      if (lane == 0) at = atomicAdd(&s.band, __popcll(between));
+      at = __shfl(at, 0, 64) + __popcll(between & ((1ull << lane) - 1));
+      if ((between >> lane & 1) && at < S::kBand) s.page[at] = begin_w + r * 64 + lane;
+    });
+    if constexpr (W > 1) {
+      if (lane == 0) s.sure[w] = sure;
+    }
+    sync<W>();
+    if constexpr (W > 1) {
+      sure = 0;
+#pragma unroll
+      for (int v = 0; v < W; ++v) sure += s.sure[v];
+    }
+    const int m = __builtin_amdgcn_readfirstlane(s.band);
+    left = need - sure;
+    if (m <= S::kBand) {
+      if (m > left)
+        for (int i = p16; i < m; i += N / 16) {
+          const u64 x = score_of(a, wgt, table, h, s.page[i], l16);
+          if (l16 == 0) s.key[i] = x;
+        }
+      sync<W>();
+      if (tid < m) {
+        const int p = s.page[tid];
+        const u64 x = s.key[tid];
+        int before = 0;
+        if (m > left)
+          for (int i = 0; i < m; ++i) before += s.key[i] > x || (s.key[i] == x && s.page[i] < p);
+        if constexpr (R > 0) {
+          if (before < left) atomicOr(reinterpret_cast<unsigned*>(s.kept) + (p - begin) / 32, 1u << (p - begin) % 32);
+        } else {
+          scores[p] = before < left ? __builtin_inff() : -__builtin_inff();
+        }
+      }
+      sync<W>();
+      // the kept ones in order: after those of the waves before
+      auto kept_of = [&](int r, unsigned x) {
+        u64 b = __ballot(x > above_k);
+        if constexpr (R > 0) b |= s.kept[w * turns + r];
+        return b;
+      };
+      int at = 0;
+      if constexpr (W > 1) {
+        int mine = 0;
+        each([&](int r, unsigned x) { mine += __popcll(kept_of(r, x)); });
+        if (lane == 0) s.sure[w] = mine;
+        sync<W>();
+        for (int v = 0; v < w; ++v) at += s.sure[v];
+      }
+      each([&](int r, unsigned x) {
+        const u64 b = kept_of(r, x);
+        if (b >> lane & 1) out[at + __popcll(b & ((1ull << lane) - 1))] = begin_w + r * 64 + lane;
+        at += __popcll(b);
+      });
+      return;
+    }
+  }
+  sync<W>();
+  for (int p = begin + p16; p < end; p += N / 16) {
+    const u64 x = score_of(a, wgt, table, h, p, l16);
+    if (l16 == 0) row[p] = x;
+  }
+  sync<W>();
+  pick_long<W>(row, begin, end, need, out, s.any);
+}
+
+// MOST: keys of a thread in registers at most (their number is the kernel's registers, and so how many workgroups share a compute unit).
+template <int MOST>
+__global__ __launch_bounds__(kThreads) void pick_pages_kernel(Args a) {
+  const int t = blockIdx.x / a.nkv, h = blockIdx.x - t * a.nkv, tid = threadIdx.x;
+  const int n = pages_of(a, t);
+  int* out = a.out + ((size_t)t * a.nkv + h) * a.count;
+  if (n <= a.count) {
+    for (int i = tid; i < a.count; i += kThreads) out[i] = i < n ? i : -1;
+    return;
+  }
+  const u64* keys = a.keys + ((size_t)t * a.nkv + h) * a.key_stride;
+  const int begin = a.first, end = n - a.recent;
+  const int need = a.count - a.first - a.recent;
+  for (int i = tid; i < a.first; i += kThreads) out[i] = i;
+  for (int i = tid; i < a.recent; i += kThreads) out[a.count - a.recent + i] = end + i;
+  if (need == 0) return;
+  out += a.first;
+  __shared__ __attribute__((aligned(16))) Shared sh;
+  if (end - begin <= 2 * kThreads) return pick<2>(keys, begin, end, need, out, sh);
+  if (end - begin <= 4 * kThreads) return pick<4>(keys, begin, end, need, out, sh);
+  if constexpr (MOST > 4) {
+    if (end - begin <= 8 * kThreads) return pick<8>(keys, begin, end, need, out, sh);
+    if (end - begin <= 16 * kThreads) return pick<16>(keys, begin, end, need, out, sh);
+    if (end - begin <= 32 * kThreads) return pick<32>(keys, begin, end, need, out, sh);
+  }
+  pick_long<kWaves>(keys, begin, end, need, out, sh.any);
+}
+
 template <int HD>
-int scores(Args a, bool groups, hipStream_t s) {
+int scores(Args& a, bool groups, hipStream_t s) {
   const int span = a.table_cols - a.first - a.recent, tiles = (a.T + kRows - 1) / kRows * a.nkv;
   // pages of a workgroup, a multiple of `unit`, so that there are about `want` workgroups
   auto chunk = [&](long long items, int unit, int want, int most) {
     return (int)min(max((items * span / want + unit - 1) / unit * unit, (long long)unit), (long long)most);
   };
-  Args rows = a;
-  rows.chunk = chunk((long long)a.nkv * a.T, 32, 2048, 1024);
-  const dim3 grid(a.nkv * a.T, (span + rows.chunk - 1) / rows.chunk);
-  if constexpr (HD <= 128) {      // 256 dims: a row's weights do not fit a lane's registers
-    if (groups) {
-      a.chunk = chunk(tiles, 64, 1024, 1 << 20);
-      page_scores_tiles_kernel<HD><<<dim3(tiles, (span + a.chunk - 1) / a.chunk * kRuns), kThreads, 0, s>>>(a);
-      DGI_CHECK_LAUNCH();
-      page_scores_kernel<HD, true><<<grid, kThreads, 0, s>>>(rows);
-      DGI_CHECK_LAUNCH();
-      return 0;
-    }
+  a.row_chunk = chunk((long long)a.nkv * a.T, 32, 2048, 1024);
+  const dim3 grid(a.nkv * a.T, (span + a.row_chunk - 1) / a.row_chunk);
+  if (!groups) {
+    page_scores_kernel<HD, false><<<grid, kThreads, 0, s>>>(a);
+    DGI_CHECK_LAUNCH();
+    return 0;
   }
-  page_scores_kernel<HD, false><<<grid, kThreads, 0, s>>>(rows);
+  a.chunk = chunk(tiles, 64, 1024, 1 << 20);
+  page_screen_kernel<HD><<<dim3(tiles, (span + a.chunk - 1) / a.chunk), kThreads, 0, s>>>(a);
+  DGI_CHECK_LAUNCH();
+  page_scores_kernel<HD, true><<<grid, kThreads, 0, s>>>(a);
   DGI_CHECK_LAUNCH();
   return 0;
+}
+
+template <int R, int W>
+void pick_screened(const Args& a, hipStream_t s) {
+  constexpr int rows = kWaves / W;
+  pick_screened_kernel<R, W><<<(a.nkv * a.T + rows - 1) / rows, kThreads, rows * 2 * a.hd * sizeof(double), s>>>(a);
 }
 
 }  // namespace
 
 extern "C" int dgi_select_pages(const void* q, long long q_stride, const void* bounds, const int* tables, int table_stride, int table_cols,
                                 int n_seqs, int num_blocks, const int* ctx, const int* row_seq, int T, int nh, int nkv, int hd, int page,
-                                int count, int first, int recent, void* keys, int key_stride, int* out, hipStream_t s) {
-  if (T == 0) return 0;
-  const Args a{(const uint16_t*)q, q_stride, (const uint16_t*)bounds, tables, table_stride, table_cols, n_seqs, num_blocks, ctx, row_seq,
-               T, nh, nkv, page, count, first, recent, (u64*)keys, key_stride, out, 0};
-  if (table_cols > count) {
-    const bool groups = row_seq && T > n_seqs;      // else hardly two rows of one sequence
-    int rc = -5;
-    if (hd == 64) rc = scores<64>(a, groups, s);
-    else if (hd == 128) rc = scores<128>(a, groups, s);
-    else if (hd == 256) rc = scores<256>(a, groups, s);
-    if (rc) return rc;
+                                int count, int first, int recent, void* keys, int key_stride, int key_rows, int* out, hipStream_t s) {
+  const bool groups = row_seq && T > n_seqs;      // else hardly two rows of one sequence
+  for (int t0 = 0; t0 < T; t0 += key_rows) {
+    Args a{(const uint16_t*)q + t0 * q_stride, q_stride, (const uint16_t*)bounds,
+           row_seq ? tables : tables + (size_t)t0 * table_stride, table_stride, table_cols, row_seq ? n_seqs : n_seqs - t0, num_blocks,
+           ctx + t0, row_seq ? row_seq + t0 : nullptr, min(key_rows, T - t0), nh, nkv, hd, page, count, first, recent, (u64*)keys,
+           key_stride, out + (size_t)t0 * nkv * count, 0, 0};
+    if (table_cols > count) {
+      int rc = -5;
+      if (hd == 64) rc = scores<64>(a, groups, s);
+      else if (hd == 128) rc = scores<128>(a, groups, s);
+      else if (hd == 256) rc = scores<256>(a, groups, s);
+      if (rc) return rc;
+    }
+    const int span = table_cols - first - recent;
+    if (!groups || table_cols <= count) {
+      if (span <= 4 * kThreads) pick_pages_kernel<4><<<nkv * a.T, kThreads, 0, s>>>(a);
+      else pick_pages_kernel<32><<<nkv * a.T, kThreads, 0, s>>>(a);
+    } else if (span <= 4 * 64) {
+      pick_screened<4, 1>(a, s);
+    } else if (span <= 16 * 64) {
+      pick_screened<16, 1>(a, s);
+    } else if (span <= 32 * kThreads) {
+      pick_screened<32, kWaves>(a, s);
+    } else {
+      pick_screened<0, kWaves>(a, s);
+    }
+    DGI_CHECK_LAUNCH();
   }
-  if (table_cols - first - recent <= 4 * kThreads) pick_pages_kernel<4><<<nkv * T, kThreads, 0, s>>>(a);
-  else pick_pages_kernel<32><<<nkv * T, kThreads, 0, s>>>(a);
-  DGI_CHECK_LAUNCH();
   return 0;
 }

@@ -211,8 +211,9 @@ def select_pages(q, bounds, block_tables, context_lens, nh: int, nkv: int, page:
     ``q`` [T, >= nh * hd] rotated; ``block_tables`` [sequences, pages], row t's is ``row_seq[t]`` (None: t); ``context_lens`` [T] the keys
     that row t sees, ``page`` tokens a page.  The first ``first`` and last ``recent`` pages are kept (the page that holds the row itself
     is among the latter, so keys behind the row decide nothing), then those with the largest
-    sum over the group's heads of max(q, 0) . largest + min(q, 0) . least, which no key of the page can exceed.  Sums are taken in 64 bits;
-    ties go to the lowest page, a sum that is no number counts as -inf."""
+    P . largest + N . least, P and N the sums over the group's heads of max(q, 0) and min(q, 0), which no key of the page can exceed.
+    Pages are compared by these sums in 64 bits; ties go to the lowest page, a sum that is no number (zero times infinite) counts as
+    -inf."""
     if _native(q):
         if out is None:
             out = torch.empty(q.shape[0], nkv, count, dtype=torch.int32, device=q.device)

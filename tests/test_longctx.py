@@ -280,6 +280,98 @@ def test_select_empty_rows_and_unknown_pages(dev):
     assert longctx.select_pages(q[:0].to(dev), b.to(dev), tables.to(dev), ctx[:0].to(dev), 4, 2, 16, 8).shape == (0, 2, 8)
 
 
+@pytest.mark.parametrize("what", ["alike", "zeros", "close", "huge", "tiny", "no numbers", "a hundred alike", "two of a kind"])
+@pytest.mark.parametrize("hd,pages", [(64, 300), (128, 1300)])
+def test_select_prompts_that_need_every_bit(dev, what, hd, pages):
+    """Rows of one sequence, whose scores leave fewer bits nothing to decide with: many alike, or out of the range of 32 bits."""
+    q, b, tables, ctx, seq = _select_case(4, 2, hd, 4, [4 * pages], 33, whole=what == "alike")
+    count = 24
+    if what == "zeros":
+        q[:, ::2] = 0.0
+        q[3:9] = 0.0
+        b[:, 0] = -b[:, 0].abs()
+    elif what == "close":
+        b[:] = b[:1]
+        b[:, :, 1, 17] += (torch.randperm(b.shape[0], generator=_gen(3)) % 5).to(BF16)[:, None] * 2.0 ** -6
+        q[:, 17::hd] = 2.0 ** -30
+    elif what == "huge":
+        q, b = q * 2.0 ** 100, b * 2.0 ** 100
+    elif what == "tiny":
+        q, b = q * 2.0 ** -100, b * 2.0 ** -100
+    elif what == "no numbers":
+        b[tables[0, 7], 0, 1, 3] = math.nan
+        b[tables[0, 9], 1] = torch.tensor([math.inf, -math.inf], dtype=BF16)[:, None]
+        b[tables[0, 11], 1, 1, 5] = math.inf
+        q[2, 70], q[5, hd + 1], q[6, 0] = math.nan, math.inf, -math.inf
+    elif what == "a hundred alike":      # the best ones, more than are kept
+        b[tables[0, 40:140].long()] = b[tables[0, 40:41].long()] + 2
+    elif what == "two of a kind":
+        b[tables[0, 1:pages // 2].long()] = b[tables[0, pages // 2: 2 * (pages // 2) - 1].long()]
+    if what != "no numbers":
+        return _select_check(dev, 4, 2, 4, count, 1, 2, q, b, tables, ctx, seq)
+    # a weight of zero times an infinite bound is no number, and what that makes of a page is said by the sum itself
+    got = longctx.select_pages(q.to(dev), b.to(dev), tables.to(dev), ctx.to(dev), 4, 2, 4, count, 1, 2, row_seq=seq.to(dev)).cpu()
+    for t in range(33):
+        n = -(-int(ctx[t]) // 4)
+        x, y = q[t].double().view(2, 2, 1, hd), b[tables[0, :n].long()].double()
+        up, down = x.clamp(min=0).sum(1), x.clamp(max=0).sum(1)
+        sums = (up * y[:, :, 1].transpose(0, 1) + down * y[:, :, 0].transpose(0, 1)).sum(-1)
+        for h in range(2):
+            most = [-math.inf if math.isnan(s) else s for s in sums[h].tolist()]
+            best = sorted(range(1, n - 2), key=lambda p: (-most[p], p))[: count - 3]
+            assert got[t, h].tolist() == [0] + sorted(best) + [n - 2, n - 1]
+
+
+@pytest.mark.parametrize("hd,pages", [(64, 200), (256, 1000), (128, 1090), (64, 5000), (128, 8300), (256, 9000)])
+def test_select_rows_of_long_prompts(dev, hd, pages):
+    _select_check(dev, 3, 1, 2, 50, 2, 3, *_select_case(3, 1, hd, 2, [2 * pages], 18))
+    q, b, tables, ctx, seq = _select_case(3, 1, hd, 2, [2 * pages], 3, whole=True)
+    q[2] = 0.0
+    _select_check(dev, 3, 1, 2, 50, 2, 3, q, b, tables, ctx, seq)
+
+
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 64), (18, 2, 128), (4, 4, 256)])
+def test_select_prompts_beside_single_rows(dev, nh, nkv, hd):
+    """Sixteen rows of one to sixteen sequences, rows without a context or a sequence, pages that are none."""
+    lens = [500, 900, 31, 1, 640, 700, 410, 1200, 800, 333, 1000, 640, 555, 1500, 900]
+    runs = [1] * 10 + [30, 3, 3, 3, 17]
+    q, b, tables, ctx, seq = _select_case(nh, nkv, hd, 8, lens, 30)
+    rows = torch.cat([torch.arange(30 * i + 30 - n, 30 * i + 30) for i, n in enumerate(runs)])
+    q, ctx, seq = q[rows].contiguous(), ctx[rows].contiguous(), seq[rows].contiguous()
+    ctx[[4, 20, 55]] = torch.tensor([0, -5, 0], dtype=I32)
+    none, b = b.shape[0], torch.cat([b, torch.stack([torch.full_like(b[:1, :, 0], math.inf), torch.full_like(b[:1, :, 0], -math.inf)], 2)])
+    tables[10, [3, 50]], tables[13, 7], tables[7, 9] = none, none, none
+    given = torch.where(tables == none, torch.tensor([-1, 1 << 30], dtype=I32)[torch.arange(tables.shape[1]) % 2], tables)
+    want = _selection64(q, b, tables, ctx, nh, nkv, 8, 20, 1, 2, seq)
+    lost = torch.tensor([6, 30, 57])      # of no known sequence: all pages alike, so the lowest
+    seq[lost] = torch.tensor([-1, 15, 1 << 30], dtype=I32)
+    for t in lost.tolist():
+        n = -(-int(ctx[t]) // 8)
+        want[t] = torch.tensor(list(range(18)) + [n - 2, n - 1], dtype=I32) if n > 20 else torch.tensor(list(range(n)) + [-1] * (20 - n), dtype=I32)
+    got = longctx.select_pages(q.to(dev), b.to(dev), given.to(dev), ctx.to(dev), nh, nkv, 8, 20, 1, 2, row_seq=seq.to(dev))
+    assert torch.equal(got.cpu(), want)
+
+
+@pytest.mark.parametrize("grouped", [False, True])
+def test_select_wide_tables(dev, grouped):
+    """Tables so wide that scores of all rows together would take 300 MB and more: rows go in several batches."""
+    lens = [900 + 7 * i for i in range(104)] if not grouped else [700, 900]
+    q, b, tables, ctx, seq = _select_case(8, 8, 64, 16, lens, 52 if grouped else 1)
+    wide = torch.full((len(lens), 50000), -1, dtype=I32)
+    wide[:, : tables.shape[1]] = tables
+    _select_check(dev, 8, 8, 16, 10, 1, 1, q, b, wide, ctx, seq)
+    if not grouped:
+        got = longctx.select_pages(q.to(dev), b.to(dev), wide.to(dev), ctx.to(dev), 8, 8, 16, 10, 1, 1)
+        assert torch.equal(got.cpu(), _selection64(q, b, tables, ctx, 8, 8, 16, 10, 1, 1, seq))
+
+
+def test_select_whole_tables_of_rows(dev):
+    """A table that has no more pages than are kept, and a row more than sequences."""
+    q, b, tables, ctx, seq = _select_case(4, 2, 64, 16, [90, 160], 20)
+    _select_check(dev, 4, 2, 16, tables.shape[1], 1, 1, q, b, tables, ctx, seq)
+    _select_check(dev, 4, 2, 16, tables.shape[1] + 9, 1, 1, q, b, tables, ctx, seq)
+
+
 # ---- attention over selected pages ------------------------------------------------------------------------------------------------------
 
 def _selected_case(nh, nkv, hd, page, lens, count, rows=1, seed=0, extra=0):
