@@ -202,6 +202,20 @@ Attention check_attention(const at::Tensor& out, const at::Tensor& q, const at::
   return {hd, page, dev};
 }
 
+// What the parts of a split sum leave: a row of hd values each, and its logarithm.  Both in one tensor: allocating takes the host a
+// microsecond, which a call of one row feels.
+struct Parts {
+  at::Tensor store;
+  float *o = nullptr, *l = nullptr;
+
+  Parts(int64_t n, int64_t hd, const at::Tensor& like) {
+    if (n == 0) return;
+    store = at::empty({n * (hd + 1)}, like.options().dtype(at::kFloat));
+    o = store.data_ptr<float>();
+    l = o + n * hd;
+  }
+};
+
 void paged_selected(at::Tensor out, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& tables,
                     const at::Tensor& ctx, const at::Tensor& pages, int64_t nh, int64_t nkv, double scale,
                     const c10::optional<at::Tensor>& row_seq) {
@@ -220,24 +234,19 @@ void paged_selected(at::Tensor out, const at::Tensor& q, const at::Tensor& k, co
   // runs of 256 keys at the least, as many as give the card two workgroups a compute unit
   const int64_t least = std::max<int64_t>(1, 256 / at_.page);
   const int64_t splits = std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(1, T * nkv), (count + least - 1) / least, 64}));
-  at::Tensor part_o, part_l;
-  if (splits > 1) {
-    part_o = at::empty({T * nh * splits * at_.hd}, q.options().dtype(at::kFloat));
-    part_l = at::empty({T * nh * splits}, q.options().dtype(at::kFloat));
-  }
+  const Parts parts(splits > 1 ? T * nh * splits : 0, at_.hd, q);
   // more rows than sequences: neighbours that may read their pages together
-  at::Tensor plan, plan_n;
-  const bool together = rows && T > tables.size(0) && nh / nkv <= 8;
-  if (together) {
-    plan = at::empty({T * nkv * count * 2}, q.options().dtype(at::kLong));
-    plan_n = at::empty({T * (nkv + 1)}, q.options().dtype(at::kInt));
+  at::Tensor plan;
+  int* plan_n = nullptr;
+  if (rows && T > tables.size(0) && nh / nkv <= 8) {
+    const int64_t pairs = T * nkv * count * 2, numbers = T * (nkv + 1);
+    plan = at::empty({pairs + (numbers + 1) / 2}, q.options().dtype(at::kLong));
+    plan_n = reinterpret_cast<int*>(plan.data_ptr<int64_t>() + pairs);
   }
   check_rc(dgi_paged_selected(q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(), tables.data_ptr<int>(), (int)tables.stride(0),
                               (int)tables.size(1), (int)tables.size(0), (int)k.size(0), ctx.data_ptr<int>(), rows, pages.data_ptr<int>(),
-                              (int)count, out.data_ptr(), out.stride(0), splits > 1 ? part_o.data_ptr<float>() : nullptr,
-                              splits > 1 ? part_l.data_ptr<float>() : nullptr, (int)splits, together ? plan.data_ptr() : nullptr,
-                              together ? plan_n.data_ptr<int>() : nullptr, together ? plan_n.data_ptr<int>() + T * nkv : nullptr, (int)T, (int)nh,
-                              (int)nkv, (int)at_.hd, (int)at_.page, (float)scale, cur_stream()), op);
+                              (int)count, out.data_ptr(), out.stride(0), parts.o, parts.l, (int)splits,
+                              plan_n ? plan.data_ptr() : nullptr, plan_n, plan_n ? plan_n + T * nkv : nullptr, (int)T, (int)nh, (int)nkv, (int)at_.hd, (int)at_.page, (float)scale, cur_stream()), op);
 }
 
 void paged_tree(at::Tensor out, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& tables,
@@ -262,32 +271,22 @@ void paged_tree(at::Tensor out, const at::Tensor& q, const at::Tensor& k, const 
     const int64_t tiles = (pairs + 127) / 128, least = 4;
     const int64_t shares = std::max<int64_t>(1, std::min<int64_t>(512 / nkv, (S * tiles * ((width + 63) / 64) + least - 1) / least));
     TORCH_CHECK_VALUE(S * tiles * nkv <= kInt, op, ": too many sequences");
-    at::Tensor part_o, part_l;
-    if (shares > 1) {
-      part_l = at::empty({shares * nkv * 2 * 128}, q.options().dtype(at::kFloat));
-      part_o = at::empty({shares * nkv * 2 * 128 * at_.hd}, q.options().dtype(at::kFloat));
-    }
+    const Parts parts(shares > 1 ? shares * nkv * 2 * 128 : 0, at_.hd, q);
     check_rc(dgi_tree_tiles(q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(), tables.data_ptr<int>(), (int)tables.stride(0),
                             (int)tables.size(1), (int)S, (int)k.size(0), (int)q.size(0), cu.data_ptr<int>(), ctx.data_ptr<int>(),
                             mask.data_ptr(), (int)mask.stride(0), (int)max_nodes, out.data_ptr(), out.stride(0),
-                            shares > 1 ? part_o.data_ptr<float>() : nullptr, shares > 1 ? part_l.data_ptr<float>() : nullptr, (int)shares,
-                            (int)least, (int)nh, (int)nkv, (int)at_.hd, (int)at_.page, (float)scale, cur_stream()), op);
+                            parts.o, parts.l, (int)shares, (int)least, (int)nh, (int)nkv, (int)at_.hd, (int)at_.page, (float)scale, cur_stream()), op);
     return;
   }
   const int64_t cols = 16, tiles = (pairs + cols - 1) / cols;
   TORCH_CHECK_VALUE(S <= kInt / (nkv * tiles), op, ": too many sequences");
   const int64_t items = S * tiles * nkv, min_part = 128;
   const int64_t splits = std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(1, items), (width + min_part - 1) / min_part, 64}));
-  at::Tensor part_o, part_l;
-  if (splits > 1) {
-    part_o = at::empty({items * splits * cols * at_.hd}, q.options().dtype(at::kFloat));
-    part_l = at::empty({items * splits * cols}, q.options().dtype(at::kFloat));
-  }
+  const Parts parts(splits > 1 ? items * splits * cols : 0, at_.hd, q);
   check_rc(dgi_tree_rows(q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(), tables.data_ptr<int>(), (int)tables.stride(0),
                           (int)tables.size(1), (int)S, (int)k.size(0), (int)q.size(0), cu.data_ptr<int>(), ctx.data_ptr<int>(),
                           mask.data_ptr(), (int)mask.stride(0), (int)max_nodes, out.data_ptr(), out.stride(0),
-                          splits > 1 ? part_o.data_ptr<float>() : nullptr, splits > 1 ? part_l.data_ptr<float>() : nullptr, (int)splits,
-                          (int)min_part, (int)nh, (int)nkv, (int)at_.hd, (int)at_.page, (float)scale, cur_stream()), op);
+                          parts.o, parts.l, (int)splits, (int)min_part, (int)nh, (int)nkv, (int)at_.hd, (int)at_.page, (float)scale, cur_stream()), op);
 }
 
 }  // namespace

@@ -486,6 +486,76 @@ def test_selected_out_and_strides(dev):
     assert longctx.paged_selected(q, k, v, tables, ctx, pages, 8, 2, 0.125).shape == (0, 512)
 
 
+@pytest.mark.parametrize("nh,nkv,hd,page", [(1, 1, 64, 16), (5, 1, 128, 4), (14, 2, 128, 32), (16, 1, 64, 16), (6, 2, 256, 16), (2, 2, 128, 128),
+                                            (3, 1, 64, 1)])
+def test_selected_prompts(dev, nh, nkv, hd, page):
+    """Neighbouring rows of two sequences, whose lists have some pages in common; heads that do not divide a tile; any page."""
+    case = _selected_case(nh, nkv, hd, page, [19 * page + 3, 40 * page], 7, rows=19)
+    pages = case[5]
+    pages[3:9] = pages[3]                                   # all in common, in another order for one
+    pages[5] = pages[5].flip(-1)
+    _selected_check(dev, nh, nkv, case)
+
+
+def test_selected_prompts_with_lists_in_any_order(dev):
+    """Rows side by side: lists with pages twice, empty entries anywhere, pages behind the context, nothing; rows without a context; rows of
+    no sequence; pages that are none."""
+    case = _selected_case(4, 2, 64, 16, [500, 300], 9, rows=24)
+    q, k, v, tables, ctx, pages, seq = case
+    pages[1] = pages[1].flip(-1)
+    pages[2, 0] = torch.tensor([3, 3, -1, 30, 30, 99, 1 << 30, -(1 << 31), 0], dtype=I32)
+    pages[4] = -1
+    pages[9, 1] = torch.tensor([7] * 9, dtype=I32)
+    pages[26:29] = torch.tensor([[-1, 2, -1, 5, 18, 17, -1, 4, 0]], dtype=I32)
+    ctx[12], ctx[13] = 0, -4
+    got = _selected_check(dev, 4, 2, case)
+    assert (got[4] == 0).all() and (got[12:14] == 0).all()
+    given = [x.clone() for x in case]
+    given[3][0, 7], given[3][1, 5], given[6][17], given[6][40] = -1, 1 << 30, 2, -1
+    got = longctx.paged_selected(*(x.to(dev) for x in given[:6]), 4, 2, 0.125, row_seq=given[6].to(dev))
+    gone = pages.clone()
+    gone[(pages == 7) & (seq == 0)[:, None, None]] = -1
+    gone[(pages == 5) & (seq == 1)[:, None, None]] = -1
+    gone[17], gone[40] = -1, -1
+    want, tol = _selected_want(4, 2, 0.125, *case[:5], gone, seq)
+    _close(got, want, tol)
+
+
+@pytest.mark.parametrize("nh,count,lens,rows", [(1, 90, [9000], 33), (2, 300, [8000], 9), (8, 150, [3000, 2500], 18)])
+def test_selected_prompts_with_long_lists(dev, nh, count, lens, rows):
+    """Rows that go together have more pages between them than a workgroup holds at a time."""
+    _selected_check(dev, nh, 1, _selected_case(nh, 1, 64, 16, lens, count, rows=rows))
+
+
+def test_selected_prompts_and_pages_of_other_rows(dev):
+    """A page that one row has in its list, and its neighbour has not, holds NaN and infinities: they reach that row alone.  So do the keys
+    of the neighbour's own step that a row does not see."""
+    case = _selected_case(4, 2, 64, 16, [320], 4, rows=22)
+    q, k, v, tables, ctx, pages, seq = case
+    pages[:] = torch.tensor([1, 4, 9, 19], dtype=I32)
+    pages[:, :, 3] = ((ctx - 1) // 16)[:, None]
+    pages[6, 0, 1], pages[7, 1, 2], pages[11, :, 0] = 5, 12, 2
+    k[tables[0, 5], 0, 3] = math.nan
+    v[tables[0, 12], 1, :, ::2] = math.inf
+    v[tables[0, 2], :, 7] = math.nan
+    k[tables[0, 19], :, 15], v[tables[0, 19], :, 15] = math.nan, math.inf      # the last row's own key
+    got = longctx.paged_selected(*(x.to(dev) for x in case[:6]), 4, 2, 0.125, row_seq=seq.to(dev)).cpu()
+    want, tol = _selected_want(4, 2, 0.125, *case)
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf())
+    fin = want.isfinite()
+    assert not fin[6, :128].any() and fin[5].all() and fin[8:11].all() and not fin[21].any()
+    _close(got[fin], want[fin], tol[fin])
+
+
+def test_selected_prompts_large_scores_and_strides(dev):
+    case = _selected_case(8, 2, 64, 16, [600, 200], 6, rows=20, extra=40)
+    case[0].mul_(1e3)
+    out = torch.full((40, 8 * 64 + 24), 5.0, dtype=BF16, device=dev)
+    for scale in (0.125, -0.125, 0.0):
+        got = _selected_check(dev, 8, 2, case, scale=scale, out=out)
+        assert got.data_ptr() == out.data_ptr() and (out[:, 512:] == 5.0).all()
+
+
 # ---- trees ------------------------------------------------------------------------------------------------------------------------------
 
 def _tree_case(nh, nkv, hd, page, ctx, nodes, seed=0, extra=0, behind=0):
@@ -600,6 +670,71 @@ def test_tree_unknown_pages(dev):
     for i, (p, o) in enumerate(ids):
         k2[i // 16, :, i % 16], v2[i // 16, :, i % 16] = k[p, :, o], v[p, :, o]
     want, tol = _tree_want(8, 2, 0.125, q, k2, v2, t2, cu, torch.tensor([84], dtype=I32), mask)
+    _close(got, want, tol)
+
+
+@pytest.mark.parametrize("nh,nkv,hd", [(32, 8, 128), (16, 1, 64), (8, 8, 64), (5, 1, 128), (16, 4, 256)])
+def test_tree_many_sequences(dev, nh, nkv, hd):
+    """More trees than a wave has lanes, of none to 20 nodes, contexts of nothing but the tree to some pages: both ways to split the work, with
+    padded sequences between."""
+    g = _gen(7)
+    nodes = torch.randint(0, 21, (70,), generator=g).tolist()
+    ctx = [n + int(c) for n, c in zip(nodes, torch.randint(0, 60, (70,), generator=g))]
+    nodes[3], ctx[3], nodes[4], ctx[4], nodes[69], ctx[69] = 0, 0, 0, 33, 20, 20
+    _tree_check(dev, nh, nkv, _tree_case(nh, nkv, hd, 16, ctx, nodes, behind=2), max_nodes=20)
+
+
+@pytest.mark.parametrize("nh,nkv,hd,nodes", [(32, 2, 64, [64, 7, 64]), (16, 1, 128, [40, 64]), (3, 1, 64, [64, 64]), (12, 4, 256, [64, 50])])
+@pytest.mark.parametrize("page", [4, 16, 256])
+def test_tree_many_nodes(dev, nh, nkv, hd, nodes, page):
+    """Trees of up to 1024 rows a kv head over contexts cut in parts."""
+    _tree_check(dev, nh, nkv, _tree_case(nh, nkv, hd, page, [n + 700 * i + 33 for i, n in enumerate(nodes)], nodes, extra=8))
+
+
+@pytest.mark.parametrize("nh,nkv,hd", [(32, 2, 64), (16, 2, 256)])
+@pytest.mark.parametrize("scale", [-0.25, 1e-30, 4.0])
+def test_tree_scales(dev, nh, nkv, hd, scale):
+    _tree_check(dev, nh, nkv, _tree_case(nh, nkv, hd, 16, [300, 40, 64], [24, 40, 64]), scale=scale)
+
+
+@pytest.mark.parametrize("nh,nkv", [(32, 2), (8, 2)])
+def test_tree_scores_without_a_scale(dev, nh, nkv):
+    """A scale of zero: every key that a row sees counts the same."""
+    case = _tree_case(nh, nkv, 64, 16, [300, 40], [24, 40])
+    got = longctx.paged_tree(*(x.to(dev) for x in case), nh, nkv, 0.0)
+    want, tol = _tree_want(nh, nkv, 0.0, *case)
+    _close(got, want, tol)
+
+
+@pytest.mark.parametrize("nh,nkv", [(32, 2), (4, 2)])
+def test_tree_rows_without_keys(dev, nh, nkv):
+    """A tree whose sequence has no context, one whose nodes see nothing and have no prefix, one with fewer keys than nodes; no page is there."""
+    case = _tree_case(nh, nkv, 64, 16, [200, 40, 33, 90], [40, 40, 33, 40])
+    q, k, v, tables, cu, ctx, mask = case
+    ctx[1] = 0
+    mask[2] = 0
+    tables[3] = -1
+    got = longctx.paged_tree(*(x.to(dev) for x in case), nh, nkv, 0.125)
+    assert (got[40:] == 0).all()
+    want, tol = _tree_want(nh, nkv, 0.125, q, k, v, tables, cu[:2], ctx[:1], mask)
+    _close(got[:40], want[:40], tol[:40])
+    ctx[0] = 7                                         # the last 40 of seven keys: nodes 33 .. 39 have keys, and none has a prefix
+    got = longctx.paged_tree(*(x.to(dev) for x in case), nh, nkv, 0.125)
+    want, tol = _tree_want(nh, nkv, 0.125, q, k, v, tables, cu[:2], ctx[:1], mask)
+    _close(got[:40], want[:40], tol[:40])
+
+
+def test_tree_more_rows_than_sequences_say(dev):
+    """More nodes than max_nodes: the first of them; row numbers behind q, and falling ones: nothing beyond."""
+    case = _tree_case(4, 2, 64, 16, [90, 70], [30, 20], behind=3)
+    out = torch.full((53, 256), 2.0, dtype=BF16, device=dev)
+    longctx.paged_tree(*(x.to(dev) for x in case), 4, 2, 0.125, max_nodes=8, out=out)
+    assert (out[8:30] == 2.0).all() and (out[38:] == 2.0).all() and (out[:8] != 2.0).any()
+    q, k, v, tables, cu, ctx, mask = case
+    cu = torch.tensor([0, 30, 99], dtype=I32)          # the second tree is cut at the last row
+    got = longctx.paged_tree(*(x.to(dev) for x in (q, k, v, tables, cu, ctx, mask)), 4, 2, 0.125)
+    want = longctx.paged_tree_ref(q, k, v, tables, torch.tensor([0, 30, 53], dtype=I32), ctx, mask, 4, 2, 0.125)
+    tol = 2 * _tree_want(4, 2, 0.125, q, k, v, tables, torch.tensor([0, 30, 53], dtype=I32), ctx, mask)[1] + 2.0 ** -8 * want.abs().double()
     _close(got, want, tol)
 
 
