@@ -1023,3 +1023,66 @@ def test_offsets_past_32_bits():
         outs.append((q, pages, o, t, kk[tt[0].long()], vv[tt[0].long()], bb[tt[0].long()]))
     for a, b in zip(*outs):
         assert torch.equal(a, b)
+
+
+@gpu
+def test_prompts_and_large_trees_on_streams_and_in_graphs():
+    """The forms for many rows: two streams at once, and two graphs that share their memory, replayed in turn between eager calls."""
+    longctx.load_native(required=True)
+    select = [[x.cuda() for x in _select_case(8, 2, 128, 16, lens, 40, seed=s)] for s, lens in ((1, [3000, 900]), (2, [1200]))]
+    selected = [[x.cuda() for x in _selected_case(8, 2, 128, 16, lens, 9, rows=40, seed=s)] for s, lens in ((3, [700, 2000]), (4, [1500]))]
+    trees = [[x.cuda() for x in _tree_case(32, 2, 128, 16, ctx, n, seed=s)] for s, ctx, n in ((5, [3000, 200, 640], [60, 33, 64]), (6, [900, 4000], [64, 40]))]
+
+    def both(i):
+        q, b, tables, ctx, seq = select[i]
+        pages = longctx.select_pages(q, b, tables, ctx, 8, 2, 16, 12, 1, 2, row_seq=seq)
+        q, k, v, tables, ctx, some, seq = selected[i]
+        return (pages, longctx.paged_selected(q, k, v, tables, ctx, some, 8, 2, 0.1, row_seq=seq), longctx.paged_tree(*trees[i], 32, 2, 0.1))
+
+    want = [both(0), both(1)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(6):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(both(i))
+    torch.cuda.synchronize()
+    with torch.inference_mode():
+        graphs, outs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+        pool = torch.cuda.graph_pool_handle()
+        for i in range(2):
+            with torch.cuda.graph(graphs[i], pool=pool):
+                outs.append(both(i))
+        for turn in range(5):
+            for i in (0, 1) if turn % 2 else (1, 0):
+                graphs[i].replay()
+                got[i].append([x.clone() for x in outs[i]])
+            got[turn % 2].append(both(turn % 2))
+            torch.cuda.synchronize()
+    for i in range(2):
+        for x in got[i]:
+            for a, b in zip(x, want[i]):
+                assert torch.equal(a, b)
+
+
+@gpu
+def test_many_rows_past_32_bits():
+    """The forms for many rows over a cache of more than 2^31 values."""
+    longctx.load_native(required=True)
+    nkv, page, hd = 8, 16, 128
+    nb = (1 << 31) // (nkv * page * hd) + 300
+    k = torch.zeros(nb, nkv, page, hd, dtype=BF16, device="cuda")
+    v, bounds = torch.zeros_like(k), torch.zeros(nb, nkv, 2, hd, dtype=BF16, device="cuda")
+    q, k0, v0, tables, ctx, pages, seq = (x.cuda() for x in _selected_case(16, nkv, hd, page, [3000], 9, rows=40))
+    far = nb - k0.shape[0]
+    b0 = torch.stack([k0.amin(2), k0.amax(2)], 2)
+    k[far:], v[far:], bounds[far:] = k0, v0, b0
+    tree = [x.cuda() for x in _tree_case(16, nkv, hd, page, [300], [64])]
+    outs = []
+    for kk, vv, bb, at in ((k, v, bounds, far), (k0, v0, b0, 0)):
+        outs.append((longctx.select_pages(q, bb, tables + at, ctx, 16, nkv, page, 12, 1, 1, row_seq=seq),
+                     longctx.paged_selected(q, kk, vv, tables + at, ctx, pages, 16, nkv, 0.1, row_seq=seq),
+                     longctx.paged_tree(tree[0], kk, vv, tables[:, :20].contiguous() + at, *tree[4:], 16, nkv, 0.1)))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b) and (a != 0).any()
