@@ -8,7 +8,7 @@
 // What they are compared by goes into a workspace [T, n_kv, pages], and another launch chooses.
 //
 // Decode rows each have bounds of their own: the scores in 64 bits as a lane multiplies what it loads, as integers of the same order, whose
-// digits from the top are counted until the threshold is found.  What bounds this is the bounds' bytes (64 rows over 4096 to 65536 keys,
+// digits from the top are counted until the threshold is found.  What bounds this is the bounds' bytes (64 rows over 4000 to 32000 keys,
 // 8 kv heads of 128, 303 MB: 72 us at 4.2 TB/s, and 7 us for the choice).
 //
 // Rows of a prompt share their sequence's bounds: 16 of them are the rows of bf16 matrix instructions, which give each score in 32 bits and
@@ -586,8 +586,8 @@ __device__ __forceinline__ u64 score_of(const Args& a, const double* wgt, const 
 }
 
 // From scores that are off by an error E at most.  With the threshold of these scores in [lo, hi], that of the true ones is in
-// [lo - E, hi + E]: pages above hi + 2 E are kept, those below lo - 2 E are not, and those between (1 to 8 of 1000 where bounds are normal) are scored again in
-// 64 bits and take the places that are left.  Where there are too many of them, or scores without a bound, all are.
+// [lo - E, hi + E]: pages above hi + 2 E are kept, those below lo - 2 E are not, and those between (1 to 8 of 1000 where
+// bounds are normal) are scored again in 64 bits and take the places that are left.  Where there are too many of them, or scores without a bound, all are.
 // W waves a row: one for up to 1024 pages (1018 rows over 730 to 1000 pages of 4 heads: 21 us, by all four of a workgroup 45), four for
 // more.  A wave has turns * 64 pages in a row, R > 0: R of them at most a lane, in registers; 0: they are read anew each time.
 template <int R, int W>
