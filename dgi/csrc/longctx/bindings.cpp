@@ -289,6 +289,47 @@ void paged_tree(at::Tensor out, const at::Tensor& q, const at::Tensor& k, const 
                           parts.o, parts.l, (int)splits, (int)min_part, (int)nh, (int)nkv, (int)at_.hd, (int)at_.page, (float)scale, cur_stream()), op);
 }
 
+// The same with an output of the call's own: allocated here, a microsecond of the host's time that the smallest calls feel is half of what it
+// takes from Python.
+at::Tensor new_rows(const at::Tensor& q, int64_t cols, const char* op) {
+  TORCH_CHECK_VALUE(q.dim() == 2 && cols >= 0 && cols <= kInt, op, ": rows of heads are two-dimensional");
+  return at::empty({q.size(0), cols}, q.options());
+}
+
+at::Tensor rope_cache_bounds_new(const at::Tensor& qkv, const at::Tensor& positions, const at::Tensor& cos_sin, int64_t nh, int64_t nkv, int64_t hd,
+                                 const at::Tensor& slots, at::Tensor k_cache, at::Tensor v_cache, at::Tensor bounds, int64_t mode) {
+  check_heads(nh, nkv, hd, "rope_cache_bounds");
+  at::Tensor out = new_rows(qkv, nh * hd, "rope_cache_bounds");
+  rope_cache_bounds(out, qkv, positions, cos_sin, nh, nkv, hd, slots, k_cache, v_cache, bounds, mode);
+  return out;
+}
+
+at::Tensor select_pages_new(const at::Tensor& q, const at::Tensor& bounds, const at::Tensor& tables, const at::Tensor& ctx, int64_t nh, int64_t nkv,
+                            int64_t page, int64_t count, int64_t first, int64_t recent, const c10::optional<at::Tensor>& row_seq) {
+  TORCH_CHECK_VALUE(q.dim() == 2 && nkv > 0 && count > 0 && count <= kInt, "select_pages: rows of heads, kv heads and pages to keep");
+  at::Tensor out = at::empty({q.size(0), nkv, count}, q.options().dtype(at::kInt));
+  select_pages(out, q, bounds, tables, ctx, nh, nkv, page, first, recent, row_seq);
+  return out;
+}
+
+at::Tensor paged_selected_new(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& tables, const at::Tensor& ctx,
+                              const at::Tensor& pages, int64_t nh, int64_t nkv, double scale, const c10::optional<at::Tensor>& row_seq) {
+  TORCH_CHECK_VALUE(k.dim() == 4, "paged_selected: k_cache must be contiguous [blocks, kv heads, block size, dims]");
+  check_heads(nh, nkv, k.size(3), "paged_selected");
+  at::Tensor out = new_rows(q, nh * k.size(3), "paged_selected");
+  paged_selected(out, q, k, v, tables, ctx, pages, nh, nkv, scale, row_seq);
+  return out;
+}
+
+at::Tensor paged_tree_new(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& tables, const at::Tensor& cu,
+                          const at::Tensor& ctx, const at::Tensor& mask, int64_t nh, int64_t nkv, double scale, int64_t max_nodes) {
+  TORCH_CHECK_VALUE(k.dim() == 4, "paged_tree: k_cache must be contiguous [blocks, kv heads, block size, dims]");
+  check_heads(nh, nkv, k.size(3), "paged_tree");
+  at::Tensor out = new_rows(q, nh * k.size(3), "paged_tree");
+  paged_tree(out, q, k, v, tables, cu, ctx, mask, nh, nkv, scale, max_nodes);
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(dgi, m) {
@@ -301,6 +342,14 @@ TORCH_LIBRARY_FRAGMENT(dgi, m) {
         "int nh, int nkv, float scale, Tensor? row_seq) -> ()");
   m.def("paged_tree(Tensor(a!) out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, Tensor cu_seqlens_q, Tensor context_lens, "
         "Tensor tree_mask, int nh, int nkv, float scale, int max_nodes) -> ()");
+  m.def("rope_cache_bounds_new(Tensor qkv, Tensor positions, Tensor cos_sin, int nh, int nkv, int hd, Tensor slot_mapping, Tensor(a!) k_cache, "
+        "Tensor(b!) v_cache, Tensor(c!) bounds, int mode) -> Tensor");
+  m.def("select_pages_new(Tensor q, Tensor bounds, Tensor block_tables, Tensor context_lens, int nh, int nkv, int page, int count, int first, "
+        "int recent, Tensor? row_seq) -> Tensor");
+  m.def("paged_selected_new(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, Tensor context_lens, Tensor pages, int nh, int nkv, "
+        "float scale, Tensor? row_seq) -> Tensor");
+  m.def("paged_tree_new(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, Tensor cu_seqlens_q, Tensor context_lens, "
+        "Tensor tree_mask, int nh, int nkv, float scale, int max_nodes) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(dgi, CUDA, m) {
@@ -309,4 +358,8 @@ TORCH_LIBRARY_IMPL(dgi, CUDA, m) {
   m.impl("select_pages", &select_pages);
   m.impl("paged_selected", &paged_selected);
   m.impl("paged_tree", &paged_tree);
+  m.impl("rope_cache_bounds_new", &rope_cache_bounds_new);
+  m.impl("select_pages_new", &select_pages_new);
+  m.impl("paged_selected_new", &paged_selected_new);
+  m.impl("paged_tree_new", &paged_tree_new);
 }

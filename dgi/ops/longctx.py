@@ -50,11 +50,12 @@ def _native(t: torch.Tensor) -> bool:
     return t.is_cuda and (_loaded or load_native(required=True))
 
 
-def _call(name: str, *args) -> None:
-    getattr(torch.ops.dgi, name)(*args)
+def _call(name: str, *args):
+    r = getattr(torch.ops.dgi, name)(*args)
     if ops._DEBUG_SYNC:
         from dgi.utils.debug import after_op
         after_op(name, *args)
+    return r
 
 
 def _need(ok: bool, op: str, what: str) -> None:
@@ -134,7 +135,7 @@ def rope_cache_bounds(qkv, positions, cos_sin, nh: int, nkv: int, hd: int, slot_
     steps of ``ModelRunner`` lay them out.  Rows with a slot outside the cache (-1) are rotated and not cached."""
     if _native(qkv):
         if out is None:
-            out = torch.empty(qkv.shape[0], nh * hd, dtype=qkv.dtype, device=qkv.device)
+            return _call("rope_cache_bounds_new", qkv, positions, cos_sin, nh, nkv, hd, slot_mapping, k_cache, v_cache, bounds, mode)
         _call("rope_cache_bounds", out, qkv, positions, cos_sin, nh, nkv, hd, slot_mapping, k_cache, v_cache, bounds, mode)
         return out
     op = "rope_cache_bounds"
@@ -216,9 +217,8 @@ def select_pages(q, bounds, block_tables, context_lens, nh: int, nkv: int, page:
     -inf."""
     if _native(q):
         if out is None:
-            out = torch.empty(q.shape[0], nkv, count, dtype=torch.int32, device=q.device)
-        else:
-            _need(out.dim() == 3 and out.shape[2] == count, "select_pages", "out must be [rows, kv heads, count]")
+            return _call("select_pages_new", q, bounds, block_tables, context_lens, nh, nkv, page, count, first, recent, row_seq)
+        _need(out.dim() == 3 and out.shape[2] == count, "select_pages", "out must be [rows, kv heads, count]")
         _call("select_pages", out, q, bounds, block_tables, context_lens, nh, nkv, page, first, recent, row_seq)
         return out
     op = "select_pages"
@@ -277,7 +277,7 @@ def paged_selected(q, k_cache, v_cache, block_tables, context_lens, pages, nh: i
     see nothing are zero."""
     if _native(q):
         if out is None:
-            out = torch.empty(q.shape[0], nh * k_cache.shape[-1], dtype=q.dtype, device=q.device)
+            return _call("paged_selected_new", q, k_cache, v_cache, block_tables, context_lens, pages, nh, nkv, scale, row_seq)
         _call("paged_selected", out, q, k_cache, v_cache, block_tables, context_lens, pages, nh, nkv, scale, row_seq)
         return out
     op = "paged_selected"
@@ -331,7 +331,7 @@ def paged_tree(q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, tr
     sequence are left as they are in ``out``, and are not set where it is None."""
     if _native(q):
         if out is None:
-            out = torch.empty(q.shape[0], nh * k_cache.shape[-1], dtype=q.dtype, device=q.device)
+            return _call("paged_tree_new", q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, tree_mask, nh, nkv, scale, max_nodes)
         _call("paged_tree", out, q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, tree_mask, nh, nkv, scale, max_nodes)
         return out
     op = "paged_tree"
