@@ -235,10 +235,14 @@ void paged_selected(at::Tensor out, const at::Tensor& q, const at::Tensor& k, co
   const int64_t least = std::max<int64_t>(1, 256 / at_.page);
   const int64_t splits = std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(1, T * nkv), (count + least - 1) / least, 64}));
   const Parts parts(splits > 1 ? T * nh * splits : 0, at_.hd, q);
-  // more rows than sequences: neighbours that may read their pages together
+  // More rows than sequences, and enough of them to take the launch that makes the unions and still fill the card: neighbours read their
+  // pages together, 16 / heads of a group at a time.  Each by itself / together, us, lists of 64 pages drawn at random, half alike, alike: 128 rows of
+  // 32 heads on 8 of 128 dims 32, 40, 30, 19; 512 103, 91, 67, 41; 256 of 16 on 4 of 256 dims 86, 74, 54, 32, but 128 of them 44, 72, 53, 31;
+  // two at a time, 256 rows of 28 on 4 31, 37, 33, 25; 512 57, 62, 54, 39; 2048 of 8 on one of 64 dims 31, 40, 36, 27.
   at::Tensor plan;
   int* plan_n = nullptr;
-  if (rows && T > tables.size(0) && nh / nkv <= 8) {
+  const int64_t side = 16 * nkv / nh;
+  if (rows && T > tables.size(0) && side >= 2 && T * nkv * std::min<int64_t>(at_.hd, 128) >= (side >= 4 ? 1 : 2) * 131072) {
     const int64_t pairs = T * nkv * count * 2, numbers = T * (nkv + 1);
     plan = at::empty({pairs + (numbers + 1) / 2}, q.options().dtype(at::kLong));
     plan_n = reinterpret_cast<int*>(plan.data_ptr<int64_t>() + pairs);

@@ -849,7 +849,12 @@ void pick_screened(const Args& a, hipStream_t s) {
 extern "C" int dgi_select_pages(const void* q, long long q_stride, const void* bounds, const int* tables, int table_stride, int table_cols,
                                 int n_seqs, int num_blocks, const int* ctx, const int* row_seq, int T, int nh, int nkv, int hd, int page,
                                 int count, int first, int recent, void* keys, int key_stride, int key_rows, int* out, hipStream_t s) {
-  const bool groups = row_seq && T > n_seqs;      // else hardly two rows of one sequence
+  // Rows in groups only if there are more than sequences (else hardly two of one), and where that saves more than the third launch and the
+  // second look at some pages take, about 9 us.  Row by row / in groups, us: 32 rows of 8 heads of 128 over 500 pages 16.8, 18.3, over
+  // 1000 22.9, 21.2; 64 over 100 13.6, 15.5, over 500 22.9, 19.3; 128 over 100 17.2, 15.7, over 1000 53, 30; 64 rows of 4 heads over 500
+  // 17.3, 19.2; 512 rows of one head of 64 over 500 15.8, 18.4, over 1000 21.1, 21.2; 128 rows of 2 heads of 256 over 500 23.9, 24.4.
+  const int span = table_cols - first - recent;
+  const bool groups = row_seq && T > n_seqs && (double)T * nkv * (span + 40) * min(hd, 128) >= 18e6;
   for (int t0 = 0; t0 < T; t0 += key_rows) {
     Args a{(const uint16_t*)q + t0 * q_stride, q_stride, (const uint16_t*)bounds,
            row_seq ? tables : tables + (size_t)t0 * table_stride, table_stride, table_cols, row_seq ? n_seqs : n_seqs - t0, num_blocks,
@@ -862,7 +867,6 @@ extern "C" int dgi_select_pages(const void* q, long long q_stride, const void* b
       else if (hd == 256) rc = scores<256>(a, groups, s);
       if (rc) return rc;
     }
-    const int span = table_cols - first - recent;
     if (!groups || table_cols <= count) {
       if (span <= 4 * kThreads) pick_pages_kernel<4><<<nkv * a.T, kThreads, 0, s>>>(a);
       else pick_pages_kernel<32><<<nkv * a.T, kThreads, 0, s>>>(a);

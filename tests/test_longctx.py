@@ -1086,3 +1086,102 @@ def test_many_rows_past_32_bits():
                      longctx.paged_tree(tree[0], kk, vv, tables[:, :20].contiguous() + at, *tree[4:], 16, nkv, 0.1)))
     for a, b in zip(*outs):
         assert torch.equal(a, b) and (a != 0).any()
+
+
+# ---- the forms for many rows, at the sizes of the tests above -----------------------------------------------------------------------------
+
+@pytest.fixture
+def crowd(monkeypatch):
+    """Behind the rows of every call as many that see nothing as make the kernels take neighbouring rows together."""
+    longctx.load_native(required=True)
+    select, selected, more = longctx.select_pages, longctx.paged_selected, 20000
+
+    def grown(x, value):
+        return torch.cat([x, x.new_full((more, *x.shape[1:]), value)])
+
+    def select_many(q, bounds, tables, ctx, *args, row_seq):
+        assert q.is_cuda
+        return select(grown(q, 1.0), bounds, tables, grown(ctx, 0), *args, row_seq=grown(row_seq, 0))[: q.shape[0]]
+
+    def selected_many(q, k, v, tables, ctx, pages, *args, row_seq, out=None):
+        assert q.is_cuda
+        big = None if out is None else grown(out, 7.0)
+        r = selected(grown(q, 1.0), k, v, tables, grown(ctx, 0), grown(pages, 3), *args, row_seq=grown(row_seq, 0), out=big)
+        assert (r[q.shape[0]:, : args[0] * k.shape[3]] == 0).all()
+        return r[: q.shape[0]] if out is None else out.copy_(r[: q.shape[0]])
+
+    monkeypatch.setattr(longctx, "select_pages", select_many)
+    monkeypatch.setattr(longctx, "paged_selected", selected_many)
+
+
+@gpu
+@pytest.mark.parametrize("rows,page,extra", [(37, 16, 0), (5, 64, 64), (64, 16, 8), (130, 32, 0)])
+def test_crowd_select_rows_of_prompts(crowd, rows, page, extra):
+    test_select_rows_of_prompts("cuda", rows, page, extra)
+
+
+@gpu
+@pytest.mark.parametrize("what", ["alike", "zeros", "close", "huge", "tiny", "no numbers", "a hundred alike", "two of a kind"])
+@pytest.mark.parametrize("hd,pages", [(64, 300), (128, 200), (128, 1300), (256, 250)])
+def test_crowd_select_every_bit(crowd, what, hd, pages):
+    test_select_prompts_that_need_every_bit("cuda", what, hd, pages)
+
+
+@gpu
+@pytest.mark.parametrize("hd,pages", [(64, 200), (256, 1000), (128, 1090), (64, 5000), (128, 8300), (256, 9000)])
+def test_crowd_select_long_prompts(crowd, hd, pages):
+    test_select_rows_of_long_prompts("cuda", hd, pages)
+
+
+@gpu
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 64), (18, 2, 128), (4, 4, 256)])
+def test_crowd_select_beside_single_rows(crowd, nh, nkv, hd):
+    test_select_prompts_beside_single_rows("cuda", nh, nkv, hd)
+
+
+@gpu
+@pytest.mark.parametrize("nh,nkv,hd,page", [(1, 1, 64, 16), (5, 1, 128, 4), (14, 2, 128, 32), (16, 1, 64, 16), (6, 2, 256, 16), (2, 2, 128, 128),
+                                            (3, 1, 64, 1)])
+def test_crowd_selected(crowd, nh, nkv, hd, page):
+    test_selected_prompts("cuda", nh, nkv, hd, page)
+
+
+@gpu
+@pytest.mark.parametrize("nh,count,lens,rows", [(1, 90, [9000], 33), (2, 300, [8000], 9), (8, 150, [3000, 2500], 18)])
+def test_crowd_selected_long_lists(crowd, nh, count, lens, rows):
+    test_selected_prompts_with_long_lists("cuda", nh, count, lens, rows)
+
+
+@gpu
+@pytest.mark.parametrize("test", ["test_selected_prompts_with_lists_in_any_order", "test_selected_prompts_and_pages_of_other_rows",
+                                  "test_selected_prompts_large_scores_and_strides", "test_selected_places_that_nobody_sees"])
+def test_crowd_selected_places(crowd, test):
+    globals()[test]("cuda")
+
+
+@gpu
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 64), (4, 1, 128)])
+def test_crowd_steps_of_a_server(crowd, nh, nkv, hd):
+    test_steps_of_a_server("cuda", nh, nkv, hd)
+
+
+@gpu
+@pytest.mark.parametrize("nh,nkv,hd,T,pages", [(28, 4, 128, 600, 90), (16, 8, 64, 700, 300), (4, 4, 256, 520, 60)])
+def test_many_rows_as_one_by_one(nh, nkv, hd, T, pages):
+    """A long portion beside decode rows: as on the CPU, and in the same step as row by row."""
+    longctx.load_native(required=True)
+    lens = [16 * pages, 16 * pages - 200, 300, 77]
+    q, b, tables, ctx, seq = _select_case(nh, nkv, hd, 16, lens, T)
+    rows = torch.cat([torch.arange(T), torch.arange(2 * T - 40, 2 * T), torch.tensor([3 * T - 1, 4 * T - 1])])
+    q, ctx, seq = q[rows].contiguous(), ctx[rows].clamp(min=1), seq[rows].contiguous()
+    want = longctx.select_pages(q, b, tables, ctx, nh, nkv, 16, 20, 1, 2, row_seq=seq)
+    q, b, tables, ctx, seq = (x.cuda() for x in (q, b, tables, ctx, seq))
+    pages_ = longctx.select_pages(q, b, tables, ctx, nh, nkv, 16, 20, 1, 2, row_seq=seq)
+    assert torch.equal(pages_.cpu(), want)
+    g = _gen(8)
+    k, v = _randn(g, b.shape[0], nkv, 16, hd, dev="cuda"), _randn(g, b.shape[0], nkv, 16, hd, dev="cuda")
+    got = longctx.paged_selected(q, k, v, tables, ctx, pages_, nh, nkv, hd ** -0.5, row_seq=seq)
+    some = torch.randperm(len(rows), generator=g)[:60].tolist() + [T - 1, T, len(rows) - 2, len(rows) - 1]
+    one = [x[some].cpu() for x in (q, ctx, pages_, seq)]
+    want, tol = _selected_want(nh, nkv, hd ** -0.5, one[0], k.cpu(), v.cpu(), tables.cpu(), one[1], one[2], one[3])
+    _close(got[some], want, tol)
