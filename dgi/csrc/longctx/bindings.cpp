@@ -267,12 +267,14 @@ void paged_tree(at::Tensor out, const at::Tensor& q, const at::Tensor& k, const 
   TORCH_CHECK_VALUE(mask.dim() == 2 && mask.size(0) >= S && mask.size(1) >= max_nodes && mask.size(1) <= kInt, op,
                     ": tree_mask must be [sequences, nodes]");
   const c10::DeviceGuard guard(at_.dev);
-  // Columns of 16 pairs a workgroup (tree_rows) or row tiles of 128 (tree_tiles), us at 32 heads on 8: one sequence of 10 / 32 nodes, 600 keys 10, 16 /
-  // 12, 18; of 8000 keys 20, 25 / 25, 28; eight of 2000 keys, 10 / 16 / 24 nodes 25, 25 / 26, 27 / 33, 30; 32 of 4000, 8 / 10 / 16 100, - / 143, 116 /
-  // 148, 122; 64 heads, one of 32 / 64 nodes, 600 keys 12, 20 / 15, 22, but of 8000 38, 34 / 60, 41.
-  const int64_t G = nh / nkv, width = tables.size(1) * at_.page, pairs = max_nodes * G, few = S * nkv * ((pairs + 15) / 16);
-  if (pairs > 32 && at_.hd <= 128 && !(few <= 256 && (pairs <= 128 || width <= 1024))) {
-    const int64_t tiles = (pairs + 127) / 128, least = 4;
+  // Columns of 16 pairs a workgroup (tree_rows) or row tiles of 128 (tree_tiles): by the workgroups of the first and the keys that all of them
+  // read, weighed by how full the tiles would be.  us of both, 32 heads on 8 of 128 dims: one sequence of 32 nodes, 300 keys 11.5, 18.2, 4000
+  // 18.9, 21.1, of 64, 8000 keys 38.5, 35.3; 16 of 16, 1000 22.9, 35.9, 4000 59.9, 61.2; 64 heads: 8 of 16, 1000 22.9, 35.9, 4000 60.5,
+  // 48.1; 32 of 32, 1000 136, 55; 14 heads on 2 of 64 dims: 8 of 64, 1000 15.4, 26.7, 4000 39.2, 34.0.
+  const int64_t G = nh / nkv, width = tables.size(1) * at_.page, pairs = max_nodes * G, cols = (pairs + 15) / 16, tiles = (pairs + 127) / 128;
+  const int64_t few = S * nkv * cols;
+  if (pairs > 32 && at_.hd <= 128 && !(few <= 1024 && few * (width + 100) * cols <= 6400000 * tiles)) {
+    const int64_t least = 4;
     const int64_t shares = std::max<int64_t>(1, std::min<int64_t>(512 / nkv, (S * tiles * ((width + 63) / 64) + least - 1) / least));
     TORCH_CHECK_VALUE(S * tiles * nkv <= kInt, op, ": too many sequences");
     const Parts parts(shares > 1 ? shares * nkv * 2 * 128 : 0, at_.hd, q);
@@ -282,11 +284,10 @@ void paged_tree(at::Tensor out, const at::Tensor& q, const at::Tensor& k, const 
                             parts.o, parts.l, (int)shares, (int)least, (int)nh, (int)nkv, (int)at_.hd, (int)at_.page, (float)scale, cur_stream()), op);
     return;
   }
-  const int64_t cols = 16, tiles = (pairs + cols - 1) / cols;
-  TORCH_CHECK_VALUE(S <= kInt / (nkv * tiles), op, ": too many sequences");
-  const int64_t items = S * tiles * nkv, min_part = 128;
+  TORCH_CHECK_VALUE(S <= kInt / 64 / (nkv * cols), op, ": too many sequences");
+  const int64_t items = few, min_part = 128;
   const int64_t splits = std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(1, items), (width + min_part - 1) / min_part, 64}));
-  const Parts parts(splits > 1 ? items * splits * cols : 0, at_.hd, q);
+  const Parts parts(splits > 1 ? items * splits * 16 : 0, at_.hd, q);
   check_rc(dgi_tree_rows(q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(), tables.data_ptr<int>(), (int)tables.stride(0),
                           (int)tables.size(1), (int)S, (int)k.size(0), (int)q.size(0), cu.data_ptr<int>(), ctx.data_ptr<int>(),
                           mask.data_ptr(), (int)mask.stride(0), (int)max_nodes, out.data_ptr(), out.stride(0),

@@ -75,10 +75,13 @@ __global__ __launch_bounds__(NT) void tree_rows_kernel(Args a) {
   __shared__ int list[kList];      // pages; -1: not in the cache
   __shared__ float ml[NW][2][16];
 
-  const int item = blockIdx.x / a.nkv, h = blockIdx.x - item * a.nkv, split = blockIdx.y;
+  // the column tiles of a (run, sequence, kv head) eight workgroups apart: on one XCD, whose L2 has the keys after the first
+  const int G = a.nh / a.nkv, tiles = (a.max_nodes * G + 15) / 16;
+  const int eight = blockIdx.x / (8 * tiles), tile_at = blockIdx.x - eight * 8 * tiles, unit = eight * 8 + tile_at % 8;
+  if (unit >= a.nkv * a.n_seqs * a.splits) return;
+  const int h = unit % a.nkv, seq = unit / a.nkv % a.n_seqs, split = unit / a.nkv / a.n_seqs, item = seq * tiles + tile_at / 8;
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, qi = lane & 15, g = lane >> 4;
-  const int G = a.nh / a.nkv, bs = 1 << a.bs_log2;
-  const int tiles = (a.max_nodes * G + 15) / 16, seq = item / tiles;
+  const int bs = 1 << a.bs_log2;
   const Runs run = runs_of(a, seq);
   const int pair0 = (item - seq * tiles) * 16;      // (node, head) pairs from here on
   if (pair0 >= run.nodes * G || split >= run.runs) return;
@@ -375,7 +378,8 @@ __global__ __launch_bounds__(256) void tree_rows_runs_kernel(Args a) {
 
 template <int HD>
 int launch(const Args& a, int items, hipStream_t s) {
-  const dim3 grid(a.nkv * items, a.splits);
+  const long long units = (long long)a.nkv * a.n_seqs * a.splits;
+  const unsigned grid = (unsigned)((units + 7) / 8 * 8 * (items / a.n_seqs));
   if (a.bs_log2 >= 4) tree_rows_kernel<HD, true><<<grid, NT, 0, s>>>(a);
   else tree_rows_kernel<HD, false><<<grid, NT, 0, s>>>(a);
   DGI_CHECK_LAUNCH();

@@ -42,42 +42,66 @@ struct Args {
 };
 
 // A sequence: its first row, its nodes, its row tiles, its context, and the steps (tiles of 64 keys, one for an empty context) that each row
-// tile takes.
+// tile counts as: those that it takes, or `pad`.
 struct Seq {
   int q0, nodes, tiles, ctx, steps;
 };
 // kLead more steps go into the deal for each: what it costs to begin and end one (10 us where a step takes 2)
 constexpr int kLead = 4;
-__device__ __forceinline__ Seq sequence(const Args& a, int s) {
+__device__ __forceinline__ Seq sequence(const Args& a, int s, int pad) {
   if (s >= a.n_seqs) return {0, 0, 0, 0, 0};
   const int q0 = a.cu[s], q1 = a.cu[s + 1], ctx = min(max(a.ctx[s], 0), a.table_cols << a.bs_log2);
   const int nodes = q0 < 0 ? 0 : max(0, min(min(q1, a.rows) - q0, a.max_nodes));
-  return {q0, nodes, (nodes * (a.nh / a.nkv) + kRows - 1) / kRows, ctx, kLead + max(1, (ctx + KT - 1) / KT)};
+  return {q0, nodes, (nodes * (a.nh / a.nkv) + kRows - 1) / kRows, ctx, pad ? pad : kLead + max(1, (ctx + KT - 1) / KT)};
 }
 
 // The order of a kv head's steps: row tile 0 of every sequence, row tile 1, ..  One wave counts; `first` is its lane's sequence, of the first
 // 64; results are in all lanes.
-__device__ int steps_before(const Args& a, const Seq& first, int lane, int mt, int seq) {      // sequences before `seq` in row tile mt, all tiles before it
+__device__ int steps_before(const Args& a, const Seq& first, int lane, int mt, int seq, int pad) {      // sequences before `seq` in row tile mt, all tiles before it
   long long sum = 0;
   Seq q = first;
   for (int s0 = 0;;) {
     sum += (long long)q.steps * (min(q.tiles, mt) + (s0 + lane < seq && q.tiles > mt ? 1 : 0));
     if ((s0 += 64) >= a.n_seqs) break;
-    q = sequence(a, s0 + lane);
+    q = sequence(a, s0 + lane, pad);
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
   return (int)min(sum, 0x7fffffffll);
 }
-// steps of a share
-__device__ __forceinline__ int share_of(const Args& a, const Seq& first, int lane) {
-  return max(a.least, (steps_before(a, first, lane, 1 << 20, 0) + a.shares - 1) / a.shares);
+// Steps of a share.  Where whole row tiles, as many for each share, are few steps more than equal shares, each counts as the longest: nothing
+// is cut.  kSlack is what a cut costs, the second beginning and the second launch (12 trees of 43 nodes, 64 heads on 8, 371 keys: 29 us, with cuts
+// 36; 16 of 60 nodes over 300 to 900 keys 46, 58; 64 of 64 over 300 109, 115).
+constexpr int kSlack = 20;
+__device__ int share_of(const Args& a, Seq& first, int lane, int& pad) {
+  pad = 0;
+  long long sum = 0;
+  int tiles = 0, longest = 0;
+  Seq q = first;
+  for (int s0 = 0;;) {
+    sum += (long long)q.steps * q.tiles;
+    tiles += q.tiles;
+    if (q.tiles > 0) longest = max(longest, q.steps);
+    if ((s0 += 64) >= a.n_seqs) break;
+    q = sequence(a, s0 + lane, 0);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    sum += __shfl_xor(sum, o, 64);
+    tiles += __shfl_xor(tiles, o, 64);
+    longest = max(longest, __shfl_xor(longest, o, 64));
+  }
+  const int len = max(a.least, ((int)min(sum, 0x7fffffffll) + a.shares - 1) / a.shares);
+  const long long whole = (long long)((tiles + a.shares - 1) / a.shares) * longest;
+  if (tiles == 0 || whole > len + kSlack) return len;
+  pad = first.steps = longest;
+  return (int)whole;
 }
 // whose step `at` is; row tile -1: behind the last one
 struct Place {
   int mt, seq, step;
 };
-__device__ Place place_of(const Args& a, const Seq& first, int lane, int at) {
+__device__ Place place_of(const Args& a, const Seq& first, int lane, int at, int pad) {
   for (int mt = 0, before = 0;; ++mt) {
     int any = 0;
     Seq q = first;
@@ -99,7 +123,7 @@ __device__ Place place_of(const Args& a, const Seq& first, int lane, int at) {
       before += all;
       any += all;
       if ((s0 += 64) >= a.n_seqs) break;
-      q = sequence(a, s0 + lane);
+      q = sequence(a, s0 + lane, pad);
     }
     if (!any) return {-1, 0, 0};
   }
@@ -108,7 +132,7 @@ __device__ Place place_of(const Args& a, const Seq& first, int lane, int at) {
 template <int HD>
 __global__ __launch_bounds__(kWaves * 64, 2) void tree_tiles_kernel(Args a) {
   __shared__ __attribute__((aligned(16))) uint16_t lds[2 * KT * 2 * HD];
-  __shared__ int s_place[4];
+  __shared__ int s_place[5];
   __shared__ unsigned s_odd[kWaves];
   const int G = a.nh / a.nkv, nkv = a.nkv, bs = 1 << a.bs_log2;
   // kv heads side by side: with eight of them each has an XCD's L2 to itself
@@ -116,29 +140,32 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_tiles_kernel(Args a) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   if (w == 0) {
-    const Seq first = sequence(a, lane);
-    const int len = share_of(a, first, lane);
-    const Place p = (long long)share * len > 0x7fffffff ? Place{-1, 0, 0} : place_of(a, first, lane, share * len);
+    Seq first = sequence(a, lane, 0);
+    int pad;
+    const int len = share_of(a, first, lane, pad);
+    const Place p = (long long)share * len > 0x7fffffff ? Place{-1, 0, 0} : place_of(a, first, lane, share * len, pad);
     if (lane == 0) {
       s_place[0] = p.mt;
       s_place[1] = p.seq;
       s_place[2] = p.step;
       s_place[3] = len;
+      s_place[4] = pad;
     }
   }
   __syncthreads();
   int mt = __builtin_amdgcn_readfirstlane(s_place[0]), seq = __builtin_amdgcn_readfirstlane(s_place[1]);
   int step0 = __builtin_amdgcn_readfirstlane(s_place[2]), left = __builtin_amdgcn_readfirstlane(s_place[3]);
+  const int pad = __builtin_amdgcn_readfirstlane(s_place[4]);
   if (mt < 0) return;
   const int most = (a.max_nodes * G + kRows - 1) / kRows;
   for (; left > 0; step0 = 0) {      // a sequence's row tile, or the part of it that is the share's
-  Seq sq = sequence(a, seq);
+  Seq sq = sequence(a, seq, pad);
   while (sq.tiles <= mt) {
     if (++seq >= a.n_seqs) {
       seq = 0;
       if (++mt >= most) return;
     }
-    sq = sequence(a, seq);
+    sq = sequence(a, seq, pad);
   }
   const int q0 = sq.q0, nodes = sq.nodes, ctx = sq.ctx, dealt = min(sq.steps - step0, left);
   left -= dealt;
@@ -437,29 +464,31 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_tiles_kernel(Args a) {
   }
 }
 
-// The parts of a sequence's row tile that several shares have, weighed by their sums: HD / 8 lanes a row, kTurns rows one after
-// another, four parts under way (16 trees of 60 nodes, 64 heads on 8, 1000 to 8000 keys, all launches: 175 us; one row and eight parts: 182).
-constexpr int kTurns = 2;
-template <int HD>
+// The parts of a sequence's row tile that several shares have, weighed by their sums: HD / 8 lanes a row, several parts under way.  Two rows
+// one after another (16 trees of 60 nodes, 64 heads on 8, 1000 to 8000 keys, all launches: 175 us; one row and eight parts at a time: 182), or,
+// where a row has eight parts and more, four groups of lanes a row, a quarter of its parts each (one tree of 64 nodes, 32 heads on 8, 8000 keys: 33 us,
+// not 43; but 6 of 49 over 290, with five parts, 34, not 25).
+template <int HD, int WAYS>
 __global__ __launch_bounds__(256) void tree_parts_kernel(Args a) {
-  constexpr int L = HD / 8, R = 256 / L;
+  constexpr int L = HD / 8, R = 256 / L / WAYS, TURNS = WAYS == 1 ? 2 : 1;
   const int G = a.nh / a.nkv, most = (a.max_nodes * G + kRows - 1) / kRows;
   const int unit = blockIdx.x / a.nkv, kvh = blockIdx.x - unit * a.nkv, seq = unit / most, mt = unit - seq * most;
-  const int lane = threadIdx.x & 63;
-  const Seq first = sequence(a, lane), sq = sequence(a, seq);
+  const int lane = threadIdx.x & 63, way = threadIdx.x / L % WAYS;
+  Seq first = sequence(a, lane, 0);
+  int pad;
+  const int len = share_of(a, first, lane, pad);
+  const Seq sq = sequence(a, seq, pad);
   if (sq.tiles <= mt) return;
-  const int len = share_of(a, first, lane);
-  const int from = steps_before(a, first, lane, mt, seq), to = from + sq.steps - 1, s0 = (from + kLead) / len, s1 = to / len;
+  const int from = steps_before(a, first, lane, mt, seq, pad), to = from + sq.steps - 1, s0 = (from + kLead) / len, s1 = to / len;
   if (s0 == s1) return;
-  for (int turn = 0; turn < kTurns; ++turn) {
-    const int in_tile = (kTurns * blockIdx.y + turn) * R + threadIdx.x / L, r = mt * kRows + in_tile, node = r / G, d = threadIdx.x % L * 8;
+  for (int turn = 0; turn < TURNS; ++turn) {
+    const int in_tile = (TURNS * blockIdx.y + turn) * R + threadIdx.x / (L * WAYS), r = mt * kRows + in_tile, node = r / G, d = threadIdx.x % L * 8;
     if (node >= sq.nodes) break;
     // the first part is one that its share begins, the others are not
     auto at = [&](int s) { return ((size_t)(s * a.nkv + kvh) * 2 + (s == s0)) * kRows + in_tile; };
-    // several parts under way at a time
     constexpr int U = 4;
     float M = -__builtin_inff(), W = 0.f, acc[8] = {};
-    for (int s = s0; s <= s1; s += U) {
+    for (int s = s0 + way * U; s <= s1; s += U * WAYS) {
       float l[U], m = M;
       f32x4 x[U], y[U];
 #pragma unroll
@@ -492,6 +521,22 @@ __global__ __launch_bounds__(256) void tree_parts_kernel(Args a) {
         }
       }
     }
+    if constexpr (WAYS > 1) {
+#pragma unroll
+      for (int o = L; o < L * WAYS; o <<= 1) {
+        const float other = __shfl_xor(M, o, 64), m = fmaxf(M, other);
+        const float mine = M == -__builtin_inff() ? 0.f : exp2f(M - m), theirs = other == -__builtin_inff() ? 0.f : exp2f(other - m);
+        const float w = __shfl_xor(W, o, 64);
+        W = W * mine + w * theirs;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float x = __shfl_xor(acc[j], o, 64);
+          acc[j] = (mine == 0.f ? 0.f : acc[j] * mine) + (theirs == 0.f ? 0.f : x * theirs);
+        }
+        M = m;
+      }
+      if (way > 0) continue;
+    }
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[j] = W == 0.f ? 0.f : acc[j] / W;
     *reinterpret_cast<u32x4*>(a.out + (size_t)(sq.q0 + node) * a.out_stride + (kvh * G + r - node * G) * HD + d) = pack8(acc);
@@ -504,7 +549,9 @@ int launch(const Args& a, hipStream_t s) {
   DGI_CHECK_LAUNCH();
   if (a.shares > 1) {
     const int most = (a.max_nodes * (a.nh / a.nkv) + kRows - 1) / kRows;
-    tree_parts_kernel<HD><<<dim3(a.n_seqs * most * a.nkv, kRows * HD / 8 / 256 / kTurns), 256, 0, s>>>(a);
+    const int units = a.n_seqs * most * a.nkv, groups = kRows * HD / 8 / 256;
+    if (a.shares < 8 * a.n_seqs * most) tree_parts_kernel<HD, 1><<<dim3(units, groups / 2), 256, 0, s>>>(a);
+    else tree_parts_kernel<HD, 4><<<dim3(units, groups * 4), 256, 0, s>>>(a);
     DGI_CHECK_LAUNCH();
   }
   return 0;

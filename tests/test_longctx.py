@@ -1185,3 +1185,84 @@ def test_many_rows_as_one_by_one(nh, nkv, hd, T, pages):
     one = [x[some].cpu() for x in (q, ctx, pages_, seq)]
     want, tol = _selected_want(nh, nkv, hd ** -0.5, one[0], k.cpu(), v.cpu(), tables.cpu(), one[1], one[2], one[3])
     _close(got[some], want, tol)
+
+
+@pytest.fixture
+def woods(monkeypatch):
+    """Before and behind the sequences of every call as many without nodes as make the kernels take a sequence's pairs as tiles."""
+    longctx.load_native(required=True)
+    tree, more = longctx.paged_tree, 600
+
+    def many(q, k, v, tables, cu, ctx, mask, nh, nkv, scale, max_nodes=64, out=None):
+        assert q.is_cuda and k.shape[3] <= 128
+        S = ctx.numel()
+        around = lambda x, value: torch.cat([x.new_full((more, *x.shape[1:]), value), x, x.new_full((more, *x.shape[1:]), value)])
+        cu = torch.cat([cu[:1].expand(more), cu, cu[-1:].expand(more)])
+        max_nodes = max_nodes if max_nodes * (nh // nkv) > 32 else min(64, mask.shape[1])
+        return tree(q, k, v, around(tables[:S], -1), cu, around(ctx, 33), around(mask[:S], -1), nh, nkv, scale, max_nodes=max_nodes, out=out)
+
+    monkeypatch.setattr(longctx, "paged_tree", many)
+
+
+@gpu
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 64), (7, 1, 128), (16, 1, 64), (8, 1, 128), (2, 2, 128)])
+@pytest.mark.parametrize("nodes", [[1], [5, 9, 2], [64, 33]])
+def test_woods(woods, nh, nkv, hd, nodes):
+    test_tree("cuda", nh, nkv, hd, nodes)
+
+
+@gpu
+@pytest.mark.parametrize("nh,nkv,hd,nodes", [(32, 2, 64, [64, 7, 64]), (16, 1, 128, [40, 64]), (3, 1, 64, [64, 64])])
+@pytest.mark.parametrize("page", [4, 16, 256])
+def test_woods_many_nodes(woods, nh, nkv, hd, nodes, page):
+    test_tree_many_nodes("cuda", nh, nkv, hd, nodes, page)
+
+
+@gpu
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 64), (8, 1, 128), (2, 2, 64)])
+def test_woods_keys_that_a_row_does_not_see(woods, nh, nkv, hd):
+    test_tree_keys_that_a_row_does_not_see("cuda", nh, nkv, hd)
+
+
+@gpu
+@pytest.mark.parametrize("page", [8, 16, 32, 128])
+def test_woods_pages(woods, page):
+    test_tree_pages("cuda", page)
+
+
+@gpu
+@pytest.mark.parametrize("scale", [-0.25, 1e-30, 4.0])
+def test_woods_scales(woods, scale):
+    test_tree_scales("cuda", 32, 2, 64, scale)
+
+
+@gpu
+@pytest.mark.parametrize("test,args", [("test_tree_long_contexts", ()), ("test_tree_empty_sequences_and_rows_behind", ()), ("test_tree_unknown_pages", ()),
+                                       ("test_tree_scores_without_a_scale", (32, 2)), ("test_tree_scores_without_a_scale", (8, 2)),
+                                       ("test_tree_rows_without_keys", (32, 2)), ("test_tree_rows_without_keys", (4, 2))])
+def test_woods_places(woods, test, args):
+    globals()[test]("cuda", *args)
+
+
+@gpu
+@pytest.mark.parametrize("nh,nkv,hd,nodes,ctx", [(32, 8, 128, [64], [9000]), (64, 8, 128, [60, 33, 64, 50] * 3, [900, 300, 2000, 64] * 3),
+                                                 (16, 1, 128, [64, 64], [20000, 64]), (64, 8, 64, [30] * 40, [1000] * 40)])
+def test_trees_in_shares(nh, nkv, hd, nodes, ctx):
+    """Whole row tiles, cut ones, and many parts of one: rows in random places against 64 bits."""
+    longctx.load_native(required=True)
+    g = _gen(11)
+    case = _tree_case(nh, nkv, hd, 16, ctx, nodes)
+    got = longctx.paged_tree(*(x.cuda() for x in case), nh, nkv, 0.1)
+    q, k, v, tables, cu, ctx, mask = case
+    for s in torch.randperm(len(nodes), generator=g)[:4].tolist():
+        n, c = nodes[s], int(ctx[s])
+        ids = tables[s, : -(-c // 16)].long()
+        for a in {0, n - 1, int(torch.randint(0, n, (1,), generator=g))}:
+            see = (torch.arange(c) < c - n) | torch.tensor([bool(int(mask[s, a]) >> max(j - c + n, 0) & 1) and j >= c - n for j in range(c)])
+            row = int(cu[s]) + a
+            for h in range(nkv):
+                kk, vv = k[ids, h].reshape(-1, hd)[:c][see], v[ids, h].reshape(-1, hd)[:c][see]
+                heads = slice(h * nh // nkv, (h + 1) * nh // nkv)
+                want, tol = _attention(q[row, : nh * hd].view(nh, hd)[heads], kk, vv, 0.1)
+                _close(got[row].view(nh, hd)[heads], want, tol, f"sequence {s} node {a} head {h}")
+
