@@ -106,26 +106,28 @@ __global__ __launch_bounds__(kThreads) void page_scores_kernel(Args a) {
   const int t = blockIdx.x / a.nkv, h = blockIdx.x - t * a.nkv;
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, l = lane % LP, p0 = lane / LP;
   if (GROUPS && together(begins_of(a, t, lane))) return;
-  const int n = pages_of(a, t);
-  const int begin = a.first + blockIdx.y * a.row_chunk, end = min(begin + a.row_chunk, n - a.recent);
-  if (n <= a.count || begin >= end) return;
-  const int G = a.nh / a.nkv;
-  __shared__ double wgt_s[2 * HD];      // of lo, of hi
+  // the first ids beside the context
   const int seq = a.row_seq ? a.row_seq[t] : t;
   const bool known = seq >= 0 && seq < a.n_seqs;
   const int* table = a.tables + (size_t)(known ? seq : 0) * a.table_stride;
+  const int begin = a.first + blockIdx.y * a.row_chunk;
+  int base = begin + w * PW, id = known && base + p0 < a.table_cols ? table[base + p0] : -1;
+  int id_next = known && base + STEP + p0 < a.table_cols ? table[base + STEP + p0] : -1;
+  const int n = pages_of(a, t), end = min(begin + a.row_chunk, n - a.recent);
+  if (n <= a.count || begin >= end) return;
+  const int G = a.nh / a.nkv;
+  __shared__ double wgt_s[2 * HD];      // of lo, of hi
   u64* keys = a.keys + ((size_t)t * a.nkv + h) * a.key_stride;
-  auto id_of = [&](int base) {
-    const int p = base + p0, id = known && p < end ? table[p] : -1;
-    return id >= 0 && id < a.num_blocks ? id : -1;
-  };
+  auto valid = [&](int base, int id) { return base + p0 < end && id >= 0 && id < a.num_blocks ? id : -1; };
+  auto id_of = [&](int base) { return valid(base, known && base + p0 < end ? table[base + p0] : -1); };
   u32x4 v[2][4];
   auto load = [&](u32x4* to, int id) {
     const uint16_t* bp = a.bounds + ((size_t)max(id, 0) * a.nkv + h) * 2 * HD + l * 8;
 #pragma unroll
     for (int i = 0; i < 4; ++i) to[i] = *reinterpret_cast<const u32x4*>(bp + LP * i * 8);
   };
-  int base = begin + w * PW, id = id_of(base), id_next = id_of(base + STEP);
+  id = valid(base, id);
+  id_next = valid(base + STEP, id_next);
   load(v[0], id);
   weigh<kThreads>(wgt_s, a.q + t * a.q_stride + h * G * HD, HD, G);
   __syncthreads();
@@ -332,7 +334,8 @@ __global__ __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) void page_screen_kerne
 }
 
 // A workgroup per (row, kv head).  The threshold is found by digits of 8 bits within the window that still holds it, the first one
-// cut from the range of the keys; then the kept pages are written in order.  R > 0: a thread has R of the keys in registers.
+// cut from the range of the keys; then the kept pages are written in order.  A thread has R of the keys in registers, the first two of
+// them from `ahead`.
 struct Long {
   u64 lo[kWaves], hi[kWaves];
   int hist[256];
@@ -393,14 +396,14 @@ __device__ __forceinline__ void write_kept(const u64* kept, int begin, int* out,
 }
 
 template <int R>
-__device__ __forceinline__ void pick(const u64* keys, int begin, int end, int need, int* out, Shared& sh) {
+__device__ __forceinline__ void pick(const u64* keys, const u64* ahead, int begin, int end, int need, int* out, Shared& sh) {
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
   u64 k[R];
   u64 lo = ~0ull, hi = 0;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const int i = begin + r * kThreads + tid;
-    k[r] = i < end ? keys[i] : 0;
+    k[r] = i < end ? r < 2 ? ahead[r] : keys[i] : 0;
     if (i < end) {
       lo = min(lo, k[r]);
       hi = max(hi, k[r]);
@@ -791,27 +794,32 @@ __global__ __launch_bounds__(kThreads) void pick_screened_kernel(Args a) {
 // MOST: keys of a thread in registers at most (their number is the kernel's registers, and so how many workgroups share a compute unit).
 template <int MOST>
 __global__ __launch_bounds__(kThreads) void pick_pages_kernel(Args a) {
-  const int t = blockIdx.x / a.nkv, h = blockIdx.x - t * a.nkv, tid = threadIdx.x;
-  const int n = pages_of(a, t);
+  const int t = blockIdx.x / a.nkv, h = blockIdx.x - t * a.nkv, tid = threadIdx.x, begin = a.first;
+  const u64* keys = a.keys + ((size_t)t * a.nkv + h) * a.key_stride;
+  u64 ahead[2];      // read beside the context; there are keys only if a table may have more pages than are kept
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int i = begin + r * kThreads + tid;
+    ahead[r] = a.table_cols > a.count && i < a.table_cols ? keys[i] : 0;
+  }
+  const int n = pages_of(a, t), end = n - a.recent;
   int* out = a.out + ((size_t)t * a.nkv + h) * a.count;
   if (n <= a.count) {
     for (int i = tid; i < a.count; i += kThreads) out[i] = i < n ? i : -1;
     return;
   }
-  const u64* keys = a.keys + ((size_t)t * a.nkv + h) * a.key_stride;
-  const int begin = a.first, end = n - a.recent;
   const int need = a.count - a.first - a.recent;
   for (int i = tid; i < a.first; i += kThreads) out[i] = i;
   for (int i = tid; i < a.recent; i += kThreads) out[a.count - a.recent + i] = end + i;
   if (need == 0) return;
   out += a.first;
   __shared__ __attribute__((aligned(16))) Shared sh;
-  if (end - begin <= 2 * kThreads) return pick<2>(keys, begin, end, need, out, sh);
-  if (end - begin <= 4 * kThreads) return pick<4>(keys, begin, end, need, out, sh);
+  if (end - begin <= 2 * kThreads) return pick<2>(keys, ahead, begin, end, need, out, sh);
+  if (end - begin <= 4 * kThreads) return pick<4>(keys, ahead, begin, end, need, out, sh);
   if constexpr (MOST > 4) {
-    if (end - begin <= 8 * kThreads) return pick<8>(keys, begin, end, need, out, sh);
-    if (end - begin <= 16 * kThreads) return pick<16>(keys, begin, end, need, out, sh);
-    if (end - begin <= 32 * kThreads) return pick<32>(keys, begin, end, need, out, sh);
+    if (end - begin <= 8 * kThreads) return pick<8>(keys, ahead, begin, end, need, out, sh);
+    if (end - begin <= 16 * kThreads) return pick<16>(keys, ahead, begin, end, need, out, sh);
+    if (end - begin <= 32 * kThreads) return pick<32>(keys, ahead, begin, end, need, out, sh);
   }
   pick_long<kWaves>(keys, begin, end, need, out, sh.any);
 }
