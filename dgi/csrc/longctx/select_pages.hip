@@ -13,7 +13,7 @@
 //
 // Rows of a prompt share their sequence's bounds: 16 of them are the rows of bf16 matrix instructions, which give each score in 32 bits and
 // a bound for its error; pages that the error leaves open are scored in 64 bits (1018 rows of 28 heads over 730 to 1000 pages of 4 kv heads
-// of 128: 55 us, of which scores 31, those of rows that do not go together 4, the choice 21; with the products in 64 bits on the matrix
+// of 128: 55 us, of which scores 31, looking for rows that do not go together 4, the choice 21; with the products in 64 bits on the matrix
 // cores, whose rate alone is 24 us, 88 us).  What bounds this is latency: of the weights ahead of 4 steps of 64 pages, and of the choice.
 #include "../common.h"
 
@@ -98,25 +98,21 @@ __device__ __forceinline__ unsigned begins_of(const Args& a, int t, int lane) {
   return begins_of(a, t, lane, seq);
 }
 
-// Row by row.  Four 16-byte chunks of a page's [lo | hi] a lane, HD / 16 lanes a page; the next pages' bounds are under way
-// while these are multiplied.  GROUPS: not the rows that page_screen_kernel takes, and scores with a bound for the error as it has them.
+// A row's pages from `begin` on, `pages` of them.  Four 16-byte chunks of a page's [lo | hi] a lane, HD / 16 lanes a page; the next pages'
+// bounds are under way while these are multiplied.  GROUPS: scores rounded to 32 bits, as page_screen_kernel leaves them.
 template <int HD, bool GROUPS>
-__global__ __launch_bounds__(kThreads) void page_scores_kernel(Args a) {
+__device__ __forceinline__ void score_pages(const Args& a, double* wgt_s, int t, int h, int begin, int pages) {
   constexpr int LP = HD / 16, PW = 64 / LP, STEP = kWaves * PW;      // lanes a page, pages a wave and a workgroup at a time
-  const int t = blockIdx.x / a.nkv, h = blockIdx.x - t * a.nkv;
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, l = lane % LP, p0 = lane / LP;
-  if (GROUPS && together(begins_of(a, t, lane))) return;
   // the first ids beside the context
   const int seq = a.row_seq ? a.row_seq[t] : t;
   const bool known = seq >= 0 && seq < a.n_seqs;
   const int* table = a.tables + (size_t)(known ? seq : 0) * a.table_stride;
-  const int begin = a.first + blockIdx.y * a.row_chunk;
   int base = begin + w * PW, id = known && base + p0 < a.table_cols ? table[base + p0] : -1;
   int id_next = known && base + STEP + p0 < a.table_cols ? table[base + STEP + p0] : -1;
-  const int n = pages_of(a, t), end = min(begin + a.row_chunk, n - a.recent);
+  const int n = pages_of(a, t), end = min(begin + pages, n - a.recent);
   if (n <= a.count || begin >= end) return;
   const int G = a.nh / a.nkv;
-  __shared__ double wgt_s[2 * HD];      // of lo, of hi
   u64* keys = a.keys + ((size_t)t * a.nkv + h) * a.key_stride;
   auto valid = [&](int base, int id) { return base + p0 < end && id >= 0 && id < a.num_blocks ? id : -1; };
   auto id_of = [&](int base) { return valid(base, known && base + p0 < end ? table[base + p0] : -1); };
@@ -137,7 +133,6 @@ __global__ __launch_bounds__(kThreads) void page_scores_kernel(Args a) {
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 8; ++j) wgt[i][j] = wgt_s[(l + LP * i) * 8 + j];
-  float largest = 0.f;
   auto score = [&](const u32x4* x4, int base, int id) {
     double sum[4] = {};
 #pragma unroll
@@ -152,14 +147,11 @@ __global__ __launch_bounds__(kThreads) void page_scores_kernel(Args a) {
     for (int o = 1; o < LP; o <<= 1) s += __shfl_xor(s, o, 64);
     if (l != 0 || base + p0 >= end) return;
     if constexpr (GROUPS) {
-      const float x = id < 0 ? -__builtin_inff() : fabs(s) <= 0x1p126 ? (float)s : __builtin_nanf("");
-      if (id >= 0) largest = fmaxf(largest, fabsf(x));
-      reinterpret_cast<float*>(keys)[base + p0] = x;
+      reinterpret_cast<float*>(keys)[base + p0] = id < 0 ? -__builtin_inff() : fabs(s) <= 0x1p126 ? (float)s : __builtin_nanf("");
     } else {
       keys[base + p0] = key_of(id >= 0 ? s : -__builtin_inf());
     }
   };
-  const int begin_w = base;
   for (; base < end; base += 2 * STEP) {
     int id2 = id_of(base + 2 * STEP);
     load(v[1], id_next);
@@ -171,10 +163,54 @@ __global__ __launch_bounds__(kThreads) void page_scores_kernel(Args a) {
     score(v[1], base + STEP, id_next);
     id_next = id2;
   }
-  if constexpr (GROUPS) {
+}
+
+// Row by row.
+template <int HD>
+__global__ __launch_bounds__(kThreads) void page_scores_kernel(Args a) {
+  __shared__ double wgt_s[2 * HD];      // of lo, of hi
+  const int t = blockIdx.x / a.nkv;
+  score_pages<HD, false>(a, wgt_s, t, blockIdx.x - t * a.nkv, a.first + blockIdx.y * a.row_chunk, a.row_chunk);
+}
+
+// The rows that page_screen_kernel does not take.  Which groups of 16 these are each workgroup finds out by itself, 256 groups at a time, and
+// takes every gridDim-th of their (group, pages, row, head); pages of a unit are such that there are some 2048 units.  (A workgroup for every
+// row and head, most of which end at once: 4.6 us where there is no such row, and 24 for 12 rows over 1000 pages beside 500 of a prompt,
+// which take 4.7 and 15.)
+template <int HD>
+__global__ __launch_bounds__(kThreads) void page_scores_alone_kernel(Args a) {
+  __shared__ double wgt_s[2 * HD];
+  __shared__ u64 alone_s[kWaves];
+  const int tid = threadIdx.x, groups = (a.T + kRows - 1) / kRows, span = a.table_cols - a.first - a.recent;
+  for (int g0 = 0; g0 < groups; g0 += kThreads) {
+    const int row0 = (g0 + tid) * kRows;
+    int runs = row0 < a.T, seqs[kRows];      // as begins_of has them
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor(largest, o, 64));
-    if (lane == 0 && begin_w < end) reinterpret_cast<float*>(keys)[a.key_stride + blockIdx.y * kWaves + w] = largest * 0x1p-23f + kLeast;
+    for (int i = 0; i < kRows; ++i) seqs[i] = row0 + i < a.T ? a.row_seq[row0 + i] : 0;
+#pragma unroll
+    for (int i = 1; i < kRows; ++i) runs += row0 + i < a.T ? seqs[i] != seqs[i - 1] : row0 + i == a.T;
+    const u64 mine = __ballot(runs > kRuns);
+    __syncthreads();
+    if ((tid & 63) == 0) alone_s[tid >> 6] = mine;
+    __syncthreads();
+    int n = 0;
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) n += __popcll(alone_s[v]);
+    const int each = min(max((int)(((long long)n * kRows * a.nkv * span / 2048 + 31) / 32 * 32), 128), 1024), chunks = (span + each - 1) / each;
+    for (long long unit = blockIdx.x; unit < (long long)n * chunks * kRows * a.nkv; unit += gridDim.x) {
+      const int h = unit % a.nkv, row = unit / a.nkv % kRows;
+      const long long place = unit / a.nkv / kRows;
+      int rank = place / chunks, v = 0;
+      u64 word = alone_s[0];
+      while (rank >= __popcll(word)) {
+        rank -= __popcll(word);
+        word = alone_s[++v];
+      }
+      for (; rank > 0; --rank) word &= word - 1;
+      const int t = (g0 + 64 * v + __ffsll(word) - 1) * kRows + row;
+      __syncthreads();      // the unit before has read its weights
+      if (t < a.T) score_pages<HD, true>(a, wgt_s, t, h, a.first + (int)(place % chunks) * each, each);
+    }
   }
 }
 
@@ -664,16 +700,20 @@ __global__ __launch_bounds__(kThreads) void pick_screened_kernel(Args a) {
       }
     }
   };
-  // errors are those of chunks of pages, 16 or 1024 / hd of them a wave at a time
-  const int chunk = tiles ? a.chunk : a.row_chunk, width = tiles ? 16 : 1024 / a.hd;
+  // errors are those of chunks of pages, 16 of them a wave at a time, or of a rounding
   float E = 0.f;
-  for (int i = tid; (i / kWaves) * chunk + width * (i % kWaves) < end - begin; i += N)
-    if (width * (i % kWaves) < chunk) E = fmaxf(E, i == tid ? E_first : scores[a.key_stride + i]);
+  if (tiles)
+    for (int i = tid; (i / kWaves) * a.chunk + 16 * (i % kWaves) < end - begin; i += N) E = fmaxf(E, i == tid ? E_first : scores[a.key_stride + i]);
   unsigned lo = ~0u, hi = 0;
   each([&](int, unsigned x) {
     lo = min(lo, x ? x : ~0u);
     hi = max(hi, x);
   });
+  if (!tiles)
+    each([&](int, unsigned x) {
+      const float size = fabsf(float_of(x));
+      if (x && size <= 0x1p126f) E = fmaxf(E, size * 0x1p-23f + kLeast);
+    });
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
     lo = min(lo, (unsigned)__shfl_xor((int)lo, o, 64));
@@ -831,17 +871,17 @@ int scores(Args& a, bool groups, hipStream_t s) {
   auto chunk = [&](long long items, int unit, int want, int most) {
     return (int)min(max((items * span / want + unit - 1) / unit * unit, (long long)unit), (long long)most);
   };
-  a.row_chunk = chunk((long long)a.nkv * a.T, 32, 2048, 1024);
-  const dim3 grid(a.nkv * a.T, (span + a.row_chunk - 1) / a.row_chunk);
   if (!groups) {
-    page_scores_kernel<HD, false><<<grid, kThreads, 0, s>>>(a);
+    a.row_chunk = chunk((long long)a.nkv * a.T, 32, 2048, 1024);
+    const dim3 grid(a.nkv * a.T, (span + a.row_chunk - 1) / a.row_chunk);
+    page_scores_kernel<HD><<<grid, kThreads, 0, s>>>(a);
     DGI_CHECK_LAUNCH();
     return 0;
   }
   a.chunk = chunk(tiles, 64, 1024, 1 << 20);
   page_screen_kernel<HD><<<dim3(tiles, (span + a.chunk - 1) / a.chunk), kThreads, 0, s>>>(a);
   DGI_CHECK_LAUNCH();
-  page_scores_kernel<HD, true><<<grid, kThreads, 0, s>>>(a);
+  page_scores_alone_kernel<HD><<<512, kThreads, 0, s>>>(a);
   DGI_CHECK_LAUNCH();
   return 0;
 }

@@ -1266,3 +1266,18 @@ def test_trees_in_shares(nh, nkv, hd, nodes, ctx):
                 want, tol = _attention(q[row, : nh * hd].view(nh, hd)[heads], kk, vv, 0.1)
                 _close(got[row].view(nh, hd)[heads], want, tol, f"sequence {s} node {a} head {h}")
 
+
+@gpu
+@pytest.mark.parametrize("nkv,hd", [(1, 64), (3, 128)])
+def test_select_rows_in_turn(nkv, hd):
+    """Thousands of rows whose sequences take turns, a long portion among them, and more: groups that go together and groups that do not."""
+    longctx.load_native(required=True)
+    g = _gen(21)
+    lens = torch.randint(600, 1000, (30,), generator=g).tolist()
+    q, b, tables, _, _ = _select_case(2 * nkv, nkv, hd, 16, lens, 1)
+    seq = torch.cat([torch.arange(300) % 30, torch.full((700,), 3), torch.arange(3500) % 29, torch.arange(64) // 4, torch.full((437,), 7)]).to(I32)
+    ctx = (torch.tensor(lens)[seq.long()] - torch.randint(0, 300, (len(seq),), generator=g)).to(I32)
+    q = _randn(g, len(seq), 2 * nkv * hd)
+    want = longctx.select_pages(q, b, tables, ctx, 2 * nkv, nkv, 16, 20, 1, 2, row_seq=seq)
+    got = longctx.select_pages(*(x.cuda() for x in (q, b, tables, ctx)), 2 * nkv, nkv, 16, 20, 1, 2, row_seq=seq.cuda())
+    assert torch.equal(got.cpu(), want)
