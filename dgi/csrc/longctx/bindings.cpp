@@ -116,7 +116,8 @@ void rope_cache_bounds(at::Tensor q_out, const at::Tensor& qkv, const at::Tensor
   const int64_t T = qkv.size(0);
   check_int(positions, dev, at::kInt, op, "positions");
   check_int(slots, dev, at::kInt, op, "slot_mapping");
-  TORCH_CHECK_VALUE(positions.numel() == T && slots.numel() == T && T <= (1 << 29), op, ": positions and slot_mapping must have a number for each row");
+  TORCH_CHECK_VALUE(positions.numel() == T && slots.numel() == T && T <= (1 << 29), op,
+                    ": positions and slot_mapping must have a number for each row");
   TORCH_CHECK_VALUE(cos_sin.is_cuda() && cos_sin.device() == dev && cos_sin.scalar_type() == at::kFloat && cos_sin.is_contiguous() &&
                         cos_sin.dim() == 2 && cos_sin.size(0) > 0 && cos_sin.size(0) <= kInt && aligned(cos_sin),
                     op, ": cos_sin must be contiguous fp32 [positions, rotated dims]");
@@ -176,7 +177,8 @@ void select_pages(at::Tensor out, const at::Tensor& q, const at::Tensor& bounds,
   const at::Tensor keys = at::empty({stride > count ? at_once * nkv * stride : 0}, q.options().dtype(at::kLong));
   check_rc(dgi_select_pages(q.data_ptr(), q.stride(0), bounds.data_ptr(), tables.data_ptr<int>(), (int)tables.stride(0), (int)tables.size(1),
                             (int)tables.size(0), (int)bounds.size(0), ctx.data_ptr<int>(), rows, (int)T, (int)nh, (int)nkv, (int)hd,
-                            (int)page, (int)count, (int)first, (int)recent, keys.data_ptr(), (int)stride, (int)at_once, out.data_ptr<int>(), cur_stream()), op);
+                            (int)page, (int)count, (int)first, (int)recent, keys.data_ptr(), (int)stride, (int)at_once, out.data_ptr<int>(),
+                            cur_stream()), op);
 }
 
 struct Attention {
@@ -236,8 +238,8 @@ void paged_selected(at::Tensor out, const at::Tensor& q, const at::Tensor& k, co
   const int64_t splits = std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(1, T * nkv), (count + least - 1) / least, 64}));
   const Parts parts(splits > 1 ? T * nh * splits : 0, at_.hd, q);
   // More rows than sequences, and enough of them to take the launch that makes the unions and still fill the card: neighbours read their
-  // pages together, 16 / heads of a group at a time.  Each by itself / together, us, lists of 64 pages drawn at random, half alike, alike: 128 rows of
-  // 32 heads on 8 of 128 dims 32, 40, 30, 19; 512 103, 91, 67, 41; 256 of 16 on 4 of 256 dims 86, 74, 54, 32, but 128 of them 44, 72, 53, 31;
+  // pages together, 16 / heads of a group at a time.  Each by itself / together, us, lists of 64 pages drawn at random, half alike, alike:
+  // 128 rows of 32 heads on 8 of 128 dims 32, 40, 30, 19; 512 103, 91, 67, 41; 256 of 16 on 4 of 256 dims 86, 74, 54, 32, but 128 of them 44, 72, 53, 31;
   // two at a time, 256 rows of 28 on 4 31, 37, 33, 25; 512 57, 62, 54, 39; 2048 of 8 on one of 64 dims 31, 40, 36, 27.
   at::Tensor plan;
   int* plan_n = nullptr;
@@ -250,7 +252,8 @@ void paged_selected(at::Tensor out, const at::Tensor& q, const at::Tensor& k, co
   check_rc(dgi_paged_selected(q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(), tables.data_ptr<int>(), (int)tables.stride(0),
                               (int)tables.size(1), (int)tables.size(0), (int)k.size(0), ctx.data_ptr<int>(), rows, pages.data_ptr<int>(),
                               (int)count, out.data_ptr(), out.stride(0), parts.o, parts.l, (int)splits,
-                              plan_n ? plan.data_ptr() : nullptr, plan_n, plan_n ? plan_n + T * nkv : nullptr, (int)T, (int)nh, (int)nkv, (int)at_.hd, (int)at_.page, (float)scale, cur_stream()), op);
+                              plan_n ? plan.data_ptr() : nullptr, plan_n, plan_n ? plan_n + T * nkv : nullptr, (int)T, (int)nh, (int)nkv,
+                              (int)at_.hd, (int)at_.page, (float)scale, cur_stream()), op);
 }
 
 void paged_tree(at::Tensor out, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& tables,
@@ -261,7 +264,8 @@ void paged_tree(at::Tensor out, const at::Tensor& q, const at::Tensor& k, const 
   check_int(ctx, at_.dev, at::kInt, op, "context_lens");
   const int64_t S = ctx.numel();
   check_int(cu, at_.dev, at::kInt, op, "cu_seqlens_q");
-  TORCH_CHECK_VALUE(cu.numel() == S + 1 && tables.size(0) >= S, op, ": cu_seqlens_q must have one number more than context_lens, block_tables as many rows");
+  TORCH_CHECK_VALUE(cu.numel() == S + 1 && tables.size(0) >= S, op,
+                    ": cu_seqlens_q must have one number more than context_lens, block_tables as many rows");
   check_int(mask, at_.dev, at::kLong, op, "tree_mask");
   TORCH_CHECK_VALUE(max_nodes >= 1 && max_nodes <= 64, op, ": trees of 1 to 64 nodes");
   TORCH_CHECK_VALUE(mask.dim() == 2 && mask.size(0) >= S && mask.size(1) >= max_nodes && mask.size(1) <= kInt, op,
@@ -281,7 +285,8 @@ void paged_tree(at::Tensor out, const at::Tensor& q, const at::Tensor& k, const 
     check_rc(dgi_tree_tiles(q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(), tables.data_ptr<int>(), (int)tables.stride(0),
                             (int)tables.size(1), (int)S, (int)k.size(0), (int)q.size(0), cu.data_ptr<int>(), ctx.data_ptr<int>(),
                             mask.data_ptr(), (int)mask.stride(0), (int)max_nodes, out.data_ptr(), out.stride(0),
-                            parts.o, parts.l, (int)shares, (int)least, (int)nh, (int)nkv, (int)at_.hd, (int)at_.page, (float)scale, cur_stream()), op);
+                            parts.o, parts.l, (int)shares, (int)least, (int)nh, (int)nkv, (int)at_.hd, (int)at_.page, (float)scale,
+                            cur_stream()), op);
     return;
   }
   TORCH_CHECK_VALUE(S <= kInt / 64 / (nkv * cols), op, ": too many sequences");
@@ -291,7 +296,8 @@ void paged_tree(at::Tensor out, const at::Tensor& q, const at::Tensor& k, const 
   check_rc(dgi_tree_rows(q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(), tables.data_ptr<int>(), (int)tables.stride(0),
                           (int)tables.size(1), (int)S, (int)k.size(0), (int)q.size(0), cu.data_ptr<int>(), ctx.data_ptr<int>(),
                           mask.data_ptr(), (int)mask.stride(0), (int)max_nodes, out.data_ptr(), out.stride(0),
-                          parts.o, parts.l, (int)splits, (int)min_part, (int)nh, (int)nkv, (int)at_.hd, (int)at_.page, (float)scale, cur_stream()), op);
+                          parts.o, parts.l, (int)splits, (int)min_part, (int)nh, (int)nkv, (int)at_.hd, (int)at_.page, (float)scale,
+                          cur_stream()), op);
 }
 
 // The same with an output of the call's own: allocated here, a microsecond of the host's time that the smallest calls feel is half of what it

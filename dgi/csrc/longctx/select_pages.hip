@@ -627,7 +627,8 @@ __device__ __forceinline__ u64 score_of(const Args& a, const double* wgt, const 
 
 // From scores that are off by an error E at most.  With the threshold of these scores in [lo, hi], that of the true ones is in
 // [lo - E, hi + E]: pages above hi + 2 E are kept, those below lo - 2 E are not, and those between (1 to 8 of 1000 where
-// bounds are normal) are scored again in 64 bits and take the places that are left.  Where there are too many of them, or scores without a bound, all are.
+// bounds are normal) are scored again in 64 bits and take the places that are left.  Where there are too many of them, or
+// scores without a bound, all are.
 // W waves a row: one for up to 1024 pages (1018 rows over 730 to 1000 pages of 4 heads: 21 us, by all four of a workgroup 45), four for
 // more.  A wave has turns * 64 pages in a row, R > 0: R of them at most a lane, in registers; 0: they are read anew each time.
 template <int R, int W>
@@ -647,7 +648,8 @@ __global__ __launch_bounds__(kThreads) void pick_screened_kernel(Args a) {
   typedef Screened<R, W> S;
   extern __shared__ __attribute__((aligned(16))) double wgt_s[];      // 2 hd a row: of lo, of hi
   __shared__ __attribute__((aligned(16))) S teams[kWaves / W];
-  const int team = __builtin_amdgcn_readfirstlane(threadIdx.x / N), tid = threadIdx.x % N, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int team = __builtin_amdgcn_readfirstlane(threadIdx.x / N), tid = threadIdx.x % N;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int item = blockIdx.x * (kWaves / W) + team, t = item / a.nkv, h = item - t * a.nkv, G = a.nh / a.nkv;
   if (t >= a.T) return;
   S& s = teams[team];

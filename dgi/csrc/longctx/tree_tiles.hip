@@ -10,9 +10,9 @@
 // another, are dealt out in equal shares, so that a long context beside short ones does not hold up the launch; what a share's ends
 // cut is added up by a second launch.
 //
-// 16 trees of 60 nodes, 64 heads on 8, 1000 to 8000 keys: 175 us, 632 TF/s of 111 Gflop (with workgroups by sequence and
-// run of its keys instead of equal shares, 260).  A tile takes 2.0 us for the two workgroups of a compute unit, 1070 TF/s; the rest is the beginning and end of the two
-// parts that a share has (20 us) and the second launch (10 us).
+// 16 trees of 60 nodes, 64 heads on 8, 1000 to 8000 keys: 175 us, 632 TF/s of 111 Gflop (with workgroups by sequence and run of
+// its keys instead of equal shares, 260).  A tile takes 2.0 us for the two workgroups of a compute unit, 1070 TF/s; the rest is the
+// beginning and end of the two parts that a share has (20 us) and the second launch (10 us).
 #include "../prefill_attention_kernel.h"
 
 using namespace dgi;
@@ -57,7 +57,8 @@ __device__ __forceinline__ Seq sequence(const Args& a, int s, int pad) {
 
 // The order of a kv head's steps: row tile 0 of every sequence, row tile 1, ..  One wave counts; `first` is its lane's sequence, of the first
 // 64; results are in all lanes.
-__device__ int steps_before(const Args& a, const Seq& first, int lane, int mt, int seq, int pad) {      // sequences before `seq` in row tile mt, all tiles before it
+// (sequences before `seq` in row tile mt, all tiles before it)
+__device__ int steps_before(const Args& a, const Seq& first, int lane, int mt, int seq, int pad) {
   long long sum = 0;
   Seq q = first;
   for (int s0 = 0;;) {
