@@ -196,7 +196,7 @@ __global__ __launch_bounds__(kThreads) void page_scores_alone_kernel(Args a) {
     int n = 0;
 #pragma unroll
     for (int v = 0; v < kWaves; ++v) n += __popcll(alone_s[v]);
-    const int each = min(max((int)(((long long)n * kRows * a.nkv * span / 2048 + 31) / 32 * 32), 128), 1024), chunks = (span + each - 1) / each;
+    const int each = (int)min(max(((long long)n * kRows * a.nkv * span / 2048 + 31) / 32 * 32, 128ll), 1024ll), chunks = (span + each - 1) / each;
     for (long long unit = blockIdx.x; unit < (long long)n * chunks * kRows * a.nkv; unit += gridDim.x) {
       const int h = unit % a.nkv, row = unit / a.nkv % kRows;
       const long long place = unit / a.nkv / kRows;
