@@ -204,6 +204,13 @@ Attention check_attention(const at::Tensor& out, const at::Tensor& q, const at::
   return {hd, page, dev};
 }
 
+// Runs of `keys` for each of `units` workgroups, at most `most`: as many as give the card two workgroups a compute unit, but no more than
+// 16, or 512 keys each, and 8 for `some` units and more: each is a part to be read again (8 rows of heads, 8192 keys: 16 runs 13.9 us, 32 15.0; 16,
+// 8 runs 18.4, 32 22.2; trees of 4 nodes over 8000 keys, 8 heads: 16 runs 15.9, 62 22.6).
+int64_t runs_of(int64_t units, int64_t keys, int64_t most, int64_t some) {
+  return std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(1, units), most, units >= some ? 8 : std::max<int64_t>(16, keys / 512), 64}));
+}
+
 // What the parts of a split sum leave: a row of hd values each, and its logarithm.  Both in one tensor: allocating takes the host a
 // microsecond, which a call of one row feels.
 struct Parts {
@@ -233,9 +240,12 @@ void paged_selected(at::Tensor out, const at::Tensor& q, const at::Tensor& k, co
   const int64_t count = pages.size(2);
   TORCH_CHECK_VALUE(T <= kInt / nkv - 16, op, ": too many rows");
   const c10::DeviceGuard guard(at_.dev);
-  // runs of 256 keys at the least, as many as give the card two workgroups a compute unit
-  const int64_t least = std::max<int64_t>(1, 256 / at_.page);
-  const int64_t splits = std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(1, T * nkv), (count + least - 1) / least, 64}));
+  // Runs of 256 keys at the least, as many as give the card two workgroups a compute unit, where that is worth a second launch.  One run /
+  // these, us, of 128 dims: 8 (row, head) pairs of 512 keys 8.6, 9.7, of 768 10.2, 9.8 (but one launch for the host), of 1024 11.7, 9.6, of 8192 58, 15; 64 of
+  // 1024 12.6, 11.7, of 8192 73, 49; 96 of 1024 13.3, 16.5, of 4096 35.5, 39.3, of 8192 109, 86; 128 of 2048 25, 29.7, of 8192 125, 109; 192 160, 170.
+  const int64_t least = std::max<int64_t>(1, 256 / at_.page), keys = count * at_.page, units = T * nkv;
+  const bool one = keys < 1024 || (units > 64 && keys < 8192) || units > 160;
+  const int64_t splits = one ? 1 : runs_of(units, keys, (count + least - 1) / least, 16);
   const Parts parts(splits > 1 ? T * nh * splits : 0, at_.hd, q);
   // More rows than sequences, and enough of them to take the launch that makes the unions and still fill the card: neighbours read their
   // pages together, 16 / heads of a group at a time.  Each by itself / together, us, lists of 64 pages drawn at random, half alike, alike:
@@ -290,8 +300,11 @@ void paged_tree(at::Tensor out, const at::Tensor& q, const at::Tensor& k, const 
     return;
   }
   TORCH_CHECK_VALUE(S <= kInt / 64 / (nkv * cols), op, ": too many sequences");
+  // One run / several, us, 32 heads on 8 of 128 dims: a tree of 4 nodes, 300 keys 10.6, 11.2, 600 13.0, 11.4; 4 of 24 nodes, 300 11.1, 14.2, 1000
+  // 17.5, 19.0; 16 of 4, 300 10.6, 12.7, 1000 17.7, 21.8; 8 of 8, 2000 26.3, 22.9; 16 of 8, 1000 18.5, 23.6, 4000 46, 52.
   const int64_t items = few, min_part = 128;
-  const int64_t splits = std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(1, items), (width + min_part - 1) / min_part, 64}));
+  const bool one = width <= 400 || (items >= 64 && width <= 10 * items) || items >= 224;
+  const int64_t splits = one ? 1 : runs_of(items, width, (width + min_part - 1) / min_part, 32);
   const Parts parts(splits > 1 ? items * splits * 16 : 0, at_.hd, q);
   check_rc(dgi_tree_rows(q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(), tables.data_ptr<int>(), (int)tables.stride(0),
                           (int)tables.size(1), (int)S, (int)k.size(0), (int)q.size(0), cu.data_ptr<int>(), ctx.data_ptr<int>(),
