@@ -78,10 +78,11 @@ __device__ __forceinline__ int rows_from(const Args& a, int t, int most, int lan
 
 // What the workgroups of rows that go together read: the union of their lists, ascending, or, where a row names a page twice (it counts
 // twice) or the bits do not fit, one list after another.  A workgroup per (first row, kv head).
-__global__ __launch_bounds__(NT) void selected_plan_kernel(Args a) {
-  __shared__ unsigned bits[kBits];        // [rows][words] the pages that a row selected
-  __shared__ int before[kBits / 2];       // [words] pages of any row in the words before
-  __shared__ int s_n[NW];
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void selected_plan_kernel(Args a, int n_bits) {
+  extern __shared__ unsigned bits[];                     // [rows][words] the pages that a row selected
+  int* before = reinterpret_cast<int*>(bits + n_bits);   // [words] pages of any row in the words before
+  __shared__ int s_n[THREADS / 64];
   const int G = a.nh / a.nkv, side = 16 / G, groups = (a.rows + side - 1) / side;
   // the first rows of all groups, the second ones, ..: most of the others have nothing to do, and would leave every other XCD without work
   const int unit = blockIdx.x / a.nkv, h = blockIdx.x - unit * a.nkv, place = unit / groups, t0 = (unit - place * groups) * side + place;
@@ -104,19 +105,19 @@ __global__ __launch_bounds__(NT) void selected_plan_kernel(Args a) {
   };
   auto fits = [&](int p) { return p >= 0 && p < a.table_cols && ((long long)p << a.bs_log2) < most; };
   const int words = min((int)(((long long)most + (32ll << a.bs_log2) - 1) >> (a.bs_log2 + 5)), (a.table_cols + 31) >> 5), all = m * a.count;
-  bool together = m > 1 && m * words <= kBits;
+  bool together = m > 1 && m * words <= n_bits;
   if (together) {
-    for (int i = tid; i < m * words; i += NT) bits[i] = 0;
+    for (int i = tid; i < m * words; i += THREADS) bits[i] = 0;
     __syncthreads();
     bool twice = false;
-    for (int i = tid; i < all; i += NT) {
+    for (int i = tid; i < all; i += THREADS) {
       const int p = entry(i);
       if (fits(p)) twice = twice || (atomicOr(&bits[i / a.count * words + (p >> 5)], 1u << (p & 31)) >> (p & 31) & 1);
     }
     together = !__syncthreads_or(twice);
   }
   if (!together) {
-    for (int i = tid; i < all; i += NT) {
+    for (int i = tid; i < all; i += THREADS) {
       const int p = entry(i), id = fits(p) ? table[p] : -1;
       const bool there = id >= 0 && id < a.num_blocks;
       list[i] = int4{there ? id : 0, there ? p << a.bs_log2 : 0, there ? 1 << (i / a.count) : 0, 0};
@@ -124,7 +125,7 @@ __global__ __launch_bounds__(NT) void selected_plan_kernel(Args a) {
     if (tid == 0) a.plan_total[t0 * a.nkv + h] = all;
     return;
   }
-  const int per = (words + NT - 1) / NT, first = min(tid * per, words), last = min(first + per, words);
+  const int per = (words + THREADS - 1) / THREADS, first = min(tid * per, words), last = min(first + per, words);
   int n = 0;
   for (int i = first; i < last; ++i) {
     unsigned u = 0;
@@ -142,10 +143,10 @@ __global__ __launch_bounds__(NT) void selected_plan_kernel(Args a) {
   __syncthreads();
   int from = sum - n;
   for (int v = 0; v < w; ++v) from += s_n[v];
-  if (tid == NT - 1) a.plan_total[t0 * a.nkv + h] = from + n;
+  if (tid == THREADS - 1) a.plan_total[t0 * a.nkv + h] = from + n;
   for (int i = first; i < last; ++i) before[i] += from;
   __syncthreads();
-  for (int i = tid; i < all; i += NT) {      // the first row that has a page writes it
+  for (int i = tid; i < all; i += THREADS) {      // the first row that has a page writes it
     const int p = entry(i), r = i / a.count, word = p >> 5;
     if (!fits(p)) continue;
     unsigned who = 0, u = 0;
@@ -496,7 +497,10 @@ template <int HD>
 int launch(const Args& a, hipStream_t s) {
   if (a.plan) {
     const int side = 16 / (a.nh / a.nkv), rows = (a.rows + side - 1) / side * side;
-    selected_plan_kernel<<<a.nkv * rows, NT, 0, s>>>(a);
+    const int words = (a.table_cols + 31) / 32, n_bits = (int)min((long long)side * words, (long long)kBits), lds = (n_bits + min(words, kBits / 2)) * 4;
+    // a wave for lists that it has in a few turns: all of them at once (2 x 509 rows of 64 pages, 4 heads: 7.3 us, four waves 9.5)
+    if ((long long)side * a.count <= 1024) selected_plan_kernel<64><<<a.nkv * rows, 64, lds, s>>>(a, n_bits);
+    else selected_plan_kernel<NT><<<a.nkv * rows, NT, lds, s>>>(a, n_bits);
     DGI_CHECK_LAUNCH();
     const dim3 grid(a.nkv * rows, a.splits);
     if (a.bs_log2 >= 4) selected_kernel<HD, true, true><<<grid, NT, 0, s>>>(a);
