@@ -5,9 +5,10 @@
 // nothing, so they are exact whatever the order, and a page's bounds can go on from step to step.  A value that is no number makes its
 // channel's bounds no number (minimum / maximum of IEEE 754-2019).
 //
-// Bound by bytes: the append reads a row's q | k | v once and writes it once (4115 rows of 64 heads on 8 of 128, 172 MB: 41 us, 4.2 TB/s;
+// Bound by bytes: the append reads a row's q | k | v once and writes it once (4115 rows of 64 heads on 8 of 128, 172 MB: 43.7 us, 3.9 TB/s;
 // one row: 3.7 us, a launch), the rebuilding reads the keys once (16384 pages of 16 keys, 8 heads of 128, 604 MB: 131 us, 4.6 TB/s).
 #include "../common.h"
+#include "page_runs.h"
 
 using namespace dgi;
 
@@ -75,9 +76,9 @@ __device__ __forceinline__ void turn(const Task& x, u32x4& a, u32x4& b) {
 
 // The first T workgroups are for the keys, the others for queries and values of a row.
 //
-// A row that is the first of the step in its page takes the keys of all rows that follow it there (rows of rising slots, side by
-// side: a page of them at most) and the page's bounds, so that every page has one writer; its waves take a row each in turn, the same task of a
-// row each lane, and are joined in LDS.  The workgroups of the rows behind it end at once.
+// A row that is the first of the step in its page takes the keys of all rows of the page (page_runs.h) and its bounds, so that
+// every page has one writer; its waves take a row each in turn, the same task of a row each lane, and are joined in LDS.  The workgroups of
+// the rows behind it end at once.
 //
 // A lane has the same task of every head that it takes, and so one read of the angles.
 __global__ __launch_bounds__(kThreads) void rope_cache_bounds_kernel(
@@ -88,7 +89,7 @@ __global__ __launch_bounds__(kThreads) void rope_cache_bounds_kernel(
   const bool keys = blockIdx.x < T;
   const int t = keys ? blockIdx.x : blockIdx.x - T, tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
   const int tasks = tasks_of(hd, rd, mode), slot = slots[t];
-  const bool cached = slot >= 0 && slot < n_slots;
+  const bool cached = has_slot(slot, n_slots);
   const int blk = cached ? slot / block_size : 0, off = cached ? slot - blk * block_size : 0;
   auto angles_at = [&](int row) { return cos_sin + (size_t)min(max(positions[row], 0), max_pos - 1) * rd; };
 
@@ -117,17 +118,10 @@ __global__ __launch_bounds__(kThreads) void rope_cache_bounds_kernel(
     return;
   }
 
-  if (!cached || (off > 0 && t > 0 && slots[t - 1] == slot - 1)) return;
-  int run = 0;      // rows of the page from here on
-  for (bool on = true; on; run += 64) {
-    const int r = run + lane;
-    const bool in = off + r < block_size && t + r < T && slots[min(t + r, T - 1)] == slot + r;
-    const unsigned long long out = ~__ballot(in);
-    if (out) {
-      run += __ffsll(out) - 1 - 64;
-      on = false;
-    }
-  }
+  if (!cached) return;
+  auto ballot = [&](auto f) { return (unsigned long long)__ballot(f(lane)); };
+  if (!begins_page(ballot, slots, n_slots, block_size, t, slot - off)) return;
+  const PageRows run = page_rows(ballot, slots, n_slots, block_size, T, t, slot - off);
   __shared__ __attribute__((aligned(16))) u32x4 part[4][kWaves][64];
   for (int base = 0; base < nkv * tasks; base += 64) {
     const int it = base + lane;
@@ -142,11 +136,13 @@ __global__ __launch_bounds__(kThreads) void rope_cache_bounds_kernel(
     }
     if (live)
 #pragma unroll 2
-      for (int r = w; r < run; r += kWaves) {
+      for (int r = w; r < run.rows; r += kWaves) {
         const uint16_t* kp = qkv + (t + r) * ld + (nh + h) * hd;
-        uint16_t* op = k_cache + (((size_t)blk * nkv + h) * block_size + off + r) * hd;
+        const int at = run.plain ? slot + r : slots[t + r];
         u32x4 a = *reinterpret_cast<const u32x4*>(kp + x.at), b = *reinterpret_cast<const u32x4*>(kp + max(x.other, 0));
         angles(x, angles_at(t + r), rd, mode);
+        if (!run.plain && !has_slot(at, n_slots)) continue;
+        uint16_t* op = k_cache + (((size_t)blk * nkv + h) * block_size + (at - (slot - off))) * hd;
         turn(x, a, b);
         float v[8];      // what attention will read
         *reinterpret_cast<u32x4*>(op + x.at) = a;

@@ -132,7 +132,8 @@ def rope_cache_bounds(qkv, positions, cos_sin, nh: int, nkv: int, hd: int, slot_
 
     A page's bounds start anew with its slot 0 and go on otherwise; they never shrink, so keys that are overwritten or given up (rejected
     drafts) leave them wider than need be, never too narrow.  Rows of one page lie side by side, by rising slots, each slot once, as the
-    steps of ``ModelRunner`` lay them out.  Rows with a slot outside the cache (-1) are rotated and not cached."""
+    steps of ``ModelRunner`` lay them out; slots may be left out.  Rows with a slot outside the cache (-1) are rotated and not cached, wherever
+    they lie."""
     if _native(qkv):
         if out is None:
             return _call("rope_cache_bounds_new", qkv, positions, cos_sin, nh, nkv, hd, slot_mapping, k_cache, v_cache, bounds, mode)

@@ -6,7 +6,11 @@ Tolerances count roundings.  A bf16 result is off by at most 2^-8 of itself; att
 2^-8 of A = sum p |v| / sum p on top; a score is a sum of hd products in fp32, off by at most d = (hd + 4) 2^-24 scale max |q| . |k|, which puts
 2 d on each weight and its sum; exp2 and the sums over n keys take (n + 16) 2^-24 of A.
 """
+import ctypes
 import math
+import os
+import random
+import subprocess
 
 import pytest
 import torch
@@ -134,6 +138,74 @@ def test_append_strided_rows_and_rows_without_a_slot(dev):
     case = _append_case(dev, 8, 2, 64, 64, 0, 16, [(3, 20)])
     case[0] = case[0].repeat_interleave(2, 0)[::2]      # every other row of a buffer
     _append_check(dev, 8, 2, 64, 0, 16, case)
+
+
+PAGE_RUNS = r"""
+#include "page_runs.h"
+template <class F> unsigned long long ballot(F f) {
+  unsigned long long b = 0;
+  for (int lane = 0; lane < 64; ++lane) b |= (unsigned long long)(bool)f(lane) << lane;
+  return b;
+}
+extern "C" void runs(const int* slots, int T, long long n_slots, int page, int* out) {
+  auto b = [](auto f) { return ballot(f); };
+  for (int t = 0; t < T; ++t) {
+    const int page0 = slots[t] / page * page;
+    out[t] = 0;
+    if (!dgi::has_slot(slots[t], n_slots) || !dgi::begins_page(b, slots, n_slots, page, t, page0)) continue;
+    const dgi::PageRows r = dgi::page_rows(b, slots, n_slots, page, T, t, page0);
+    out[t] = r.plain ? r.rows : -r.rows;
+  }
+}
+"""
+
+
+def test_append_a_page_has_one_writer(tmp_path):
+    """Which rows write a page's bounds, and what rows they look at, as the kernel finds it, on the CPU: rows without a slot and slots that are left
+    out between a page's rows make no second writer."""
+    src, lib = tmp_path / "runs.cpp", tmp_path / "runs.so"
+    src.write_text(PAGE_RUNS)
+    folder = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "dgi", "csrc", "longctx")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", "-I", folder, str(src), "-o", str(lib)], check=True)
+    runs = ctypes.CDLL(str(lib)).runs
+    rng = random.Random(5)
+    for case in range(600):
+        page, n_pages = rng.choice([1, 5, 16, 64, 256]), rng.choice([3, 40])
+        drop, hole = rng.choice([0, 0.1, 0.6]), rng.choice([0, 0.1, 0.9])
+        slots = [-1] * rng.choice([0, 0, 70, 200])
+        for at in rng.sample(range(n_pages), rng.randint(1, min(n_pages, 12))):
+            for off in range(rng.randrange(page), rng.randint(1, page)):
+                if rng.random() >= drop:
+                    slots += [rng.choice([-1, -(1 << 31), page * n_pages, (1 << 31) - 1])] * (rng.random() < hole) * rng.choice([1, 1, 1, 65])
+                    slots.append(at * page + off)
+        slots += [-1] * rng.choice([0, 0, 63, 64, 65, 130])
+        T = len(slots)
+        out = (ctypes.c_int * T)()
+        runs((ctypes.c_int * T)(*slots), T, ctypes.c_longlong(page * n_pages), page, out)
+        have = [s // page if 0 <= s < page * n_pages else -1 for s in slots]
+        first, last = {}, {}
+        for t, p in enumerate(have):
+            if p >= 0:
+                first.setdefault(p, t)
+                last[p] = t
+        want = [0] * T
+        for p, t in first.items():
+            want[t] = (last[p] - t + 1) * (1 if slots[t:last[p] + 1] == list(range(slots[t], slots[t] + last[p] + 1 - t)) else -1)
+        assert list(out) == want, (case, page, slots)
+        for p, t in first.items():      # the rows that it looks at have no other page's
+            assert {x for x in have[t:t + abs(want[t])] if x >= 0} == {p}
+
+
+@pytest.mark.parametrize("page", [16, 32])
+def test_append_rows_without_a_slot_within_a_page(dev, page):
+    """Every second row of a portion is not cached, slots are left out, and as many rows as a wave has lie between two of a page."""
+    case = _append_case(dev, 8, 2, 64, 64, 0, page, [(3, 3 * page), (page, 100), (1, 2)])
+    case[3][1: 3 * page: 2] = -1
+    case[3][3 * page + 1: 3 * page + 99] = -1
+    _append_check(dev, 8, 2, 64, 0, page, case)
+    rows = [0, 1, 4, 5, 9, page - 4, page, 2 * page + 3, 3 * page + 1]
+    qkv, pos, cs, slots, k, v, bounds = _append_case(dev, 8, 2, 64, 64, 0, page, [(3, 4 * page)], seed=1)
+    _append_check(dev, 8, 2, 64, 0, page, [qkv[rows], pos[rows], cs, slots[rows], k, v, bounds])
 
 
 def test_append_no_rows_one_row_many_rows(dev):
