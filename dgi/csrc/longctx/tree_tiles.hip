@@ -294,10 +294,11 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_tiles_kernel(Args a) {
       each<0, 2 * NP>([&](auto l) __attribute__((always_inline)) { load(l, 1 - stage); });
     } else if (kb0 + KT < kv_end) load_part(kb0 + KT, 1 - stage, id);
     id = read_id(kb0 + 2 * KT);
-    // Values of the tree's keys that are infinite or no numbers reach the rows that see them alone, but zero times such a value is no
-    // number: they are taken out of the tile here and added below where the weight is not zero.
+    // Values of the tree's keys that are infinite or no numbers reach the rows that see them alone, and those that stand for keys that are
+    // not there reach none, but zero times such a value is no number: they are taken out of the tile here and added below where the weight
+    // is not zero.
     unsigned long long odd = 0;
-    if (kb0 + KT > tree_key) {
+    if (kb0 + KT > tree_key || bad) {
       // a wave looks at the rows that it staged; row r of the tile is bit r
       uint16_t* vt = lds + stage * KT * 2 * HD + KT * HD + row0 * HD;
       unsigned mine = 0;

@@ -745,6 +745,41 @@ def test_tree_unknown_pages(dev):
     _close(got, want, tol)
 
 
+def _without(case, gone):
+    """The same trees over tables whose pages ``gone`` (sequence, place) are not there, and what they see: 64 bits and tolerances."""
+    nh, nkv, scale, q, k, v, tables, cu, ctx, mask = case
+    page, hd, G = k.shape[2], k.shape[3], nh // nkv
+    o, tol = torch.zeros(q.shape[0], nh, hd, dtype=F64), torch.zeros(q.shape[0], nh, hd, dtype=F64)
+    for s in range(len(cu) - 1):
+        n, c = int(cu[s + 1] - cu[s]), int(ctx[s])
+        ids = tables[s, : -(-c // page)].long()
+        for a in range(n):
+            see = torch.tensor([(s, j // page) not in gone and (j < c - n or bool(int(mask[s, a]) >> (j - c + n) & 1)) for j in range(c)], dtype=torch.bool)
+            row = int(cu[s]) + a
+            for h in range(nkv):
+                kk, vv = k[ids, h].reshape(-1, hd)[:c][see], v[ids, h].reshape(-1, hd)[:c][see]
+                heads = slice(h * G, (h + 1) * G)
+                o[row, heads], tol[row, heads] = _attention(q[row, : nh * hd].view(nkv, G, hd)[h], kk, vv, scale)
+    return o.view(q.shape[0], -1), tol.view(q.shape[0], -1)
+
+
+@pytest.mark.parametrize("nh,nkv,hd,page", [(8, 2, 64, 16), (16, 1, 128, 16), (8, 2, 64, 4), (8, 2, 64, 128)])
+def test_tree_pages_that_are_not_there(dev, nh, nkv, hd, page):
+    """Ids outside the cache before the tree, among its own keys, at the end and everywhere, where page 0, which is nobody's, holds no numbers."""
+    q, k, v, tables, cu, ctx, mask = _tree_case(nh, nkv, hd, page, [700, 200, 260, 150], [40, 33, 9, 12])
+    nobody = torch.full_like(k[:1], math.nan), torch.full_like(v[:1], math.inf)
+    nobody[1][:, :, ::2] = math.nan
+    k, v, tables = torch.cat([nobody[0], k]), torch.cat([nobody[1], v]), tables + (tables >= 0)
+    last = [-(-c // page) - 1 for c in ctx.tolist()]
+    gone = {(0, 1), (0, last[0] // 2), (1, 0), (1, last[1]), (2, last[2] - 1)} | {(3, p) for p in range(last[3] + 1)}
+    want, tol = _without((nh, nkv, 0.125, q, k, v, tables, cu, ctx, mask), gone)
+    for i, (s, p) in enumerate(sorted(gone)):
+        tables[s, p] = (-1, k.shape[0], 1 << 30, -(1 << 31))[i % 4]
+    got = longctx.paged_tree(*(x.to(dev) for x in (q, k, v, tables, cu, ctx, mask)), nh, nkv, 0.125)
+    _close(got, want, tol)
+    assert (got[82:] == 0).all()
+
+
 @pytest.mark.parametrize("nh,nkv,hd", [(32, 8, 128), (16, 1, 64), (8, 8, 64), (5, 1, 128), (16, 4, 256)])
 def test_tree_many_sequences(dev, nh, nkv, hd):
     """More trees than a wave has lanes, of none to 20 nodes, contexts of nothing but the tree to some pages: both ways to split the work, with
@@ -1314,6 +1349,12 @@ def test_woods_scales(woods, scale):
                                        ("test_tree_rows_without_keys", (32, 2)), ("test_tree_rows_without_keys", (4, 2))])
 def test_woods_places(woods, test, args):
     globals()[test]("cuda", *args)
+
+
+@gpu
+@pytest.mark.parametrize("nh,nkv,hd,page", [(8, 2, 64, 16), (16, 1, 128, 16), (8, 2, 64, 4), (8, 2, 64, 128)])
+def test_woods_pages_that_are_not_there(woods, nh, nkv, hd, page):
+    test_tree_pages_that_are_not_there("cuda", nh, nkv, hd, page)
 
 
 @gpu
