@@ -462,6 +462,7 @@ __global__ __launch_bounds__(256) void selected_runs_kernel(Args a) {
   f32x4 acc = {0, 0, 0, 0};
   for (int s = 0; s < a.splits; s += U) {
     float l[U], top = M;
+    bool any = false;
     f32x4 x[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -473,8 +474,9 @@ __global__ __launch_bounds__(256) void selected_runs_kernel(Args a) {
     for (int u = 0; u < U; ++u) {
       if (s + u >= a.splits) l[u] = -__builtin_inff();
       top = fmaxf(top, l[u]);
+      any = any || l[u] != -__builtin_inff();      // a sum that is no number is not of the maximum, and stays
     }
-    if (top == -__builtin_inff()) continue;
+    if (!any) continue;
     const float old = __builtin_amdgcn_exp2f(M - top);
     M = top;
     W *= old;
@@ -483,7 +485,7 @@ __global__ __launch_bounds__(256) void selected_runs_kernel(Args a) {
     for (int u = 0; u < U; ++u) {
       const float wgt = __builtin_amdgcn_exp2f(l[u] - M);
       W += wgt;
-      if (wgt != 0.f) acc += wgt * x[u];
+      if (l[u] != -__builtin_inff()) acc += wgt * x[u];
     }
   }
   if (W != 0.f) acc /= W;

@@ -492,6 +492,7 @@ __global__ __launch_bounds__(256) void tree_parts_kernel(Args a) {
     float M = -__builtin_inff(), W = 0.f, acc[8] = {};
     for (int s = s0 + way * U; s <= s1; s += U * WAYS) {
       float l[U], m = M;
+      bool any = false;
       f32x4 x[U], y[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -504,8 +505,9 @@ __global__ __launch_bounds__(256) void tree_parts_kernel(Args a) {
       for (int u = 0; u < U; ++u) {
         if (s + u > s1) l[u] = -__builtin_inff();
         m = fmaxf(m, l[u]);
+        any = any || l[u] != -__builtin_inff();      // a sum that is no number is not of the maximum, and stays
       }
-      if (m == -__builtin_inff()) continue;
+      if (!any) continue;
       const float old = exp2f(M - m);
       M = m;
       W *= old;
@@ -515,7 +517,7 @@ __global__ __launch_bounds__(256) void tree_parts_kernel(Args a) {
       for (int u = 0; u < U; ++u) {
         const float wgt = exp2f(l[u] - M);
         W += wgt;
-        if (wgt == 0.f) continue;      // of a part without keys
+        if (l[u] == -__builtin_inff()) continue;      // a part without keys
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           acc[j] += wgt * x[u][j];
@@ -526,14 +528,13 @@ __global__ __launch_bounds__(256) void tree_parts_kernel(Args a) {
     if constexpr (WAYS > 1) {
 #pragma unroll
       for (int o = L; o < L * WAYS; o <<= 1) {
-        const float other = __shfl_xor(M, o, 64), m = fmaxf(M, other);
-        const float mine = M == -__builtin_inff() ? 0.f : exp2f(M - m), theirs = other == -__builtin_inff() ? 0.f : exp2f(other - m);
-        const float w = __shfl_xor(W, o, 64);
+        const float other = __shfl_xor(M, o, 64), m = fmaxf(M, other), w = __shfl_xor(W, o, 64);
+        const float mine = W == 0.f ? 0.f : exp2f(M - m), theirs = w == 0.f ? 0.f : exp2f(other - m);      // zero: no keys
         W = W * mine + w * theirs;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float x = __shfl_xor(acc[j], o, 64);
-          acc[j] = (mine == 0.f ? 0.f : acc[j] * mine) + (theirs == 0.f ? 0.f : x * theirs);
+          acc[j] = acc[j] * mine + x * theirs;
         }
         M = m;
       }

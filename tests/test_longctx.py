@@ -628,6 +628,34 @@ def test_selected_prompts_large_scores_and_strides(dev):
         assert got.data_ptr() == out.data_ptr() and (out[:, 512:] == 5.0).all()
 
 
+@pytest.mark.parametrize("count,lens,nh", [(12, [500], 4), (200, [9000], 4), (700, [13000], 4), (90, [3000] * 8, 16)])
+def test_selected_what_is_no_number_stays(dev, count, lens, nh):
+    """A query that is no number, such a key among the first of a list that is empty behind it, and an infinite value that hardly counts, where lists
+    are cut and where they are not."""
+    q, k, v, tables, ctx, pages, seq = case = _selected_case(nh, 1, 64, 16, lens, count)
+    scale = 0.125
+    tol = _selected_want(nh, 1, scale, *case)[1]
+    q[0, 70] = math.nan                                # the second head
+    got = longctx.paged_selected(*(x.to(dev) for x in case[:6]), nh, 1, scale)
+    want, _ = _selected_want(nh, 1, scale, *case)
+    assert want[0, 64:128].isnan().all() and torch.equal(got.isnan().cpu(), want.isnan())
+    fin = want.isfinite()
+    _close(got.cpu()[fin], want[fin], tol[fin])
+    q[0, 70] = 1.0
+    full = pages.clone()
+    pages[0, 0, 1:] = -1
+    k[tables[0, pages[0, 0, 0]], 0, 5] = math.nan
+    assert longctx.paged_selected(*(x.to(dev) for x in case[:6]), nh, 1, scale)[0].isnan().all()
+    k[tables[0, pages[0, 0, 0]], 0, 5] = 0.0
+    pages.copy_(full)
+    at = tables[0, pages[0, 0, 0]]                     # keys far below the others: weights of nothing in 32 bits
+    q.abs_()
+    k[at] = -200.0
+    v[at, 0, 3, ::2] = math.inf
+    got = longctx.paged_selected(*(x.to(dev) for x in case[:6]), nh, 1, scale)[0].view(nh, 32, 2).cpu()
+    assert not got[..., 0].isfinite().any() and got[..., 1].isfinite().all()
+
+
 # ---- trees ------------------------------------------------------------------------------------------------------------------------------
 
 def _tree_case(nh, nkv, hd, page, ctx, nodes, seed=0, extra=0, behind=0):
@@ -796,6 +824,29 @@ def test_tree_many_sequences(dev, nh, nkv, hd):
 def test_tree_many_nodes(dev, nh, nkv, hd, nodes, page):
     """Trees of up to 1024 rows a kv head over contexts cut in parts."""
     _tree_check(dev, nh, nkv, _tree_case(nh, nkv, hd, page, [n + 700 * i + 33 for i, n in enumerate(nodes)], nodes, extra=8))
+
+
+@pytest.mark.parametrize("nh,nkv,hd,ctx,nodes", [(4, 1, 64, [5000], [6]), (4, 1, 64, [9000, 300], [3, 8]), (8, 2, 64, [200], [6]), (16, 1, 128, [20000], [60])])
+def test_tree_what_is_no_number_stays(dev, nh, nkv, hd, ctx, nodes):
+    """A query that is no number, an infinite value that hardly counts, a key of the context's beginning that is no number."""
+    q, k, v, tables, cu, ctx, mask = case = _tree_case(nh, nkv, hd, 16, ctx, nodes)
+    most = max(nodes)
+    call = lambda: longctx.paged_tree(*(x.to(dev) for x in case), nh, nkv, 0.125, max_nodes=most).cpu()
+    clean = call()
+    q[2, hd + 3] = math.nan
+    got = call()
+    assert got[2, hd: 2 * hd].isnan().all()
+    got[2, hd: 2 * hd] = clean[2, hd: 2 * hd]
+    assert torch.equal(got, clean)                     # nothing else
+    q[2, hd + 3] = 1.0
+    q.abs_()
+    k[tables[0, 1]] = -200.0                           # keys far below the others: weights of nothing in 32 bits
+    v[tables[0, 1], :, 3, ::2] = math.inf
+    got = call()[: nodes[0]].view(nodes[0], nh, hd // 2, 2)
+    assert not got[..., 0].isfinite().any() and got[..., 1].isfinite().all()
+    k[tables[0, 0], :, 2] = math.nan
+    got = call()
+    assert got[: nodes[0]].isnan().all() and got[nodes[0]:].isfinite().all()
 
 
 @pytest.mark.parametrize("nh,nkv,hd", [(32, 2, 64), (16, 2, 256)])
@@ -1355,6 +1406,12 @@ def test_woods_places(woods, test, args):
 @pytest.mark.parametrize("nh,nkv,hd,page", [(8, 2, 64, 16), (16, 1, 128, 16), (8, 2, 64, 4), (8, 2, 64, 128)])
 def test_woods_pages_that_are_not_there(woods, nh, nkv, hd, page):
     test_tree_pages_that_are_not_there("cuda", nh, nkv, hd, page)
+
+
+@gpu
+@pytest.mark.parametrize("nh,nkv,hd,ctx,nodes", [(4, 1, 64, [5000], [6]), (8, 2, 64, [200], [6]), (16, 1, 128, [900, 9000], [60, 7])])
+def test_woods_what_is_no_number_stays(woods, nh, nkv, hd, ctx, nodes):
+    test_tree_what_is_no_number_stays("cuda", nh, nkv, hd, ctx, nodes)
 
 
 @gpu
