@@ -177,7 +177,7 @@ __global__ __launch_bounds__(NT) void tree_rows_kernel(Args a) {
       unsigned odd = 0;
       if (!full) {
         // Values of keys that are not there are zeros.  Values of the tree's keys that are infinite or no numbers reach the rows that see
-        // them alone, but zero times such a value is no number: they are taken out here and added below where the weight is not zero.
+        // them alone, but zero times such a value is no number: they are taken out here and added below for the rows that see them.
 #pragma unroll
         for (int i = 0; i < VCH / 2; ++i) {
           const int tok = 32 * t + i * R + lane / VCH;
@@ -258,12 +258,14 @@ __global__ __launch_bounds__(NT) void tree_rows_kernel(Args a) {
         const uint16_t* vp = a.v + row_of(32 * t + kk, there) * HD + 4 * g;
         const uint32_t two = __shfl(j & 4 ? (j & 2 ? pf[3] : pf[2]) : (j & 2 ? pf[1] : pf[0]), 16 * (kk >> 2 & 3) + qi, 64);
         const float p = __uint_as_float(j & 1 ? two & 0xffff0000u : two << 16);
+        const int node = at + 32 * t + kk - tree_key;
+        const bool sees = node < 0 || (bits >> node & 1);
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const uint16_t x = vp[16 * c + i];
-            if ((x & 0x7f80) == 0x7f80 && p != 0.f) o[c][i] += p * bf16_to_f32(x);
+            if (sees && (x & 0x7f80) == 0x7f80) o[c][i] += p * bf16_to_f32(x);
           }
       }
     };

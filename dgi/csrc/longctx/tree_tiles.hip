@@ -295,8 +295,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_tiles_kernel(Args a) {
     } else if (kb0 + KT < kv_end) load_part(kb0 + KT, 1 - stage, id);
     id = read_id(kb0 + 2 * KT);
     // Values of the tree's keys that are infinite or no numbers reach the rows that see them alone, and those that stand for keys that are
-    // not there reach none, but zero times such a value is no number: they are taken out of the tile here and added below where the weight
-    // is not zero.
+    // not there reach none, but zero times such a value is no number: they are taken out of the tile here and added below for the rows that
+    // see them.
     unsigned long long odd = 0;
     if (kb0 + KT > tree_key || bad) {
       // a wave looks at the rows that it staged; row r of the tile is bit r
@@ -424,13 +424,15 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_tiles_kernel(Args a) {
       for (int i = 0; i < 32; ++i)
         if (i == ((kk >> 5) << 4 | (kk >> 3 & 3) << 2 | (kk & 3))) p = sc[i >> 4][i & 15];
       p = __shfl(p, lr + 32 * (kk >> 2 & 1), 64);
-      const uint16_t* vp = a.v + ((size_t)known(bt[key >> a.bs_log2]) * nkv + kvh) * head_stride + (size_t)(key & (bs - 1)) * HD;
+      const int id = bt[key >> a.bs_log2], node = key - tree_key;
+      const bool sees = known(id) == id && (node < 0 || (tmask >> node & 1));
+      const uint16_t* vp = a.v + ((size_t)known(id) * nkv + kvh) * head_stride + (size_t)(key & (bs - 1)) * HD;
 #pragma unroll
       for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const uint16_t x = vp[32 * d + 8 * (i >> 2) + 4 * hh + (i & 3)];
-          if ((x & 0x7f80) == 0x7f80 && p != 0.f) o[d][i] += p * bf16_to_f32(x);
+          if (sees && (x & 0x7f80) == 0x7f80) o[d][i] += p * bf16_to_f32(x);
         }
     }
   };

@@ -849,6 +849,20 @@ def test_tree_what_is_no_number_stays(dev, nh, nkv, hd, ctx, nodes):
     assert got[: nodes[0]].isnan().all() and got[nodes[0]:].isfinite().all()
 
 
+@pytest.mark.parametrize("nh,nkv,hd,nodes", [(4, 1, 64, 6), (8, 2, 128, 33), (4, 2, 256, 5)])
+def test_tree_own_values_that_hardly_count(dev, nh, nkv, hd, nodes):
+    """An infinite value of a node whose score leaves it a weight of nothing in 32 bits: no row that sees it is finite, all others are."""
+    q, k, v, tables, cu, ctx, mask = case = _tree_case(nh, nkv, hd, 16, [200], [nodes])
+    q.abs_()
+    at = 200 - nodes + 1
+    k[tables[0, at // 16], :, at % 16] = -200.0
+    v[tables[0, at // 16], :, at % 16, ::2] = math.inf
+    got = longctx.paged_tree(*(x.to(dev) for x in case), nh, nkv, 0.125).cpu().view(nodes, nh, hd // 2, 2)
+    sees = (mask[0, :nodes] >> 1 & 1).bool()
+    assert sees.any() and not sees.all()
+    assert not got[sees][..., 0].isfinite().any() and got[~sees].isfinite().all() and got[..., 1].isfinite().all()
+
+
 @pytest.mark.parametrize("nh,nkv,hd", [(32, 2, 64), (16, 2, 256)])
 @pytest.mark.parametrize("scale", [-0.25, 1e-30, 4.0])
 def test_tree_scales(dev, nh, nkv, hd, scale):
@@ -1412,6 +1426,12 @@ def test_woods_pages_that_are_not_there(woods, nh, nkv, hd, page):
 @pytest.mark.parametrize("nh,nkv,hd,ctx,nodes", [(4, 1, 64, [5000], [6]), (8, 2, 64, [200], [6]), (16, 1, 128, [900, 9000], [60, 7])])
 def test_woods_what_is_no_number_stays(woods, nh, nkv, hd, ctx, nodes):
     test_tree_what_is_no_number_stays("cuda", nh, nkv, hd, ctx, nodes)
+
+
+@gpu
+@pytest.mark.parametrize("nh,nkv,hd,nodes", [(4, 1, 64, 6), (8, 2, 128, 33)])
+def test_woods_own_values_that_hardly_count(woods, nh, nkv, hd, nodes):
+    test_tree_own_values_that_hardly_count("cuda", nh, nkv, hd, nodes)
 
 
 @gpu
