@@ -184,7 +184,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_tiles_kernel(Args a) {
   const unsigned long long tmask = row_valid ? a.mask[(size_t)seq * a.mask_stride + node] : 0;
 
   constexpr int NS = HD / 16, ND = HD / 32, CH = HD / 8;
-  const float scale = fmaxf(fabsf(a.scale_log2), 1e-30f);
+  const float scale = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
   float m_run = -1e30f, l_run = 0.f;
   f32x16 o[ND];
 #pragma unroll
@@ -264,10 +264,16 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_tiles_kernel(Args a) {
     } else load_part(kv_begin, 0, id);
     id = read_id(kv_begin + KT);
   }
-  // the softmax takes maxima of raw scores: a negative scale is the query's sign, zero stays above it (unseen keys are -inf)
-  if (a.scale_log2 < 0.f) {
+  // the softmax takes maxima of raw scores, and unseen keys are -inf: a negative scale is the query's sign, zero a query of zeros (no number
+  // where it is infinite or none)
+  if (a.scale_log2 <= 0.f) {
 #pragma unroll
-    for (int s = 0; s < NS; ++s) qf[s] ^= 0x80008000u;
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t x = qf[s][j], none = ((x & 0x7f80u) == 0x7f80u ? 0x7fc0u : 0u) | ((x & 0x7f800000u) == 0x7f800000u ? 0x7fc00000u : 0u);
+        qf[s][j] = a.scale_log2 == 0.f ? none : x ^ 0x80008000u;
+      }
   }
   // LDS addresses of this lane's operands in stage 0: keys lr, dims 16 s + 8 hh ..; values of dims 32 d .., keys 4 hh + tq
   typedef __attribute__((address_space(3))) const char* lds_at;

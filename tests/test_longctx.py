@@ -878,6 +878,24 @@ def test_tree_scores_without_a_scale(dev, nh, nkv):
     _close(got, want, tol)
 
 
+@pytest.mark.parametrize("nh,nkv", [(32, 2), (8, 2)])
+@pytest.mark.parametrize("scale", [0.0, 2.0 ** -108, -(2.0 ** -110)])
+def test_tree_large_scores_and_scales_of_nothing(dev, nh, nkv, scale):
+    """Scores up to 2^112 before scales that are zero or bring them to the ordinary."""
+    q, k, v, tables, cu, ctx, mask = case = _tree_case(nh, nkv, 64, 16, [300, 40], [24, 40])
+    q.mul_(2.0 ** 60)
+    k.mul_(2.0 ** 46)
+    got = longctx.paged_tree(*(x.to(dev) for x in case), nh, nkv, scale)
+    want, tol = _tree_want(nh, nkv, scale, *case)
+    _close(got, want, tol)
+    clean = got.cpu()
+    q[3, 70], q[5, 2] = math.nan, math.inf             # a head of two rows
+    got = longctx.paged_tree(*(x.to(dev) for x in case), nh, nkv, scale).cpu()
+    assert got[3, 64:128].isnan().all() and got[5, :64].isnan().all()
+    got[3, 64:128], got[5, :64] = clean[3, 64:128], clean[5, :64]
+    assert torch.equal(got, clean)                     # nothing else
+
+
 @pytest.mark.parametrize("nh,nkv", [(32, 2), (4, 2)])
 def test_tree_rows_without_keys(dev, nh, nkv):
     """A tree whose sequence has no context, one whose nodes see nothing and have no prefix, one with fewer keys than nodes; no page is there."""
@@ -1432,6 +1450,12 @@ def test_woods_what_is_no_number_stays(woods, nh, nkv, hd, ctx, nodes):
 @pytest.mark.parametrize("nh,nkv,hd,nodes", [(4, 1, 64, 6), (8, 2, 128, 33)])
 def test_woods_own_values_that_hardly_count(woods, nh, nkv, hd, nodes):
     test_tree_own_values_that_hardly_count("cuda", nh, nkv, hd, nodes)
+
+
+@gpu
+@pytest.mark.parametrize("scale", [0.0, 2.0 ** -108, -(2.0 ** -110)])
+def test_woods_large_scores_and_scales_of_nothing(woods, scale):
+    test_tree_large_scores_and_scales_of_nothing("cuda", 32, 2, scale)
 
 
 @gpu
