@@ -374,13 +374,13 @@ __global__ __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) void page_screen_kerne
 // them from `ahead`.
 struct Long {
   u64 lo[kWaves], hi[kWaves];
-  int hist[256];
+  alignas(16) int hist[256];      // read four at a time
   int eq[kWaves], kept[kWaves], digit, above, in;
 };
 
 struct Shared {
   u64 lo[kWaves], hi[kWaves];
-  int hist[3][256];
+  alignas(16) int hist[3][256];
   int eq[32][kWaves], kept[32][kWaves];
   Long any;
 };
@@ -647,7 +647,8 @@ __global__ __launch_bounds__(kThreads) void pick_screened_kernel(Args a) {
   constexpr int N = 64 * W;
   typedef Screened<R, W> S;
   extern __shared__ __attribute__((aligned(16))) double wgt_s[];      // 2 hd a row: of lo, of hi
-  __shared__ __attribute__((aligned(16))) S teams[kWaves / W];
+  __shared__ S teams[kWaves / W];
+  static_assert(alignof(S) >= 16 && offsetof(S, any.hist) % 16 == 0, "each team's counts are read 16 bytes at a time");
   const int team = __builtin_amdgcn_readfirstlane(threadIdx.x / N), tid = threadIdx.x % N;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int item = blockIdx.x * (kWaves / W) + team, t = item / a.nkv, h = item - t * a.nkv, G = a.nh / a.nkv;
@@ -855,7 +856,7 @@ __global__ __launch_bounds__(kThreads) void pick_pages_kernel(Args a) {
   for (int i = tid; i < a.recent; i += kThreads) out[a.count - a.recent + i] = end + i;
   if (need == 0) return;
   out += a.first;
-  __shared__ __attribute__((aligned(16))) Shared sh;
+  __shared__ Shared sh;
   if (end - begin <= 2 * kThreads) return pick<2>(keys, ahead, begin, end, need, out, sh);
   if (end - begin <= 4 * kThreads) return pick<4>(keys, ahead, begin, end, need, out, sh);
   if constexpr (MOST > 4) {
