@@ -6,8 +6,8 @@
 // A workgroup owns the G heads of a kv head for one row or, where rows of one sequence follow each other, for as many of them as
 // make 16 query columns: neighbours of a prompt mostly select the same pages, which are then read once, and the columns of the matrix
 // instruction are used.  It reads the union of their lists (made by a launch of its own, a bit per page and row in LDS), each column
-// masked to its own row's.  Its waves take tiles of 32 keys in turn and are merged through LDS; lists are cut between workgroups where
-// rows are few, and added up by a second launch.
+// masked to its own row's.  Its waves take tiles of 32 keys in turn and are merged through LDS; where rows are few, each is by itself, and its
+// list is cut between workgroups, whose sums a second launch adds up.
 //
 // Scores are formed transposed, S^T = K Q^T, so that a lane owns a query column and the weights stay in the registers that the product
 // O^T += V^T P^T takes them from.  Weights are rounded to bf16 for that product (as the cached values are; their sum is taken before),
@@ -162,7 +162,7 @@ __global__ __launch_bounds__(THREADS) void selected_plan_kernel(Args a, int n_bi
   }
 }
 
-// PLAN: rows that go together and their list come from the launch before; otherwise each row is by itself.
+// PLAN: rows that go together and their list, which is not cut, come from the launch before; otherwise each row is by itself.
 template <int HD, bool WIDE, bool PLAN>
 __global__ __launch_bounds__(NT, HD == 256 ? 1 : 2) void selected_kernel(Args a) {
   constexpr int KS = HD / 32, NC = HD / 16, VCH = HD / 8;
@@ -181,7 +181,7 @@ __global__ __launch_bounds__(NT, HD == 256 ? 1 : 2) void selected_kernel(Args a)
     m = a.plan_rows[t0];
     if (m == 0) return;
   }
-  const int split = blockIdx.y, tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, qi = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, qi = lane & 15, g = lane >> 4;
   uint16_t* vt = reinterpret_cast<uint16_t*>(smem + w * wave_lds<HD>());
 
   const int seq = a.row_seq ? a.row_seq[t0] : t0;
@@ -206,7 +206,8 @@ __global__ __launch_bounds__(NT, HD == 256 ? 1 : 2) void selected_kernel(Args a)
   most = __builtin_amdgcn_readfirstlane(most);      // lane 0's column is live
   if constexpr (!PLAN) least = most;
   const int total = PLAN ? a.plan_total[t0 * a.nkv + h] : a.count;
-  const int part = (total + a.splits - 1) / a.splits, lo = split * part, hi = most > 0 ? min(lo + part, total) : lo;
+  const int splits = PLAN ? 1 : a.splits, split = PLAN ? 0 : blockIdx.y;
+  const int part = (total + splits - 1) / splits, lo = split * part, hi = most > 0 ? min(lo + part, total) : lo;
   const int4* planned = PLAN ? a.plan + (size_t)t0 * a.nkv * a.count + (size_t)h * m * a.count : nullptr;
 
   // where the lane's chunk of row i 64 / VCH + lane / VCH goes in LDS: the same for every P-th i, but for whole rows
@@ -435,13 +436,13 @@ __global__ __launch_bounds__(NT, HD == 256 ? 1 : 2) void selected_kernel(Args a)
 #pragma unroll
       for (int i = 0; i < 4; ++i) odd = odd || !(fabsf(acc[i]) < __builtin_inff());
       const int head_at = h * G + col - row * G;
-      if (a.splits == 1) {
+      if (splits == 1) {
         uint2 r;
         r.x = pack_bf16x2(acc[0], acc[1]);
         r.y = pack_bf16x2(acc[2], acc[3]);
         *reinterpret_cast<uint2*>(a.out + (size_t)(t0 + row) * a.out_stride + head_at * HD + 4 * d) = r;
       } else {
-        const size_t slab = (((size_t)(t0 + row) * a.nkv + h) * a.splits + split) * G + col - row * G;
+        const size_t slab = (((size_t)(t0 + row) * a.nkv + h) * splits + split) * G + col - row * G;
         *reinterpret_cast<f32x4*>(a.part_o + slab * HD + 4 * d) = acc;
         if (d == 0) a.part_l[slab] = L == 0.f ? -__builtin_inff() : M + __builtin_amdgcn_logf(L);
       }
@@ -504,9 +505,8 @@ int launch(const Args& a, hipStream_t s) {
     if ((long long)side * a.count <= 1024) selected_plan_kernel<64><<<a.nkv * rows, 64, lds, s>>>(a, n_bits);
     else selected_plan_kernel<NT><<<a.nkv * rows, NT, lds, s>>>(a, n_bits);
     DGI_CHECK_LAUNCH();
-    const dim3 grid(a.nkv * rows, a.splits);
-    if (a.bs_log2 >= 4) selected_kernel<HD, true, true><<<grid, NT, 0, s>>>(a);
-    else selected_kernel<HD, false, true><<<grid, NT, 0, s>>>(a);
+    if (a.bs_log2 >= 4) selected_kernel<HD, true, true><<<a.nkv * rows, NT, 0, s>>>(a);
+    else selected_kernel<HD, false, true><<<a.nkv * rows, NT, 0, s>>>(a);
   } else {
     const dim3 grid(a.nkv * a.rows, a.splits);
     if (a.bs_log2 >= 4) selected_kernel<HD, true, false><<<grid, NT, 0, s>>>(a);
@@ -527,6 +527,7 @@ extern "C" int dgi_paged_selected(const void* q, long long q_stride, const void*
                                   void* out, long long out_stride, float* part_o, float* part_l, int splits, void* plan, int* plan_total,
                                   int* plan_rows, int T, int nh, int nkv, int hd, int block_size, float scale, hipStream_t s) {
   if (T == 0) return 0;
+  if (splits < 1 || (plan && splits > 1)) return -5;      // lists of rows that go together are not cut
   Args a{(const uint16_t*)q, q_stride, (const uint16_t*)k, (const uint16_t*)v, tables, table_stride, table_cols, n_seqs, num_blocks, T, ctx,
          row_seq, pages, count, (uint16_t*)out, out_stride, part_o, part_l, splits, nh, nkv, 0, scale * 1.4426950408889634f,
          (int4*)plan, plan_total, plan_rows};

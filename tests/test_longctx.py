@@ -15,6 +15,7 @@ import subprocess
 import pytest
 import torch
 
+import dgi.build
 from dgi import ops
 from dgi.ops import longctx
 
@@ -654,6 +655,15 @@ def test_selected_what_is_no_number_stays(dev, count, lens, nh):
     v[at, 0, 3, ::2] = math.inf
     got = longctx.paged_selected(*(x.to(dev) for x in case[:6]), nh, 1, scale)[0].view(nh, 32, 2).cpu()
     assert not got[..., 0].isfinite().any() and got[..., 1].isfinite().all()
+
+
+def test_selected_lists_that_go_together_are_not_cut():
+    """The entry refuses it before any launch, and the rule never asks for it: rows go together from 1024 (row, kv head) pairs on, lists are cut up to
+    160 of them."""
+    lib, at, n = ctypes.CDLL(dgi.build.build(group="longctx")), ctypes.c_void_p(4096), ctypes.c_longlong
+    call = lambda plan, splits: lib.dgi_paged_selected(at, n(512), at, at, at, 4, 4, 1, 4, at, at, at, 4, at, n(512), at, at, splits, plan, plan, plan, 4,  # noqa: E731
+                                                       8, 2, 64, 16, ctypes.c_float(0.1), None)
+    assert call(at, 2) == -5 and call(at, 0) == -5 and call(None, 0) == -5
 
 
 # ---- trees ------------------------------------------------------------------------------------------------------------------------------
