@@ -247,23 +247,28 @@ void paged_selected(at::Tensor out, const at::Tensor& q, const at::Tensor& k, co
   const bool one = keys < 1024 || (units > 64 && keys < 8192) || units > 160;
   const int64_t splits = one ? 1 : runs_of(units, keys, (count + least - 1) / least, 16);
   const Parts parts(splits > 1 ? T * nh * splits : 0, at_.hd, q);
+  auto run = [&](int64_t t0, int64_t n, void* plan, int* plan_total, int* plan_rows) {
+    const auto from = [&](const at::Tensor& t) { return static_cast<char*>(t.data_ptr()) + t0 * t.stride(0) * t.element_size(); };
+    check_rc(dgi_paged_selected(from(q), q.stride(0), k.data_ptr(), v.data_ptr(), tables.data_ptr<int>(), (int)tables.stride(0),
+                                (int)tables.size(1), (int)tables.size(0), (int)k.size(0), ctx.data_ptr<int>() + t0, rows ? rows + t0 : nullptr,
+                                pages.data_ptr<int>() + t0 * nkv * count, (int)count, from(out), out.stride(0), parts.o, parts.l, (int)splits, plan,
+                                plan_total, plan_rows, (int)n, (int)nh, (int)nkv, (int)at_.hd, (int)at_.page, (float)scale, cur_stream()), op);
+  };
   // More rows than sequences, and enough of them to take the launch that makes the unions and still fill the card: neighbours read their
   // pages together, 16 / heads of a group at a time.  Each by itself / together, us, lists of 64 pages drawn at random, half alike, alike:
   // 128 rows of 32 heads on 8 of 128 dims 32, 40, 30, 19; 512 103, 91, 67, 41; 256 of 16 on 4 of 256 dims 86, 74, 54, 32, but 128 of them 44, 72, 53, 31;
   // two at a time, 256 rows of 28 on 4 31, 37, 33, 25; 512 57, 62, 54, 39; 2048 of 8 on one of 64 dims 31, 40, 36, 27.
-  at::Tensor plan;
-  int* plan_n = nullptr;
   const int64_t side = 16 * nkv / nh;
   if (rows && T > tables.size(0) && side >= 2 && T * nkv * std::min<int64_t>(at_.hd, 128) >= (side >= 4 ? 1 : 2) * 131072) {
-    const int64_t pairs = T * nkv * count * 2, numbers = T * (nkv + 1);
-    plan = at::empty({pairs + (numbers + 1) / 2}, q.options().dtype(at::kLong));
-    plan_n = reinterpret_cast<int*>(plan.data_ptr<int64_t>() + pairs);
+    // unions of as many rows at a time (by 16) as 256 MB hold
+    const int64_t at_once = std::min(T, 16 * std::max<int64_t>((1 << 28) / (16 * nkv * count * 16), 1));
+    const int64_t entries = at_once * nkv * count * 2, numbers = at_once * (nkv + 1);
+    const at::Tensor plan = at::empty({entries + (numbers + 1) / 2}, q.options().dtype(at::kLong));
+    int* plan_n = reinterpret_cast<int*>(plan.data_ptr<int64_t>() + entries);
+    for (int64_t t0 = 0; t0 < T; t0 += at_once) run(t0, std::min(at_once, T - t0), plan.data_ptr(), plan_n, plan_n + at_once * nkv);
+  } else {
+    run(0, T, nullptr, nullptr, nullptr);
   }
-  check_rc(dgi_paged_selected(q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(), tables.data_ptr<int>(), (int)tables.stride(0),
-                              (int)tables.size(1), (int)tables.size(0), (int)k.size(0), ctx.data_ptr<int>(), rows, pages.data_ptr<int>(),
-                              (int)count, out.data_ptr(), out.stride(0), parts.o, parts.l, (int)splits,
-                              plan_n ? plan.data_ptr() : nullptr, plan_n, plan_n ? plan_n + T * nkv : nullptr, (int)T, (int)nh, (int)nkv,
-                              (int)at_.hd, (int)at_.page, (float)scale, cur_stream()), op);
 }
 
 void paged_tree(at::Tensor out, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& tables,

@@ -1387,6 +1387,30 @@ def test_many_rows_as_one_by_one(nh, nkv, hd, T, pages):
     _close(got[some], want, tol)
 
 
+@gpu
+def test_selected_long_lists_of_many_rows():
+    """Unions of so many rows that they are made for some of them at a time: no more memory than that, and rows on both sides of the border."""
+    longctx.load_native(required=True)
+    g, T, count = _gen(12), 5000, 512
+    q, k, v, tables, _, _, _ = _selected_case(16, 8, 64, 16, [16 * 600], 1)
+    q = _randn(g, T, 16 * 64)
+    ctx = 16 * 600 - torch.randint(0, 200, (T,), generator=g).to(I32)
+    pages = torch.full((T, 8, count), -1, dtype=I32)
+    pages[:, :, 100:140] = torch.stack([torch.randperm(600, generator=g)[:40] for _ in range(T)]).to(I32)[:, None]
+    seq = torch.zeros(T, dtype=I32)
+    dev = [x.cuda() for x in (q, k, v, tables, ctx, pages)]
+    seq_dev, out = seq.cuda(), torch.empty(T, 16 * 64, dtype=BF16, device="cuda")
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    longctx.paged_selected(*dev, 16, 8, 0.125, row_seq=seq_dev, out=out)
+    assert torch.cuda.max_memory_allocated() - before <= 260 << 20
+    some = [0, 1, 7, 8, 4080, 4095, 4096, 4097, 4103, 4111, 4999]
+    want, tol = _selected_want(16, 8, 0.125, q[some], k, v, tables, ctx[some], pages[some], seq[some])
+    _close(out[some], want, tol)
+
+
 @pytest.fixture
 def woods(monkeypatch):
     """Before and behind the sequences of every call as many without nodes as make the kernels take a sequence's pairs as tiles."""
