@@ -217,7 +217,9 @@ __global__ __launch_bounds__(kThreads) void page_scores_alone_kernel(Args a) {
 // Rows that go together: 16 x 16 (rows, pages) at a time, 32 channels an instruction, in fewer bits than the choice needs: a weight w
 // is the sum of two bf16 numbers to |w| 2^-16, their products with the bounds are exact in 32 bits, and each of the 4 HD additions is
 // off by no more than two steps of the last place, 2^-22 of S = sum |w| |bound| (all 256 of a chain together: 2^-20.8 of S at the worst, of half a
-// million with exponents spread over 2 to 40); G heads are added up for a weight, each to 2^-24.  A third
+// million with exponents spread over 2 to 40); G heads are added up for a weight, each to 2^-24.  Small weights lose no more: queries are
+// multiples of 2^-133, the last place of subnormal bf16 numbers, and so are their sums and what is left of them, so that a second number
+// below 2^-126 is exact, and the matrix cores take subnormal numbers as they are.  A third
 // product gives S (of the weights' first numbers, no less than 1 - 2^-8 of it).  Written are the score and, for a wave's pages of a
 // row, the largest error; what no such bound holds for (infinite or no numbers) is written as none.
 // A lane has row lane % 16's weights and page lane % 16's bounds of the chunks 4 j + lane / 16 of [lo | hi], eight values each.

@@ -395,6 +395,15 @@ def test_select_prompts_that_need_every_bit(dev, what, hd, pages):
             assert got[t, h].tolist() == [0] + sorted(best) + [n - 2, n - 1]
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("q_exp,b_exp", [(-122, 40), (-127, 60), (-112, 0), (60, -130), (100, -128)])
+def test_select_prompts_of_the_least_numbers(dev, hd, q_exp, b_exp):
+    """Weights whose lower bits, or bounds that are subnormal, against large ones."""
+    q, b, tables, ctx, seq = _select_case(4, 2, hd, 4, [1200], 33)
+    q, b = (q.double() * 2.0 ** q_exp).to(BF16), (b.double() * 2.0 ** b_exp).to(BF16)
+    _select_check(dev, 4, 2, 4, 24, 1, 2, q, b, tables, ctx, seq)
+
+
 @pytest.mark.parametrize("hd,pages", [(64, 200), (256, 1000), (128, 1090), (64, 5000), (128, 8300), (256, 9000)])
 def test_select_rows_of_long_prompts(dev, hd, pages):
     _select_check(dev, 3, 1, 2, 50, 2, 3, *_select_case(3, 1, hd, 2, [2 * pages], 18))
@@ -1325,6 +1334,13 @@ def test_crowd_select_rows_of_prompts(crowd, rows, page, extra):
 @pytest.mark.parametrize("hd,pages", [(64, 300), (128, 200), (128, 1300), (256, 250)])
 def test_crowd_select_every_bit(crowd, what, hd, pages):
     test_select_prompts_that_need_every_bit("cuda", what, hd, pages)
+
+
+@gpu
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("q_exp,b_exp", [(-122, 40), (-127, 60), (-112, 0), (60, -130), (100, -128)])
+def test_crowd_select_the_least_numbers(crowd, hd, q_exp, b_exp):
+    test_select_prompts_of_the_least_numbers("cuda", hd, q_exp, b_exp)
 
 
 @gpu
