@@ -156,9 +156,10 @@ void select_pages(at::Tensor out, const at::Tensor& q, const at::Tensor& bounds,
   const char* op = "select_pages";
   const at::Device dev = q.device();
   TORCH_CHECK_VALUE(bounds.dim() == 4, op, ": bounds must be contiguous [blocks, kv heads, 2, dims]");
-  const int64_t hd = bounds.size(3), T = q.size(0);
+  const int64_t hd = bounds.size(3);
   check_heads(nh, nkv, hd, op);
   check_rows(q, nh * hd, dev, op, "q");
+  const int64_t T = q.size(0);
   check_bounds(bounds, nkv, hd, dev, op);
   check_tables(tables, dev, op);
   check_int(ctx, dev, at::kInt, op, "context_lens");

@@ -88,7 +88,7 @@ def _check_attention(op, q, k_cache, v_cache, block_tables, nh, nkv, out):
     _check_heads(op, nh, nkv)
     _need(k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.shape[1] == nkv and k_cache.is_contiguous()
           and v_cache.is_contiguous(), op, "k_cache and v_cache must be contiguous [blocks, kv heads, block size, dims]")
-    _need(k_cache.shape[2] & (k_cache.shape[2] - 1) == 0, op, "pages of a power of two")
+    _need(k_cache.shape[0] > 0 and k_cache.shape[2] > 0 and k_cache.shape[2] & (k_cache.shape[2] - 1) == 0, op, "pages of a power of two")
     _check_rows(op, q, nh * k_cache.shape[3], "q")
     _check_ints(op, block_tables, torch.int32, "block_tables")
     _need(block_tables.dim() == 2, op, "block_tables must be [sequences, pages]")
@@ -148,6 +148,7 @@ def rope_cache_bounds(qkv, positions, cos_sin, nh: int, nkv: int, hd: int, slot_
     _check_ints(op, positions, torch.int32, "positions", qkv.shape[0])
     _check_ints(op, slot_mapping, torch.int32, "slot_mapping", qkv.shape[0])
     _need(mode in (0, 1), op, "mode is 0 (halves) or 1 (interleaved pairs)")
+    _need(cos_sin.dim() == 2 and cos_sin.shape[0] > 0, op, "cos_sin must be [positions, rotated dims]")
     rd = cos_sin.shape[1]
     _need(0 < rd <= hd and rd % (8 if mode else 16) == 0, op, "rotated dims must be a multiple of 16 (mode 1: 8) and at most the head's")
     _need(out is None or (out.is_contiguous() and out.shape == (qkv.shape[0], nh * hd)), op, "out must be contiguous [rows, heads * dims]")

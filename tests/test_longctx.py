@@ -1089,6 +1089,27 @@ def test_refusals(dev):
     refused(f, *case, 8, 3, 0.125)
 
 
+def test_refusals_of_dimensions(dev):
+    """Tensors of fewer dimensions than an argument has, and caches without pages or tokens."""
+    qkv, pos, cs, slots, k, v, b = _append_case(dev, 8, 2, 64, 64, 0, 16, [(3, 5)])
+    one = torch.zeros(1, dtype=I32, device=dev)
+    none = torch.zeros(0, 2, 16, 64, dtype=BF16, device=dev), torch.zeros(4, 2, 0, 64, dtype=BF16, device=dev)
+    calls = [lambda: longctx.rope_cache_bounds(qkv, pos, cs[0].contiguous(), 8, 2, 64, slots, k, v, b),
+             lambda: longctx.rope_cache_bounds(qkv, pos, cs[:0], 8, 2, 64, slots, k, v, b),
+             lambda: longctx.rope_cache_bounds(qkv[0], pos, cs, 8, 2, 64, slots, k, v, b)]
+    for q in (qkv[0, 0], qkv[0]):
+        calls += [lambda q=q: longctx.select_pages(q, b, one[None], one, 8, 2, 16, 4),
+                  lambda q=q: longctx.select_pages(q, b, one[None], one, 8, 2, 16, 4, out=torch.zeros(1, 2, 4, dtype=I32, device=dev)),
+                  lambda q=q: longctx.paged_selected(q, k, v, one[None], one, one[None, None], 8, 2, 0.125),
+                  lambda q=q: longctx.paged_tree(q, k, v, one[None], torch.cat([one, one]), one, one[None].long(), 8, 2, 0.125, max_nodes=1)]
+    for c in none:
+        calls += [lambda c=c: longctx.paged_selected(qkv[:1], c, c, one[None], one, one[None, None].expand(1, 2, 1).contiguous(), 8, 2, 0.125),
+                  lambda c=c: longctx.paged_tree(qkv[:1], c, c, one[None], torch.cat([one, one + 1]), one, one[None].long(), 8, 2, 0.125, max_nodes=1)]
+    for call in calls:
+        with pytest.raises(ValueError):
+            call()
+
+
 @gpu
 def test_refusals_of_the_kernels():
     """What only the kernels cannot take: other types and head sizes, starts off 16 bytes, tensors of other devices."""
