@@ -21,6 +21,7 @@ using namespace dgi::prefill;
 namespace {
 
 constexpr int kRows = 128, kWaves = 4;      // rows of a workgroup
+constexpr float kLowest = -__FLT_MAX__;     // maximum of no key
 
 struct Args {
   const uint16_t* q;
@@ -185,7 +186,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_tiles_kernel(Args a) {
 
   constexpr int NS = HD / 16, ND = HD / 32, CH = HD / 8;
   const float scale = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
-  float m_run = -1e30f, l_run = 0.f;
+  float m_run = kLowest, l_run = 0.f;
+  bool huge = false;      // the wave's maxima
   f32x16 o[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d)
@@ -395,11 +397,25 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_tiles_kernel(Args a) {
 #pragma unroll
       for (int d = 0; d < ND; ++d) o[d] *= alpha;
       m_run = m_new;
+      huge = __any(fabsf(m_run) > 0x1p24f && m_run != kLowest);
+    }
+    // A score's product with the scale is not rounded before the maximum, which is, is taken off: where half a last place of that is much, the
+    // difference is made ahead.
+    const float scale_now = huge ? 1.f : scale, m_now = huge ? 0.f : m_run;
+    if (huge) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float x = sc[kb][i] * scale;
+          asm("" : "+v"(x));
+          sc[kb][i] = x - m_run;
+        }
     }
     float ps[4];
     u32x4 pf;
     auto weight = [&](int kb, int i) __attribute__((always_inline)) {
-      sc[kb][i] = __builtin_amdgcn_exp2f(sc[kb][i] * scale - m_run);
+      sc[kb][i] = __builtin_amdgcn_exp2f(sc[kb][i] * scale_now - m_now);
       ps[i & 3] = kb == 0 && i < 4 ? sc[kb][i] : ps[i & 3] + sc[kb][i];
     };
 #pragma unroll

@@ -915,6 +915,36 @@ def test_tree_large_scores_and_scales_of_nothing(dev, nh, nkv, scale):
     assert torch.equal(got, clean)                     # nothing else
 
 
+@pytest.mark.parametrize("nh,nkv,ctx,nodes", [(32, 2, [300, 40], [24, 40]), (8, 2, [300, 40], [24, 40]), (4, 1, [5000], [6]), (16, 1, [9000], [64])])
+@pytest.mark.parametrize("signs", [1, -1])
+@pytest.mark.parametrize("exp", [26, 34, 60, 105])
+def test_tree_scores_of_any_size(dev, nh, nkv, ctx, nodes, signs, exp):
+    """Scores around 2^exp, or all below -2^exp: a row's weight is its best key's wherever the next one is behind by more than the error of both."""
+    q, k, v, tables, cu, ctx, mask = case = _tree_case(nh, nkv, 64, 16, ctx, nodes)
+    if signs < 0:
+        q.abs_()
+        k.copy_(-k.abs())
+    q.mul_(2.0 ** (exp // 2))
+    k.mul_(2.0 ** (exp - exp // 2))
+    got = longctx.paged_tree(*(x.to(dev) for x in case), nh, nkv, 0.125).cpu().view(-1, nkv, nh // nkv, 64)
+    told = 0
+    for s, (c, n) in enumerate(zip(ctx.tolist(), nodes)):
+        ids = tables[s, : -(-c // 16)].long()
+        for h in range(nkv):
+            kk, vv = (x[ids, h].reshape(-1, 64)[:c].double() for x in (k, v))
+            for a in range(n):
+                row = int(cu[s]) + a
+                see = torch.tensor([j < c - n or bool(int(mask[s, a]) >> (j - c + n) & 1) for j in range(c)])
+                x = q[row].double().view(nkv, -1, 64)[h]
+                score = (x @ kk.t() * 0.125).masked_fill(~see, -math.inf)
+                error = 68 * U24 * 0.125 * (x.abs() @ kk.abs().t()).amax(1)
+                best = score.topk(2, 1)
+                clear = best.values[:, 0] - best.values[:, 1] > 2 * error + 100
+                assert torch.equal(got[row, h][clear].double(), vv[best.indices[clear, 0]])
+                told += int(clear.sum())
+    assert told > 0.9 * sum(nodes) * nh and got.isfinite().all()
+
+
 @pytest.mark.parametrize("nh,nkv", [(32, 2), (4, 2)])
 def test_tree_rows_without_keys(dev, nh, nkv):
     """A tree whose sequence has no context, one whose nodes see nothing and have no prefix, one with fewer keys than nodes; no page is there."""
@@ -1527,6 +1557,14 @@ def test_woods_own_values_that_hardly_count(woods, nh, nkv, hd, nodes):
 @pytest.mark.parametrize("scale", [0.0, 2.0 ** -108, -(2.0 ** -110)])
 def test_woods_large_scores_and_scales_of_nothing(woods, scale):
     test_tree_large_scores_and_scales_of_nothing("cuda", 32, 2, scale)
+
+
+@gpu
+@pytest.mark.parametrize("signs", [1, -1])
+@pytest.mark.parametrize("exp", [26, 34, 60, 105])
+def test_woods_scores_of_any_size(woods, signs, exp):
+    test_tree_scores_of_any_size("cuda", 32, 2, [300, 40], [24, 40], signs, exp)
+    test_tree_scores_of_any_size("cuda", 16, 1, [3000], [64], signs, exp)
 
 
 @gpu
