@@ -290,7 +290,8 @@ void paged_tree(at::Tensor out, const at::Tensor& q, const at::Tensor& k, const 
   // Columns of 16 pairs a workgroup (tree_rows) or row tiles of 128 (tree_tiles): by the workgroups of the first and the keys that all of them
   // read, weighed by how full the tiles would be.  us of both, 32 heads on 8 of 128 dims: one sequence of 32 nodes, 300 keys 11.5, 18.2, 4000
   // 18.9, 21.1, of 64, 8000 keys 38.5, 35.3; 16 of 16, 1000 22.9, 35.9, 4000 59.9, 61.2; 64 heads: 8 of 16, 1000 22.9, 35.9, 4000 60.5,
-  // 48.1; 32 of 32, 1000 136, 55; 14 heads on 2 of 64 dims: 8 of 64, 1000 15.4, 26.7, 4000 39.2, 34.0.
+  // 48.1; 32 of 32, 1000 136, 55; 14 heads on 2 of 64 dims: 8 of 64, 1000 15.4, 26.7, 4000 39.2, 34.0.  The tables were as wide as the contexts:
+  // the host does not know these, and a wider table counts as its width.
   const int64_t G = nh / nkv, width = tables.size(1) * at_.page, pairs = max_nodes * G, cols = (pairs + 15) / 16, tiles = (pairs + 127) / 128;
   const int64_t few = S * nkv * cols;
   if (pairs > 32 && at_.hd <= 128 && !(few <= 1024 && few * (width + 100) * cols <= 6400000 * tiles)) {

@@ -5,8 +5,9 @@
 // nothing, so they are exact whatever the order, and a page's bounds can go on from step to step.  A value that is no number makes its
 // channel's bounds no number (minimum / maximum of IEEE 754-2019).
 //
-// Bound by bytes: the append reads a row's q | k | v once and writes it once (4115 rows of 64 heads on 8 of 128, 172 MB: 43.7 us, 3.9 TB/s;
-// one row: 3.7 us, a launch), the rebuilding reads the keys once (16384 pages of 16 keys, 8 heads of 128, 604 MB: 131 us, 4.6 TB/s).
+// Bound by bytes: the append reads a row's q | k | v once and writes it once (4115 rows of 64 heads on 8 of 128, 172 MB: 45 us, 3.8 TB/s;
+// one row: 4.0 us, a launch), the rebuilding reads the keys once (16384 pages of 16 keys, 8 heads of 128, 604 MB: 132 us, 4.6 TB/s, where a
+// kernel that only reads reaches 6.4).
 #include "../common.h"
 #include "page_runs.h"
 

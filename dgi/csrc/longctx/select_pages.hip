@@ -8,12 +8,12 @@
 // What they are compared by goes into a workspace [T, n_kv, pages], and another launch chooses.
 //
 // Decode rows each have bounds of their own: the scores in 64 bits as a lane multiplies what it loads, as integers of the same order, whose
-// digits from the top are counted until the threshold is found.  What bounds this is the bounds' bytes (64 rows over 4000 to 32000 keys,
-// 8 kv heads of 128, 303 MB: 72 us at 4.2 TB/s, and 7 us for the choice).
+// digits from the top are counted until the threshold is found.  What bounds this are the loads of the bounds (64 rows over 4000 to 32000 keys,
+// 8 kv heads of 128, 303 MB: 71 us at 4.3 TB/s, where a kernel that only reads reaches 6.3, and 7 us for the choice).
 //
 // Rows of a prompt share their sequence's bounds: 16 of them are the rows of bf16 matrix instructions, which give each score in 32 bits and
 // a bound for its error; pages that the error leaves open are scored in 64 bits (1018 rows of 28 heads over 730 to 1000 pages of 4 kv heads
-// of 128: 55 us, of which scores 31, looking for rows that do not go together 4, the choice 21; with the products in 64 bits on the matrix
+// of 128: 53 us, of which scores 30, looking for rows that do not go together 4, the choice 21; with the products in 64 bits on the matrix
 // cores, whose rate alone is 24 us, 88 us).  What bounds this is latency: of the weights ahead of 4 steps of 64 pages, and of the choice.
 #include "../common.h"
 
@@ -905,7 +905,9 @@ extern "C" int dgi_select_pages(const void* q, long long q_stride, const void* b
   // Rows in groups only if there are more than sequences (else hardly two of one), and where that saves more than the third launch and the
   // second look at some pages take, about 9 us.  Row by row / in groups, us: 32 rows of 8 heads of 128 over 500 pages 16.8, 18.3, over
   // 1000 22.9, 21.2; 64 over 100 13.6, 15.5, over 500 22.9, 19.3; 128 over 100 17.2, 15.7, over 1000 53, 30; 64 rows of 4 heads over 500
-  // 17.3, 19.2; 512 rows of one head of 64 over 500 15.8, 18.4, over 1000 21.1, 21.2; 128 rows of 2 heads of 256 over 500 23.9, 24.4.
+  // 17.3, 19.2; 512 rows of one head of 64 over 500 15.8, 18.4, over 1000 21.1, 21.2; 128 rows of 2 heads of 256 over 500 23.9, 24.4.  The tables
+  // were as wide as the contexts: how long these are the host does not know, and a wider table counts as its width, here and in the keys of a
+  // lane below (1018 rows of 28 heads on 4 over 730 to 1000 pages 53, of a table of 8192 columns 87).
   const int span = table_cols - first - recent;
   const bool groups = row_seq && T > n_seqs && (double)T * nkv * (span + 40) * min(hd, 128) >= 18e6;
   for (int t0 = 0; t0 < T; t0 += key_rows) {

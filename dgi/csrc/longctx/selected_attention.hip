@@ -15,7 +15,7 @@
 // through LDS: operands of the key product loaded as they are needed touch every line twice, 64 bytes at a time.
 //
 // Decode rows are bound by the bytes of their pages: 64 rows of 64 heads on 8, 128 pages of 16 keys each, 97 us, 5.5 TB/s.  Rows of
-// prompts by the path from the L2 to a compute unit's registers: 2 x 509 rows of 28 heads on 4, 64 pages each, 100 us, 1.5 GB of keys
+// prompts by the path from the L2 to a compute unit's registers: 2 x 509 rows of 28 heads on 4, 64 pages each, 97 us, 1.5 GB of keys
 // and values where row by row it is 2.1 GB (205 us; together with key operands straight from memory 133; without the loads 70).
 // Three workgroups a compute unit spill registers (104).
 #include "../common.h"

@@ -10,7 +10,7 @@
 // another, are dealt out in equal shares, so that a long context beside short ones does not hold up the launch; what a share's ends
 // cut is added up by a second launch.
 //
-// 16 trees of 60 nodes, 64 heads on 8, 1000 to 8000 keys: 175 us, 632 TF/s of 111 Gflop (with workgroups by sequence and run of
+// 16 trees of 60 nodes, 64 heads on 8, 1000 to 8000 keys: 174 us, 636 TF/s of 111 Gflop (with workgroups by sequence and run of
 // its keys instead of equal shares, 260).  A tile takes 2.0 us for the two workgroups of a compute unit, 1070 TF/s; the rest is the
 // beginning and end of the two parts that a share has (20 us) and the second launch (10 us).
 #include "../prefill_attention_kernel.h"
@@ -491,7 +491,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void tree_tiles_kernel(Args a) {
 }
 
 // The parts of a sequence's row tile that several shares have, weighed by their sums: HD / 8 lanes a row, several parts under way.  Two rows
-// one after another (16 trees of 60 nodes, 64 heads on 8, 1000 to 8000 keys, all launches: 175 us; one row and eight parts at a time: 182), or,
+// one after another (16 trees of 60 nodes, 64 heads on 8, 1000 to 8000 keys, all launches: 174 us; one row and eight parts at a time: 182), or,
 // where a row has eight parts and more, four groups of lanes a row, a quarter of its parts each (one tree of 64 nodes, 32 heads on 8, 8000 keys: 33 us,
 // not 43; but 6 of 49 over 290, with five parts, 34, not 25).
 template <int HD, int WAYS>
